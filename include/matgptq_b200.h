@@ -269,11 +269,68 @@ int matgptq_b200_causal_mask(const int64_t *positions, void *mask, int64_t seq, 
 int matgptq_b200_argmax(const void *logits, int64_t *out, int64_t rows, int64_t cols, uint32_t flags, void *stream);
 
 /*
+ * A key/value cache in 4 bits, its writing, attention over it, thinning it out and reading it back.  The reference keeps its cache
+ * in 16 bits and leaves it to vLLM / transformers.  Everything is device memory of the caller.  T is fp16, or bf16 with FLAG_BF16.
+ *   k_codes [batch, n_kv_heads, capacity, head_dim/2] bytes: byte i holds channels 2i (low half) and 2i + 1
+ *   v_codes [batch, n_kv_heads, capacity/2, head_dim] bytes: the rows of entries 2p and 2p + 1, in turns of two bytes
+ *   params  [batch, n_kv_heads, capacity, 4] T: scale and minimum of K, scale and minimum of V
+ * A code c stands for minimum + scale * c.  head_dim is 64 or 128, capacity a multiple of 64, batch * n_kv_heads at most 65535, the
+ * three pointers 16-byte aligned.
+ * lengths[batch] (int32) counts the entries of each sequence, the tokens of the call among them: token i of `seq` is entry
+ * lengths[b] - seq + i.  Where that is negative the token is padding (a prompt padded on the left): nothing is read or written for
+ * it and its results are zeros.  A length past the capacity, or a position outside the tables, leaves 106 in
+ * matgptq_b200_device_status; nothing outside the buffers is touched.  A length below zero counts as zero.
+ */
+typedef struct {
+  void *k_codes, *v_codes, *params;
+  int64_t batch, n_kv_heads, head_dim, capacity;
+} matgptq_b200_kv4_cache;
+
+/*
+ * qkv[batch, seq, (n_heads + 2 n_kv_heads) * head_dim] -> q_out[batch, seq, n_heads, head_dim], rotated; the new entries, k rotated:
+ * scale = T((max - min) / 15) over a row, code = min(15, rint((x - min) / scale)) of the values rounded to T.  Rotation as
+ * matgptq_b200_rope_kv (pairs 2i, 2i + 1); cos and sin are [n_positions, head_dim/2] fp32, token i of sequence b is at
+ * positions[b * position_stride + i] (stride 0: the same for all sequences).  A row with an infinity or a NaN (or a range beyond
+ * fp32) reads back as NaN, as does a token whose position is outside the tables.
+ */
+int matgptq_b200_append_kv4(const matgptq_b200_kv4_cache *cache, const void *qkv, const int64_t *positions, int64_t position_stride,
+                            const float *cos_table, const float *sin_table, int64_t n_positions, const int32_t *lengths, void *q_out,
+                            int64_t seq, int64_t n_heads, uint32_t flags, void *stream);
+
+/*
+ * out[batch, seq, n_heads, head_dim] = softmax(scale * q . K) V for q of that shape, over the entries that a query sees: query i is
+ * entry p = lengths[b] - seq + i itself and sees entry j when j <= p and (window == 0, or j > p - window, or j < sinks).  Window
+ * and sinks count entries.  A query that sees nothing gives zeros.  Head h reads key/value head h / (n_heads / n_kv_heads).
+ * With weights[batch, n_kv_heads, capacity] (fp32, may be NULL) each entry's softmax weights, summed over the queries and heads that
+ * share it, are added to what is there, in a fixed order; this needs matgptq_b200_attention_kv4_workspace_bytes(...) bytes of
+ * workspace (its contents do not matter; one per call in flight).  K and V are not rounded; sums are fp32.
+ */
+int64_t matgptq_b200_attention_kv4_workspace_bytes(int64_t batch, int64_t seq, int64_t n_heads, int with_weights);
+int matgptq_b200_attention_kv4(const matgptq_b200_kv4_cache *cache, const void *q, int64_t seq, int64_t n_heads, const int32_t *lengths,
+                               int64_t window, int64_t sinks, float scale, float *weights, void *out, void *workspace,
+                               int64_t workspace_bytes, uint32_t flags, void *stream);
+
+/*
+ * Cuts every sequence of more than keep + slack entries back to `keep`: its first `sinks`, its last `recent`, and of the others, head
+ * by head, those with the largest weights (ties: the lowest entry; a NaN counts as the largest).  They keep their order and move to
+ * the front, their weights with them; the weights of the entries given up are set to 0, the codes behind the last entry are left.
+ *   new_lengths[batch]            lengths afterwards; must not be `lengths`
+ *   kept[batch, n_kv_heads, keep] the entries that stayed, by their old index; -1 throughout for a sequence that was not cut
+ */
+int matgptq_b200_evict_kv4(const matgptq_b200_kv4_cache *cache, float *weights, const int32_t *lengths, int64_t keep, int64_t slack,
+                           int64_t sinks, int64_t recent, int32_t *new_lengths, int32_t *kept, uint32_t flags, void *stream);
+
+/* The last `count` entries of every sequence as dense k_out, v_out[batch, n_kv_heads, count, head_dim] of type T; zeros in front
+ * where a sequence has fewer. */
+int matgptq_b200_dequantize_kv4(const matgptq_b200_kv4_cache *cache, const int32_t *lengths, int64_t count, void *k_out, void *v_out,
+                                uint32_t flags, void *stream);
+
+/*
  * Waits inside the kernels (on asynchronous copies) are bounded: a kernel that gives
  * up records a non-zero code instead of hanging, and its output is then undefined.
  * This call synchronises with the device, returns the first code recorded on the
  * current device since the last reset (0 = none; 101 weight copy, 102 activation
- * copy, 103 tensor-core completion, 105 a peer rank's partial sums) and clears it when reset != 0.  The reference has
+ * copy, 103 tensor-core completion, 105 a peer rank's partial sums, 106 a length or position outside a 4-bit cache) and clears it when reset != 0.  The reference has
  * no counterpart: its only error path is exit(1) in CHECK_CUDA (csrc/include/common.cuh:44-51).
  */
 int matgptq_b200_device_status(int *status_out, int reset);

@@ -35,6 +35,12 @@ class Comm(ctypes.Structure):
                 ("slot_elems", ctypes.c_int64), ("rank", ctypes.c_int), ("nranks", ctypes.c_int), ("push_only", ctypes.c_int)]
 
 
+class Kv4Cache(ctypes.Structure):
+    """``matgptq_b200_kv4_cache`` of the C header: a key/value cache in 4 bits."""
+    _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("params", ctypes.c_void_p), ("batch", ctypes.c_int64),
+                ("n_kv_heads", ctypes.c_int64), ("head_dim", ctypes.c_int64), ("capacity", ctypes.c_int64)]
+
+
 # symbol -> (restype, argtypes); must list every function declared in include/matgptq_b200.h
 SIGNATURES = {
     "matgptq_b200_version": (_c_int, []),
@@ -53,6 +59,11 @@ SIGNATURES = {
     "matgptq_b200_causal_mask": (_c_int, [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_u32, _c_ptr]),
     "matgptq_b200_argmax": (_c_int, [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_u32, _c_ptr]),
     "matgptq_b200_silu_mul": (_c_int, [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_u32, _c_ptr]),
+    "matgptq_b200_append_kv4": (_c_int, [ctypes.POINTER(Kv4Cache), _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_u32, _c_ptr]),
+    "matgptq_b200_attention_kv4_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_int]),
+    "matgptq_b200_attention_kv4": (_c_int, [ctypes.POINTER(Kv4Cache), _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, ctypes.c_float, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_u32, _c_ptr]),
+    "matgptq_b200_evict_kv4": (_c_int, [ctypes.POINTER(Kv4Cache), _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_u32, _c_ptr]),
+    "matgptq_b200_dequantize_kv4": (_c_int, [ctypes.POINTER(Kv4Cache), _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_u32, _c_ptr]),
     "matgptq_b200_slice": (_c_int, [_c_ptr, _c_ptr, _c_i64, _c_int, _c_int, _c_ptr]),
     "matgptq_b200_pack_qweights": (_c_int, [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_int, _c_int, _c_ptr]),
     "matgptq_b200_pack_qweights_host": (_c_int, [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_int, _c_int]),

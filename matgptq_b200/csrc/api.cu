@@ -33,10 +33,10 @@ int matgptq_b200_version(void) { return 100; }
 const char *matgptq_b200_strerror(int status) {
   switch (status) {
     case MG_OK: return "ok";
-    case MG_ERR_BAD_ARG: return "bad argument (bitwidth must be 2,3,4,6,8; group size -1,32,128; N % 16 == 0; K % 64 == 0; non-null pointers)";
+    case MG_ERR_BAD_ARG: return "bad argument (bitwidth must be 2,3,4,6,8; group size -1,32,128; N % 16 == 0; K % 64 == 0; cache capacity % 64 == 0; non-null pointers)";
     case MG_ERR_CUDA: return "CUDA runtime call or kernel launch failed";
     case MG_ERR_UNSUPPORTED:
-      return "unsupported: K must be a multiple of 128, or the forced kernel does not take this shape or scratch size";
+      return "unsupported: K must be a multiple of 128, the head dimension of a 4-bit cache 64 or 128, or the kernel does not take this shape or scratch size";
     case MG_ERR_ALIGNMENT: return "pointer is not 16-byte aligned";
     case MATGPTQ_B200_ERR_SCRATCH_TOO_SMALL:
       return "this shape needs more split-K scratch than the built-in array holds: pass scratch through matgptq_b200_matmul_ws";
@@ -363,7 +363,14 @@ int matgptq_b200_device_status(int *status_out, int reset) {
   int e = 0;
   r = mg::selftest_device_status(&e, reset);
   if (r != MG_OK) return r;
-  if (status_out) *status_out = a ? a : (b ? b : (d ? d : (f ? f : e)));
+  int k = 0;
+  r = mg::kv4_device_status(&k, reset);
+  if (r != MG_OK) return r;
+  int k2 = 0;
+  r = mg::kv4_attention_device_status(&k2, reset);
+  if (r != MG_OK) return r;
+  if (k == 0) k = k2;
+  if (status_out) *status_out = a ? a : (b ? b : (d ? d : (f ? f : (k ? k : e))));
   return MG_OK;
 }
 

@@ -1,0 +1,416 @@
+// The key/value cache in 4 bits (layout: kv4.cuh): writing entries, reading them back, thinning the cache out.  Attention over it
+// is in kv4_attention.cu.  The reference keeps its cache in 16 bits and leaves it to vLLM / transformers.
+#include <cuda_runtime.h>
+
+#include <cfloat>
+#include <initializer_list>
+
+#include "../../include/matgptq_b200.h"
+#include "async.cuh"
+#include "helper_kernels.cuh"
+#include "kernels.h"
+#include "kv4.cuh"
+
+namespace mg {
+
+MG_DEFINE_STATUS_ACCESSOR(kv4_device_status)
+
+// ---- writing ----------------------------------------------------------------------------------------------------------
+//
+// One row (a token's head) per d/8 lanes, eight channels a lane.  q and k are turned by the angles of the token's position in
+// pairs (2i, 2i + 1) and rounded to fp32, then to the model's type; k (rounded) and v are then quantised:
+//   scale = T((max - min) / 15),  code = min(15, rint((x - min) / scale))
+// with fp32 differences and quotients, each rounded once.  A code is the nearest one for the scale as it is kept.
+// A row with an infinity, a NaN or a range beyond fp32 gets a NaN for its scale, so that what reads it comes out as NaN.
+// Bound by memory for prompts (reads 2 bytes and writes 2 or 0.5 bytes per element), by latency for single tokens.
+// x a + y b rounded to fp32 and then to T, as if computed without any other error: a code next to a border, and with the smallest
+// value of a row all of its codes, would go by the last bit.  The fp32 result is off by less than `off`; where that leaves T in doubt
+// (one value in 2000 in fp16, one in 16000 in bf16) 64 bits decide.
+template <typename T> __device__ __forceinline__ T turned(float x, float a, float y, float b) {
+  const float product = __fmul_rn(y, b), r = __fmaf_rn(x, a, product);
+  const float off = __fmaf_rn(0x1p-23f, fabsf(r), __fmaf_rn(0x1p-23f, fabsf(product), FLT_MIN));
+  const T low = from_f<T>(r - off), high = from_f<T>(r + off);
+  if (*reinterpret_cast<const uint16_t *>(&low) == *reinterpret_cast<const uint16_t *>(&high)) return low;
+  return from_f<T>(static_cast<float>(static_cast<double>(x) * a + static_cast<double>(y) * b));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) append_kv4_kernel(const T *__restrict__ qkv, const long long *__restrict__ positions,
+                                                         long long position_stride, const float *__restrict__ cos_t,
+                                                         const float *__restrict__ sin_t, long long n_positions,
+                                                         const int *__restrict__ lengths, T *__restrict__ q_out, Kv4Cache cache, int seq,
+                                                         int heads) {
+  pdl_prologue();
+  const int lanes = cache.dim >> 3;  // of a row: 8 or 16
+  const int all = heads + 2 * cache.kv_heads;
+  const long long rows = static_cast<long long>(cache.batch) * seq * all;
+  const long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) / lanes;
+  const int c0 = (threadIdx.x & (lanes - 1)) * 8;
+  const bool live = row < rows;
+  const long long safe = live ? row : 0;
+  const int head = static_cast<int>(safe % all);
+  const long long token = safe / all;
+  const int b = static_cast<int>(token / seq), s = static_cast<int>(token - static_cast<long long>(b) * seq);
+  const long long slot = static_cast<long long>(lengths[b]) - seq + s;
+  const bool padding = slot < 0;
+  bool outside = !padding && slot >= cache.capacity;
+
+  uint4 raw = make_uint4(0, 0, 0, 0);
+  if (live && !padding) raw = *reinterpret_cast<const uint4 *>(qkv + (token * all + head) * cache.dim + c0);
+  T *e = reinterpret_cast<T *>(&raw);
+  if (head < heads + cache.kv_heads && live && !padding) {
+    const long long pos = positions[b * position_stride + s];
+    if (pos < 0 || pos >= n_positions) {
+      outside = true;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = from_f<T>(NAN);
+    } else {
+      const float4 cs = *reinterpret_cast<const float4 *>(cos_t + pos * (cache.dim >> 1) + (c0 >> 1));
+      const float4 sn = *reinterpret_cast<const float4 *>(sin_t + pos * (cache.dim >> 1) + (c0 >> 1));
+      const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const float x = to_f(e[2 * p]), y = to_f(e[2 * p + 1]);
+        e[2 * p] = turned<T>(x, cv[p], y, -sv[p]);
+        e[2 * p + 1] = turned<T>(y, cv[p], x, sv[p]);
+      }
+    }
+  }
+  if (outside) report_status(kStatusCacheRange);
+
+  float x[8], low = FLT_MAX, high = -FLT_MAX;
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = to_f(e[i]);
+    odd |= !(fabsf(x[i]) <= FLT_MAX);
+    low = fminf(low, x[i]);
+    high = fmaxf(high, x[i]);
+  }
+  if (odd) high = INFINITY;
+  for (int off = lanes >> 1; off >= 1; off >>= 1) {  // whole warps come here: rows of one warp differ, lanes of one row do not
+    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, off));
+    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, off));
+  }
+  if (!live) return;
+  if (head < heads) {
+    *reinterpret_cast<uint4 *>(q_out + (token * heads + head) * cache.dim + c0) = raw;
+    return;
+  }
+  if (padding || slot >= cache.capacity) return;
+  const float range = __fsub_rn(high, low);
+  const T scale16 = from_f<T>(range <= FLT_MAX ? __fdiv_rn(range, 15.f) : NAN);
+  const float scale = to_f(scale16);
+  uint32_t word = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float c = scale > 0.f ? fminf(15.f, rintf(__fdiv_rn(__fsub_rn(x[i], low), scale))) : 0.f;
+    word |= static_cast<uint32_t>(c) << (4 * i);
+  }
+  const bool is_v = head >= heads + cache.kv_heads;
+  const size_t entry = (static_cast<size_t>(b) * cache.kv_heads + (head - heads - (is_v ? cache.kv_heads : 0))) * cache.capacity + slot;
+  if (is_v) {
+    uint16_t *units = reinterpret_cast<uint16_t *>(cache.v + (entry >> 1) * cache.dim) + (entry & 1) + (c0 >> 1);
+    units[0] = static_cast<uint16_t>(word);
+    units[2] = static_cast<uint16_t>(word >> 16);
+  } else {
+    *reinterpret_cast<uint32_t *>(cache.k + entry * (cache.dim >> 1) + (c0 >> 1)) = word;
+  }
+  if (c0 == 0) {
+    const T low16 = from_f<T>(low);
+    const uint32_t both = static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(&scale16)) |
+                          static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(&low16)) << 16;
+    *reinterpret_cast<uint32_t *>(cache.params + entry * 4 + (is_v ? 2 : 0)) = both;
+  }
+}
+
+// ---- reading back -----------------------------------------------------------------------------------------------------
+//
+// The last `count` entries of every sequence as dense rows of the model's type, zeros in front where a sequence has fewer: eight
+// channels of one entry's K and V a thread.  One multiply-add in fp32 (the product is exact: 4 bits x 11) and one rounding.
+// Bound by memory: 4 d bytes written for d + 8 read.
+template <typename T>
+__global__ void __launch_bounds__(256) dequantize_kv4_kernel(Kv4Cache cache, const int *__restrict__ lengths, int count, T *__restrict__ k_out,
+                                                             T *__restrict__ v_out) {
+  pdl_prologue();
+  const int lanes = cache.dim >> 3;
+  const long long rows = static_cast<long long>(cache.batch) * cache.kv_heads * count;
+  const long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) / lanes;
+  if (row >= rows) return;
+  const int c0 = (threadIdx.x & (lanes - 1)) * 8;
+  const long long bh = row / count;
+  const int i = static_cast<int>(row - bh * count), b = static_cast<int>(bh / cache.kv_heads);
+  const int slot = kv4_length(lengths, b, cache.capacity) - count + i;
+  uint4 k4 = make_uint4(0, 0, 0, 0), v4 = k4;
+  if (slot >= 0) {
+    const size_t entry = static_cast<size_t>(bh) * cache.capacity + slot;
+    const uint32_t kw = *reinterpret_cast<const uint32_t *>(cache.k + entry * (cache.dim >> 1) + (c0 >> 1));
+    const uint16_t *units = reinterpret_cast<const uint16_t *>(cache.v + (entry >> 1) * cache.dim) + (entry & 1) + (c0 >> 1);
+    const uint32_t vw = units[0] | static_cast<uint32_t>(units[2]) << 16;
+    const uint2 p = *reinterpret_cast<const uint2 *>(cache.params + entry * 4);
+    const float ks = kv4_to_f<T>(static_cast<uint16_t>(p.x)), kl = kv4_to_f<T>(static_cast<uint16_t>(p.x >> 16));
+    const float vs = kv4_to_f<T>(static_cast<uint16_t>(p.y)), vl = kv4_to_f<T>(static_cast<uint16_t>(p.y >> 16));
+    T *ke = reinterpret_cast<T *>(&k4), *ve = reinterpret_cast<T *>(&v4);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      ke[c] = from_f<T>(__fmaf_rn(ks, static_cast<float>((kw >> (4 * c)) & 15u), kl));
+      ve[c] = from_f<T>(__fmaf_rn(vs, static_cast<float>((vw >> (4 * c)) & 15u), vl));
+    }
+  }
+  *reinterpret_cast<uint4 *>(k_out + row * cache.dim + c0) = k4;
+  *reinterpret_cast<uint4 *>(v_out + row * cache.dim + c0) = v4;
+}
+
+// ---- thinning out -----------------------------------------------------------------------------------------------------
+//
+// A sequence of more than keep + slack entries is cut back to `keep`: its first `sinks`, its last `recent`, and of the others the
+// ones with the largest weights, ties to the lowest index, all in their order.  evict_kv4_select_kernel, a CTA per sequence and
+// head, finds the smallest weight that stays by four passes over the weights' bits (8 at a time, from the top), writes the indices
+// that stay and moves the weights; evict_kv4_move_kernel moves codes and scales.
+constexpr int kEvictThreads = 1024;
+
+// larger weights have larger keys; a NaN counts as the largest weight, -0 as 0
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  if (w != w) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(w + 0.f);
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+__global__ void __launch_bounds__(kEvictThreads, 1) evict_kv4_select_kernel(float *__restrict__ weights, const int *__restrict__ lengths,
+                                                                           int kv_heads, int capacity, int keep, int slack, int sinks,
+                                                                           int recent, int *__restrict__ new_lengths, int *__restrict__ kept) {
+  pdl_prologue();
+  const int bh = blockIdx.x, b = bh / kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int n = kv4_length(lengths, b, capacity);
+  const bool cut = n > static_cast<long long>(keep) + slack;
+  if (bh % kv_heads == 0 && tid == 0) new_lengths[b] = cut ? keep : n;
+  int *mine = kept + static_cast<size_t>(bh) * keep;
+  if (!cut) {
+    for (int i = tid; i < keep; i += kEvictThreads) mine[i] = -1;
+    return;
+  }
+  float *w = weights + static_cast<size_t>(bh) * capacity;
+  const int first = sinks, last = n - recent;  // those between compete
+  int want = keep - sinks - recent;            // places for them, fewer than there are
+  __shared__ int hist[256];
+  __shared__ uint32_t s_prefix;
+  __shared__ int s_want;
+  uint32_t prefix = 0;  // the top bits of the smallest key that stays
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    for (int i = tid; i < 256; i += kEvictThreads) hist[i] = 0;
+    __syncthreads();
+    for (int j = first + tid; j < last; j += kEvictThreads) {
+      const uint32_t key = weight_key(w[j]);
+      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1);
+    }
+    __syncthreads();
+    if (tid == 0) {
+      int above = 0, digit = 255;
+      for (; digit > 0 && above + hist[digit] < want; --digit) above += hist[digit];
+      s_prefix = prefix | static_cast<uint32_t>(digit) << shift;
+      s_want = want - above;
+    }
+    __syncthreads();
+    prefix = s_prefix;
+    want = s_want;
+  }
+  // `want` of the entries whose key is `prefix` stay, the first ones.  With no place at all (want == 0) none does, nor can a key
+  // be above it: the passes then end at the top digit of each.
+  const bool none = keep == sinks + recent;
+  __shared__ int s_equal[32], s_keep[32];
+  int equal_before = 0, keep_before = 0;
+  for (int base = 0; base < n; base += kEvictThreads) {
+    const int j = base + tid;
+    const float value = j < n ? w[j] : 0.f;
+    const bool fixed = j < n && (j < first || j >= last);
+    const bool rival = j < n && !fixed && !none;
+    const uint32_t key = weight_key(value);
+    const bool equal = rival && key == prefix;
+    const unsigned eq_mask = __ballot_sync(0xffffffffu, equal);
+    if (lane == 0) s_equal[warp] = __popc(eq_mask);
+    __syncthreads();
+    int eq_rank = equal_before + __popc(eq_mask & ((1u << lane) - 1));
+    int eq_total = 0;
+    for (int i = 0; i < 32; ++i) {
+      if (i < warp) eq_rank += s_equal[i];
+      eq_total += s_equal[i];
+    }
+    const bool stays = fixed || (rival && key > prefix) || (equal && eq_rank < want);
+    const unsigned mask = __ballot_sync(0xffffffffu, stays);
+    if (lane == 0) s_keep[warp] = __popc(mask);
+    __syncthreads();  // also: every weight of these 1024 has been read
+    int at = keep_before + __popc(mask & ((1u << lane) - 1));
+    int total = 0;
+    for (int i = 0; i < 32; ++i) {
+      if (i < warp) at += s_keep[i];
+      total += s_keep[i];
+    }
+    if (stays && at < keep) {
+      mine[at] = j;
+      w[at] = value;  // at <= j: behind what is still to be read
+    }
+    equal_before += eq_total;
+    keep_before += total;
+    __syncthreads();
+  }
+  for (int j = keep + tid; j < n; j += kEvictThreads) w[j] = 0.f;
+}
+
+// A CTA moves one column slice (32 bytes of the K rows, 32 bytes of the V pairs, or the params) of one sequence and head: entry
+// i comes from kept[i] >= i, and what a step reads is read before the step writes, so nothing is overwritten that is still needed.
+constexpr int kMoveThreads = 512;
+
+__global__ void __launch_bounds__(kMoveThreads) evict_kv4_move_kernel(Kv4Cache cache, const int *__restrict__ kept, int keep) {
+  pdl_prologue();
+  const int bh = blockIdx.y;
+  const int *src = kept + static_cast<size_t>(bh) * keep;
+  if (keep == 0 || src[0] < 0) return;  // not cut
+  const int k_slices = cache.dim / 64, v_slices = cache.dim / 32;
+  const int slice = blockIdx.x, tid = threadIdx.x;
+  const size_t first = static_cast<size_t>(bh) * cache.capacity;
+  if (slice < k_slices) {
+    const int row_bytes = cache.dim >> 1;
+    uint8_t *base = cache.k + first * row_bytes + slice * 32 + (tid & 1) * 16;
+    for (int i0 = 0; i0 < keep; i0 += kMoveThreads / 2) {
+      const int i = i0 + (tid >> 1);
+      const int from = i < keep ? src[i] : i;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (from != i) v = *reinterpret_cast<const uint4 *>(base + static_cast<size_t>(from) * row_bytes);
+      __syncthreads();
+      if (from != i) *reinterpret_cast<uint4 *>(base + static_cast<size_t>(i) * row_bytes) = v;
+    }
+  } else if (slice < k_slices + v_slices) {
+    // a pair at a time: each word takes the half of one entry's unit and the half of another's
+    uint8_t *base = cache.v + (first >> 1) * cache.dim + (slice - k_slices) * 32 + (tid & 1) * 16;
+    const int pairs = (keep + 1) >> 1;
+    for (int p0 = 0; p0 < pairs; p0 += kMoveThreads / 2) {
+      const int p = p0 + (tid >> 1);
+      const bool live = p < pairs;
+      const int a = live ? src[2 * p] : 0;
+      const int c = live && 2 * p + 1 < keep ? src[2 * p + 1] : 2 * p + 1;  // behind the last entry: as it was
+      const bool moves = live && (a != 2 * p || c != 2 * p + 1);
+      uint32_t out[4] = {0, 0, 0, 0};
+      if (moves) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(base + static_cast<size_t>(a >> 1) * cache.dim);
+        const uint4 y = *reinterpret_cast<const uint4 *>(base + static_cast<size_t>(c >> 1) * cache.dim);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+        const unsigned pick = (a & 1 ? 0x32u : 0x10u) | ((c & 1 ? 0x76u : 0x54u) << 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = __byte_perm(xs[i], ys[i], pick);
+      }
+      __syncthreads();
+      if (moves) *reinterpret_cast<uint4 *>(base + static_cast<size_t>(p) * cache.dim) = make_uint4(out[0], out[1], out[2], out[3]);
+    }
+  } else {
+    uint2 *base = reinterpret_cast<uint2 *>(cache.params) + first;
+    for (int i0 = 0; i0 < keep; i0 += kMoveThreads) {
+      const int i = i0 + tid;
+      const int from = i < keep ? src[i] : i;
+      uint2 v = make_uint2(0, 0);
+      if (from != i) v = base[from];
+      __syncthreads();
+      if (from != i) base[i] = v;
+    }
+  }
+}
+
+}  // namespace mg
+
+namespace mg {
+
+int kv4_check_cache(const matgptq_b200_kv4_cache *c) {
+  if (!c || !c->k_codes || !c->v_codes || !c->params) return MG_ERR_BAD_ARG;
+  if (c->batch < 0 || c->n_kv_heads <= 0 || c->n_kv_heads > (1 << 16) || c->capacity <= 0 || c->capacity > (1 << 30)) return MG_ERR_BAD_ARG;
+  if (c->capacity % 64 != 0) return MG_ERR_BAD_ARG;
+  if (c->batch > 65535 || c->batch * c->n_kv_heads > 65535) return MG_ERR_UNSUPPORTED;
+  if (c->head_dim != 64 && c->head_dim != 128) return MG_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(c->k_codes) | reinterpret_cast<uintptr_t>(c->v_codes) | reinterpret_cast<uintptr_t>(c->params)) % 16 != 0)
+    return MG_ERR_ALIGNMENT;
+  return MG_OK;
+}
+
+Kv4Cache kv4_cache(const matgptq_b200_kv4_cache *c) {
+  return Kv4Cache{static_cast<uint8_t *>(c->k_codes),       static_cast<uint8_t *>(c->v_codes), static_cast<uint16_t *>(c->params),
+                  static_cast<int>(c->batch),               static_cast<int>(c->n_kv_heads),    static_cast<int>(c->head_dim),
+                  static_cast<int>(c->capacity)};
+}
+
+}  // namespace mg
+
+namespace {
+
+using mg::Kv4Cache;
+
+bool misaligned(std::initializer_list<const void *> pointers) {
+  uintptr_t all = 0;
+  for (const void *p : pointers) all |= reinterpret_cast<uintptr_t>(p);
+  return all % 16 != 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int matgptq_b200_append_kv4(const matgptq_b200_kv4_cache *cache, const void *qkv, const int64_t *positions, int64_t position_stride,
+                            const float *cos_table, const float *sin_table, int64_t n_positions, const int32_t *lengths, void *q_out,
+                            int64_t seq, int64_t n_heads, uint32_t flags, void *stream) {
+  const int st = mg::kv4_check_cache(cache);
+  if (st != MG_OK) return st;
+  if (!qkv || !positions || !cos_table || !sin_table || !lengths || !q_out) return MG_ERR_BAD_ARG;
+  if (seq < 0 || seq > (1 << 30) || n_heads <= 0 || n_heads > (1 << 20) || n_positions <= 0 || position_stride < 0) return MG_ERR_BAD_ARG;
+  if (misaligned({qkv, cos_table, sin_table, q_out})) return MG_ERR_ALIGNMENT;
+  const Kv4Cache c = mg::kv4_cache(cache);
+  const long long threads = cache->batch * seq * (n_heads + 2 * cache->n_kv_heads) * (c.dim / 8);
+  if (threads == 0) return MG_OK;
+  if ((threads + 255) / 256 > INT32_MAX) return MG_ERR_UNSUPPORTED;
+  const auto go = [&](auto tag) {
+    using T = decltype(tag);
+    return mg::launch_helper(mg::append_kv4_kernel<T>, dim3(static_cast<unsigned>((threads + 255) / 256)), 256, static_cast<cudaStream_t>(stream),
+                             (flags & MATGPTQ_B200_FLAG_PDL) != 0, static_cast<const T *>(qkv), reinterpret_cast<const long long *>(positions),
+                             static_cast<long long>(position_stride), cos_table, sin_table, static_cast<long long>(n_positions),
+                             static_cast<const int *>(lengths), static_cast<T *>(q_out), c, static_cast<int>(seq), static_cast<int>(n_heads));
+  };
+  return (flags & MATGPTQ_B200_FLAG_BF16) ? go(__nv_bfloat16{}) : go(__half{});
+}
+
+int matgptq_b200_dequantize_kv4(const matgptq_b200_kv4_cache *cache, const int32_t *lengths, int64_t count, void *k_out, void *v_out,
+                                uint32_t flags, void *stream) {
+  const int st = mg::kv4_check_cache(cache);
+  if (st != MG_OK) return st;
+  if (!lengths || count < 0 || count > (1 << 30) || (count > 0 && (!k_out || !v_out))) return MG_ERR_BAD_ARG;
+  if (misaligned({k_out, v_out})) return MG_ERR_ALIGNMENT;
+  const Kv4Cache c = mg::kv4_cache(cache);
+  const long long threads = cache->batch * cache->n_kv_heads * count * (c.dim / 8);
+  if (threads == 0) return MG_OK;
+  if ((threads + 255) / 256 > INT32_MAX) return MG_ERR_UNSUPPORTED;
+  const auto go = [&](auto tag) {
+    using T = decltype(tag);
+    return mg::launch_helper(mg::dequantize_kv4_kernel<T>, dim3(static_cast<unsigned>((threads + 255) / 256)), 256,
+                             static_cast<cudaStream_t>(stream), (flags & MATGPTQ_B200_FLAG_PDL) != 0, c, static_cast<const int *>(lengths),
+                             static_cast<int>(count), static_cast<T *>(k_out), static_cast<T *>(v_out));
+  };
+  return (flags & MATGPTQ_B200_FLAG_BF16) ? go(__nv_bfloat16{}) : go(__half{});
+}
+
+int matgptq_b200_evict_kv4(const matgptq_b200_kv4_cache *cache, float *weights, const int32_t *lengths, int64_t keep, int64_t slack,
+                           int64_t sinks, int64_t recent, int32_t *new_lengths, int32_t *kept, uint32_t flags, void *stream) {
+  const int st = mg::kv4_check_cache(cache);
+  if (st != MG_OK) return st;
+  if (!weights || !lengths || !new_lengths || !kept || lengths == new_lengths) return MG_ERR_BAD_ARG;
+  if (keep <= 0 || keep > cache->capacity || slack < 0 || slack > cache->capacity || sinks < 0 || recent < 0 || sinks > keep ||
+      recent > keep - sinks)
+    return MG_ERR_BAD_ARG;
+  const Kv4Cache c = mg::kv4_cache(cache);
+  const unsigned bh = static_cast<unsigned>(cache->batch * cache->n_kv_heads);
+  if (bh == 0) return MG_OK;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  const bool pdl = (flags & MATGPTQ_B200_FLAG_PDL) != 0;
+  const int r = mg::launch_helper(mg::evict_kv4_select_kernel, dim3(bh), mg::kEvictThreads, cs, pdl, weights, static_cast<const int *>(lengths),
+                                  c.kv_heads, c.capacity, static_cast<int>(keep), static_cast<int>(slack), static_cast<int>(sinks),
+                                  static_cast<int>(recent), static_cast<int *>(new_lengths), static_cast<int *>(kept));
+  if (r != MG_OK) return r;
+  return mg::launch_helper(mg::evict_kv4_move_kernel, dim3(c.dim / 64 + c.dim / 32 + 1, bh), mg::kMoveThreads, cs, true, c,
+                           static_cast<const int *>(kept), static_cast<int>(keep));
+}
+
+}  // extern "C"

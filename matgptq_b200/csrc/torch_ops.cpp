@@ -42,6 +42,11 @@ struct Library {
   decltype(&matgptq_b200_pack_qweights) pack_qweights = nullptr;
   decltype(&matgptq_b200_reorder_scales) reorder_scales = nullptr;
   decltype(&matgptq_b200_dequantize) dequantize = nullptr;
+  decltype(&matgptq_b200_append_kv4) append_kv4 = nullptr;
+  decltype(&matgptq_b200_attention_kv4) attention_kv4 = nullptr;
+  decltype(&matgptq_b200_attention_kv4_workspace_bytes) attention_kv4_workspace_bytes = nullptr;
+  decltype(&matgptq_b200_evict_kv4) evict_kv4 = nullptr;
+  decltype(&matgptq_b200_dequantize_kv4) dequantize_kv4 = nullptr;
 };
 Library lib;  // filled once by bind() when the package is imported
 
@@ -285,6 +290,130 @@ Tensor matmul_zeros(const Tensor &input, const Tensor &weights, const Tensor &sc
   return out;
 }
 
+// ---- key/value cache in 4 bits ----------------------------------------------------------------------------------
+bool aligned16(const Tensor &t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
+
+// The cache's tensors against one another; what the C ABI sees are addresses and sizes.
+matgptq_b200_kv4_cache check_kv4(const char *what, const Tensor &k_codes, const Tensor &v_codes, const Tensor &params, const Tensor &lengths,
+                                 int64_t flags) {
+  TORCH_CHECK(k_codes.is_cuda(), what, ": expected k_codes to be a CUDA tensor");
+  for (const Tensor *t : {&v_codes, &params, &lengths})
+    TORCH_CHECK(t->is_cuda() && t->device() == k_codes.device(), what, ": k_codes, v_codes, params and lengths must be on the same GPU");
+  TORCH_CHECK(k_codes.scalar_type() == at::kByte && k_codes.dim() == 4, what, ": k_codes must be uint8 of shape (B, KV, capacity, d/2)");
+  const int64_t b = k_codes.size(0), kv = k_codes.size(1), capacity = k_codes.size(2), d = 2 * k_codes.size(3);
+  TORCH_CHECK(d == 64 || d == 128, what, ": the head dimension must be 64 or 128, got ", d);
+  TORCH_CHECK(capacity > 0 && capacity % 64 == 0, what, ": the capacity must be a multiple of 64, got ", capacity);
+  TORCH_CHECK(v_codes.scalar_type() == at::kByte && v_codes.sizes() == at::IntArrayRef({b, kv, capacity / 2, d}), what,
+              ": v_codes must be uint8 of shape (", b, ", ", kv, ", ", capacity / 2, ", ", d, ")");
+  TORCH_CHECK(params.scalar_type() == type_of(flags) && params.sizes() == at::IntArrayRef({b, kv, capacity, 4}), what, ": params must be ",
+              type_name(flags), " of shape (", b, ", ", kv, ", ", capacity, ", 4) for feature_flag=", flags);
+  TORCH_CHECK(lengths.scalar_type() == at::kInt && lengths.sizes() == at::IntArrayRef({b}) && lengths.is_contiguous(), what,
+              ": lengths must be contiguous int32 of shape (", b, ")");
+  TORCH_CHECK(k_codes.is_contiguous() && v_codes.is_contiguous() && params.is_contiguous() && aligned16(k_codes) && aligned16(v_codes) &&
+                  aligned16(params),
+              what, ": k_codes, v_codes and params must be contiguous and 16-byte aligned");
+  // the operators that write the cache say so in their schema
+  return {const_cast<void *>(k_codes.const_data_ptr()), const_cast<void *>(v_codes.const_data_ptr()),
+          const_cast<void *>(params.const_data_ptr()), b, kv, d, capacity};
+}
+
+// the same values, dense and 16-byte aligned
+Tensor dense16(const Tensor &t) {
+  Tensor x = t.is_contiguous() ? t : t.contiguous();
+  return aligned16(x) ? x : x.clone();
+}
+
+Tensor append_kv4(const Tensor &qkv, const Tensor &positions, const Tensor &cos_table, const Tensor &sin_table, const Tensor &lengths,
+                  const Tensor &k_codes, const Tensor &v_codes, const Tensor &params, int64_t n_heads, int64_t flags) {
+  const matgptq_b200_kv4_cache cache = check_kv4("append_kv4", k_codes, v_codes, params, lengths, flags);
+  const c10::Device dev = k_codes.device();
+  for (const Tensor *t : {&qkv, &positions, &cos_table, &sin_table})
+    TORCH_CHECK(t->is_cuda() && t->device() == dev, "append_kv4: qkv, positions, cos_table and sin_table must be on the GPU of the cache");
+  const int64_t b = cache.batch, d = cache.head_dim;
+  TORCH_CHECK(n_heads > 0 && qkv.scalar_type() == type_of(flags) && qkv.dim() == 2 && qkv.size(1) == (n_heads + 2 * cache.n_kv_heads) * d,
+              "append_kv4: qkv must be ", type_name(flags), " of shape (B * S, (n_heads + 2 * KV) * d) for feature_flag=", flags);
+  TORCH_CHECK(b > 0 ? qkv.size(0) % b == 0 : qkv.size(0) == 0, "append_kv4: qkv must have the same number of rows for each of the ", b, " sequences");
+  const int64_t seq = b > 0 ? qkv.size(0) / b : 0;
+  const bool shared = positions.dim() == 1;
+  TORCH_CHECK(positions.scalar_type() == at::kLong && (shared || (positions.dim() == 2 && positions.size(0) == b)) && positions.size(-1) == seq,
+              "append_kv4: positions must be int64 of shape (", seq, ") or (", b, ", ", seq, ")");
+  TORCH_CHECK(cos_table.scalar_type() == at::kFloat && sin_table.scalar_type() == at::kFloat && cos_table.dim() == 2 &&
+                  cos_table.size(0) > 0 && cos_table.size(1) == d / 2 && sin_table.sizes() == cos_table.sizes(),
+              "append_kv4: cos_table and sin_table must be float32 of shape (positions, ", d / 2, ")");
+  const c10::cuda::CUDAGuard on_device(dev);
+  const Tensor x = dense16(qkv), pos = positions.contiguous(), cos = dense16(cos_table), sin = dense16(sin_table);
+  Tensor q = empty_on({b, seq, n_heads, d}, type_of(flags), dev);
+  if (q.numel() == 0) return q;
+  check_status(lib.append_kv4(&cache, x.const_data_ptr(), pos.const_data_ptr<int64_t>(), shared ? 0 : seq, cos.const_data_ptr<float>(),
+                              sin.const_data_ptr<float>(), cos.size(0), lengths.const_data_ptr<int32_t>(), q.data_ptr(), seq, n_heads,
+                              static_cast<uint32_t>(flags), stream_of(dev)),
+               "append_kv4");
+  return q;
+}
+
+Tensor attention_kv4(const Tensor &q, const Tensor &k_codes, const Tensor &v_codes, const Tensor &params, const Tensor &lengths, int64_t window,
+                     int64_t sinks, double scale, int64_t flags, const std::optional<Tensor> &weights) {
+  const matgptq_b200_kv4_cache cache = check_kv4("attention_kv4", k_codes, v_codes, params, lengths, flags);
+  const c10::Device dev = k_codes.device();
+  TORCH_CHECK(q.is_cuda() && q.device() == dev, "attention_kv4: q must be on the GPU of the cache");
+  TORCH_CHECK(q.scalar_type() == type_of(flags) && q.dim() == 4 && q.size(0) == cache.batch && q.size(3) == cache.head_dim,
+              "attention_kv4: q must be ", type_name(flags), " of shape (", cache.batch, ", S, H, ", cache.head_dim, ") for feature_flag=", flags);
+  const int64_t seq = q.size(1), heads = q.size(2);
+  TORCH_CHECK(heads > 0 && heads % cache.n_kv_heads == 0, "attention_kv4: the number of heads (", heads, ") must be a multiple of the cache's (",
+              cache.n_kv_heads, ")");
+  TORCH_CHECK(window >= 0 && sinks >= 0, "attention_kv4: window (0: none) and sinks must not be negative");
+  if (weights)
+    TORCH_CHECK(weights->is_cuda() && weights->device() == dev && weights->scalar_type() == at::kFloat && weights->is_contiguous() &&
+                    weights->sizes() == at::IntArrayRef({cache.batch, cache.n_kv_heads, cache.capacity}),
+                "attention_kv4: weights must be contiguous float32 of shape (", cache.batch, ", ", cache.n_kv_heads, ", ", cache.capacity,
+                ") on the GPU of the cache");
+  const c10::cuda::CUDAGuard on_device(dev);
+  const Tensor x = dense16(q);
+  Tensor out = empty_on({cache.batch, seq, heads, cache.head_dim}, type_of(flags), dev);
+  if (out.numel() == 0) return out;
+  const int64_t need = lib.attention_kv4_workspace_bytes(cache.batch, seq, heads, weights.has_value());
+  const Tensor ws = need > 0 ? empty_on({need}, at::kByte, dev) : Tensor();
+  check_status(lib.attention_kv4(&cache, x.const_data_ptr(), seq, heads, lengths.const_data_ptr<int32_t>(), window, sinks,
+                                 static_cast<float>(scale), weights ? weights->data_ptr<float>() : nullptr, out.data_ptr(),
+                                 ws.defined() ? ws.data_ptr() : nullptr, need, static_cast<uint32_t>(flags), stream_of(dev)),
+               "attention_kv4");
+  return out;
+}
+
+std::tuple<Tensor, Tensor> evict_kv4(const Tensor &k_codes, const Tensor &v_codes, const Tensor &params, const Tensor &weights,
+                                     const Tensor &lengths, int64_t keep, int64_t slack, int64_t sinks, int64_t recent, int64_t flags) {
+  const matgptq_b200_kv4_cache cache = check_kv4("evict_kv4", k_codes, v_codes, params, lengths, flags);
+  const c10::Device dev = k_codes.device();
+  TORCH_CHECK(weights.is_cuda() && weights.device() == dev && weights.scalar_type() == at::kFloat && weights.is_contiguous() &&
+                  weights.sizes() == at::IntArrayRef({cache.batch, cache.n_kv_heads, cache.capacity}),
+              "evict_kv4: weights must be contiguous float32 of shape (", cache.batch, ", ", cache.n_kv_heads, ", ", cache.capacity,
+              ") on the GPU of the cache");
+  TORCH_CHECK(keep > 0 && keep <= cache.capacity && slack >= 0 && slack <= cache.capacity, "evict_kv4: keep must be 1 to the capacity (",
+              cache.capacity, "), slack 0 to the capacity");
+  TORCH_CHECK(sinks >= 0 && recent >= 0 && sinks <= keep && recent <= keep - sinks, "evict_kv4: sinks + recent must fit in keep=", keep);
+  const c10::cuda::CUDAGuard on_device(dev);
+  Tensor new_lengths = empty_on({cache.batch}, at::kInt, dev), kept = empty_on({cache.batch, cache.n_kv_heads, keep}, at::kInt, dev);
+  if (cache.batch == 0) return {new_lengths, kept};
+  check_status(lib.evict_kv4(&cache, weights.data_ptr<float>(), lengths.const_data_ptr<int32_t>(), keep, slack, sinks, recent,
+                             new_lengths.data_ptr<int32_t>(), kept.data_ptr<int32_t>(), static_cast<uint32_t>(flags), stream_of(dev)),
+               "evict_kv4");
+  return {new_lengths, kept};
+}
+
+std::tuple<Tensor, Tensor> dequantize_kv4(const Tensor &k_codes, const Tensor &v_codes, const Tensor &params, const Tensor &lengths,
+                                          int64_t count, int64_t flags) {
+  const matgptq_b200_kv4_cache cache = check_kv4("dequantize_kv4", k_codes, v_codes, params, lengths, flags);
+  TORCH_CHECK(count >= 0, "dequantize_kv4: count must not be negative");
+  const c10::Device dev = k_codes.device();
+  const c10::cuda::CUDAGuard on_device(dev);
+  Tensor k = empty_on({cache.batch, cache.n_kv_heads, count, cache.head_dim}, type_of(flags), dev), v = at::empty_like(k);
+  if (k.numel() == 0) return {k, v};
+  check_status(lib.dequantize_kv4(&cache, lengths.const_data_ptr<int32_t>(), count, k.data_ptr(), v.data_ptr(), static_cast<uint32_t>(flags),
+                                  stream_of(dev)),
+               "dequantize_kv4");
+  return {k, v};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(matgptq_cuda, m) {
@@ -302,6 +431,14 @@ TORCH_LIBRARY(matgptq_cuda, m) {
         "SymInt n_in_features, SymInt[] bitwidths, SymInt group_size, SymInt feature_flag) -> Tensor", tags);
   m.def("matmul_matgptq_zeros(Tensor input, Tensor matgptq_weights, Tensor matgptq_scales, Tensor matgptq_zeros, "
         "SymInt n_out_features, SymInt n_in_features, SymInt bitwidth, SymInt group_size, SymInt feature_flag) -> Tensor", tags);
+  m.def("append_kv4(Tensor qkv, Tensor positions, Tensor cos_table, Tensor sin_table, Tensor lengths, Tensor(a5!) k_codes, "
+        "Tensor(a6!) v_codes, Tensor(a7!) params, SymInt n_heads, SymInt feature_flag) -> Tensor", tags);
+  m.def("attention_kv4(Tensor q, Tensor k_codes, Tensor v_codes, Tensor params, Tensor lengths, SymInt window, SymInt sinks, float scale, "
+        "SymInt feature_flag, Tensor(a9!)? weights=None) -> Tensor", tags);
+  m.def("evict_kv4(Tensor(a0!) k_codes, Tensor(a1!) v_codes, Tensor(a2!) params, Tensor(a3!) weights, Tensor lengths, SymInt keep, "
+        "SymInt slack, SymInt sinks, SymInt recent, SymInt feature_flag) -> (Tensor, Tensor)", tags);
+  m.def("dequantize_kv4(Tensor k_codes, Tensor v_codes, Tensor params, Tensor lengths, SymInt count, SymInt feature_flag) -> "
+        "(Tensor, Tensor)", tags);
   m.def("dequantize_matgptq(Tensor matgptq_weights, Tensor matgptq_scales, SymInt n_out_features, SymInt n_in_features, "
         "SymInt bitwidth, SymInt group_size, SymInt feature_flag) -> Tensor", tags);
 }
@@ -318,6 +455,10 @@ TORCH_LIBRARY(matgptq_cuda, m) {
     m.impl("matmul_matgptq_grouped", matmul_grouped);                       \
     m.impl("matmul_matgptq_zeros", matmul_zeros);                           \
     m.impl("dequantize_matgptq", dequantize);                               \
+    m.impl("append_kv4", append_kv4);                                       \
+    m.impl("attention_kv4", attention_kv4);                                 \
+    m.impl("evict_kv4", evict_kv4);                                         \
+    m.impl("dequantize_kv4", dequantize_kv4);                               \
   }
 MG_REGISTER(CPU)
 MG_REGISTER(CUDA)
@@ -351,30 +492,41 @@ void without_derivative(const c10::OperatorHandle &op, c10::DispatchKeySet keys,
   }
   if (inputs.empty() || op.schema().returns().empty()) return;
   const auto node = std::make_shared<torch::autograd::NotImplemented>(op.schema().name(), torch::autograd::collect_next_edges(inputs));
-  Tensor result = stack->back().toTensor();
-  torch::autograd::set_history(result, node);
+  const size_t returns = op.schema().returns().size();
+  for (size_t i = stack->size() - returns; i < stack->size(); ++i) {
+    Tensor result = (*stack)[i].toTensor();
+    if (result.is_floating_point()) torch::autograd::set_history(result, node);
+  }
 }
 
-// matmul_matgptq_out writes its last argument
+// what an operator writes counts as written
 void counts_as_write(const c10::OperatorHandle &op, c10::DispatchKeySet keys, torch::jit::Stack *stack) {
-  const Tensor out = stack->back().toTensor();
+  std::vector<Tensor> written;
+  const auto &arguments = op.schema().arguments();
+  const size_t first = stack->size() - arguments.size();
+  for (size_t i = 0; i < arguments.size(); ++i)
+    if (arguments[i].alias_info() && arguments[i].alias_info()->isWrite() && (*stack)[first + i].isTensor())
+      written.push_back((*stack)[first + i].toTensor());
   {
     const at::AutoDispatchBelowADInplaceOrView below;
     op.redispatchBoxed(keys & c10::after_ADInplaceOrView_keyset, stack);
   }
-  if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+  for (const Tensor &t : written)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 }  // namespace
 
 TORCH_LIBRARY_IMPL(matgptq_cuda, Autograd, m) {
   for (const char *name : {"pack_matgptq_qweights", "slice_pack_matgptq_qweights", "reorder_matgptq_scales", "matmul_matgptq",
-                           "matmul_matgptq_out", "matmul_matgptq_grouped", "matmul_matgptq_zeros", "dequantize_matgptq"})
+                           "matmul_matgptq_out", "matmul_matgptq_grouped", "matmul_matgptq_zeros", "dequantize_matgptq", "append_kv4",
+                           "attention_kv4", "evict_kv4", "dequantize_kv4"})
     m.impl(name, torch::CppFunction::makeFromBoxedFunction<&without_derivative>());
 }
 
 TORCH_LIBRARY_IMPL(matgptq_cuda, ADInplaceOrView, m) {
-  m.impl("matmul_matgptq_out", torch::CppFunction::makeFromBoxedFunction<&counts_as_write>());
+  for (const char *name : {"matmul_matgptq_out", "append_kv4", "attention_kv4", "evict_kv4"})
+    m.impl(name, torch::CppFunction::makeFromBoxedFunction<&counts_as_write>());
 }
 
 // ---- Python module --------------------------------------------------------------------------------------------
@@ -529,6 +681,11 @@ PyObject *py_bind(PyObject *, PyObject *path) {
   find(lib.pack_qweights, "matgptq_b200_pack_qweights");
   find(lib.reorder_scales, "matgptq_b200_reorder_scales");
   find(lib.dequantize, "matgptq_b200_dequantize");
+  find(lib.append_kv4, "matgptq_b200_append_kv4");
+  find(lib.attention_kv4, "matgptq_b200_attention_kv4");
+  find(lib.attention_kv4_workspace_bytes, "matgptq_b200_attention_kv4_workspace_bytes");
+  find(lib.evict_kv4, "matgptq_b200_evict_kv4");
+  find(lib.dequantize_kv4, "matgptq_b200_dequantize_kv4");
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }

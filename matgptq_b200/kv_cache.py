@@ -1,0 +1,107 @@
+"""A key/value cache in 4 bits for every layer of a model, over the operators ``*_kv4`` of ``matgptq_b200.ops``.
+
+The reference leaves its cache to vLLM / transformers, in 16 bits (``inference_lib/inference_demo_vllm.py``,
+``inference_demo_transformers.py:141-173``).  Here an entry takes ``head_dim + 8`` bytes per key/value head instead of ``4 * head_dim``:
+codes of 4 bits with a scale and a minimum for each row of K and of V.  Attention reads the codes as they are, over all entries or over a
+sliding window and the first ``sinks`` entries; with ``weights=True`` it adds up what each entry is attended with, and ``evict`` keeps the
+entries that were attended most.
+
+One step of a model::
+
+    cache.advance(S)                                          # every sequence gets S new entries
+    for i, layer in enumerate(layers):
+        q = cache.append(i, qkv, positions, cos, sin, n_heads)  # [B, S, H, d]
+        out = cache.attend(i, q, window=1024, sinks=4)          # [B, S, H, d]
+    cache.evict(keep=1024, slack=128, sinks=4, recent=256)    # optional
+
+All calls work on the current stream, allocate through torch's allocator and can be captured into a CUDA graph.  A prompt batch of unequal
+lengths is padded on the left: ``advance`` takes the tokens of each sequence as a tensor.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _native, ops
+
+
+class KV4Cache:
+    """``n_layers`` caches of ``capacity`` entries (rounded up to a multiple of 64) for ``batch`` sequences, with one count of entries for all
+    layers: ``lengths``, int32 on the device."""
+
+    def __init__(self, n_layers: int, batch: int, n_kv_heads: int, head_dim: int, capacity: int, dtype: torch.dtype = torch.float16,
+                 device: torch.device | str = "cuda", weights: bool = False):
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"the type of a 4-bit cache's scales must be float16 or bfloat16, got {dtype}")
+        if head_dim not in (64, 128):
+            raise ValueError(f"the head dimension of a 4-bit cache must be 64 or 128, got {head_dim}")
+        if min(n_layers, batch, n_kv_heads, capacity) < 1:
+            raise ValueError("n_layers, batch, n_kv_heads and capacity must be at least 1")
+        self.n_layers, self.batch, self.n_kv_heads, self.head_dim = n_layers, batch, n_kv_heads, head_dim
+        self.capacity = -(-capacity // 64) * 64
+        self.dtype = dtype
+        self.flag = _native.FLAG_ASYNC | (_native.FLAG_BF16 if dtype == torch.bfloat16 else 0)
+        new = lambda t, *s: [torch.zeros(batch, n_kv_heads, *s, dtype=t, device=device) for _ in range(n_layers)]  # noqa: E731
+        self.k_codes = new(torch.uint8, self.capacity, head_dim // 2)
+        self.v_codes = new(torch.uint8, self.capacity // 2, head_dim)
+        self.params = new(dtype, self.capacity, 4)
+        self.weights = new(torch.float32, self.capacity) if weights else None
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.most = 0  # no sequence has more entries, as far as the calls from the host tell
+
+    def layer(self, i: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        return self.k_codes[i], self.v_codes[i], self.params[i]
+
+    def reset(self) -> None:
+        """No entries, no weights."""
+        self.lengths.zero_()
+        self.most = 0
+        for w in self.weights or ():
+            w.zero_()
+
+    def advance(self, tokens: int, valid: torch.Tensor | None = None) -> None:
+        """Counts ``tokens`` new entries for every sequence, before the layers append them; ``valid`` int32 ``[batch]``: only so many of
+        each sequence's are real, the ones in front are padding (the sequence has to be empty so far)."""
+        if self.most + tokens > self.capacity:
+            raise RuntimeError(f"the cache holds {self.capacity} entries: {self.most} and {tokens} more do not fit")
+        self.lengths.add_(tokens if valid is None else valid)
+        self.most += tokens
+
+    def append(self, i: int, qkv: torch.Tensor, positions: torch.Tensor, cos_table: torch.Tensor, sin_table: torch.Tensor, n_heads: int,
+               pdl: bool = False) -> torch.Tensor:
+        """Writes the tokens of ``qkv`` into layer ``i`` and returns q, rotated, ``[B, S, H, d]`` (``ops.append_kv4``)."""
+        return ops.append_kv4(qkv, positions, cos_table, sin_table, self.lengths, *self.layer(i), n_heads, self._flags(pdl))
+
+    def attend(self, i: int, q: torch.Tensor, window: int = 0, sinks: int = 0, scale: float | None = None, pdl: bool = False) -> torch.Tensor:
+        """Attention of ``q [B, S, H, d]`` over layer ``i`` (``ops.attention_kv4``); adds to the layer's weights if the cache has them."""
+        return ops.attention_kv4(q, *self.layer(i), self.lengths, window, sinks, 1.0 / math.sqrt(self.head_dim) if scale is None else scale,
+                                 self._flags(pdl), self.weights[i] if self.weights is not None else None)
+
+    def evict(self, keep: int, slack: int = 0, sinks: int = 0, recent: int = 0, pdl: bool = False) -> list[torch.Tensor]:
+        """Cuts sequences of more than ``keep + slack`` entries back to ``keep`` in every layer (``ops.evict_kv4``).  Returns, layer by
+        layer, the old indices of the entries that stayed."""
+        if self.weights is None:
+            raise RuntimeError("eviction goes by the attention weights: make the cache with weights=True")
+        kept, lengths = [], self.lengths
+        for i in range(self.n_layers):
+            lengths, indices = ops.evict_kv4(*self.layer(i), self.weights[i], self.lengths, keep, slack, sinks, recent, self._flags(pdl))
+            kept.append(indices)
+        self.lengths.copy_(lengths)
+        if self.most > keep + slack:
+            self.most = keep + slack
+        return kept
+
+    def dequantize(self, i: int, count: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """The last ``count`` entries of layer ``i`` as dense K and V ``[B, KV, count, d]`` (``ops.dequantize_kv4``)."""
+        return ops.dequantize_kv4(*self.layer(i), self.lengths, count, self.flag)
+
+    def tensors(self) -> list[torch.Tensor]:
+        """Everything that a step changes on the device."""
+        return [*self.k_codes, *self.v_codes, *self.params, *(self.weights or []), self.lengths]
+
+    def bytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in self.tensors())
+
+    def _flags(self, pdl: bool) -> int:
+        return self.flag | (_native.FLAG_PDL if pdl else 0)

@@ -7,8 +7,9 @@ matmul_matgptq}``.  They are registered and checked in C++ (``csrc/torch_ops.cpp
 ``_torch_ops``), because a call with few rows costs more on the host than on the GPU; PyTorch supplies
 device memory and the current stream, and the work is done by ``libmatgptq_b200.so`` through its C ABI.
 Additions sit beside them: ``slice_pack_matgptq_qweights`` (slicing fused into packing),
-``matmul_matgptq_out``, ``matmul_matgptq_grouped``, ``matmul_matgptq_zeros`` and
-``dequantize_matgptq`` (dense weights for checks).
+``matmul_matgptq_out``, ``matmul_matgptq_grouped``, ``matmul_matgptq_zeros``,
+``dequantize_matgptq`` (dense weights for checks), and a key/value cache in 4 bits: ``append_kv4``,
+``attention_kv4``, ``evict_kv4``, ``dequantize_kv4`` (``matgptq_b200.kv_cache`` holds its tensors).
 """
 from __future__ import annotations
 
@@ -165,6 +166,63 @@ def dequantize_matgptq(matgptq_weights: torch.Tensor, matgptq_scales: torch.Tens
 @torch.library.register_fake("matgptq_cuda::dequantize_matgptq")
 def _dequant_fake(matgptq_weights, matgptq_scales, n_out_features, n_in_features, bitwidth, group_size, feature_flag):
     return matgptq_scales.new_empty((n_out_features, n_in_features))
+
+
+def append_kv4(qkv: torch.Tensor, positions: torch.Tensor, cos_table: torch.Tensor, sin_table: torch.Tensor, lengths: torch.Tensor,
+               k_codes: torch.Tensor, v_codes: torch.Tensor, params: torch.Tensor, n_heads: int, feature_flag: int) -> torch.Tensor:
+    """Addition: writes the tokens of ``qkv [B * S, (H + 2 KV) * d]`` (k rotated) into a cache in 4 bits and returns q, rotated,
+    ``[B, S, H, d]``.
+
+    ``k_codes`` uint8 ``[B, KV, capacity, d/2]``, ``v_codes`` uint8 ``[B, KV, capacity/2, d]`` and ``params [B, KV, capacity, 4]`` are the
+    cache (layout: ``include/matgptq_b200.h``); ``lengths`` int32 ``[B]`` counts the entries of each sequence with the new ones: token
+    ``i`` becomes entry ``lengths[b] - S + i``, and is padding where that is negative.  ``positions`` int64 ``[S]`` or ``[B, S]`` select the
+    rows of the fp32 tables ``[positions, d/2]``; pairs of channels are ``(2i, 2i + 1)``."""
+    return _ops.append_kv4(qkv, positions, cos_table, sin_table, lengths, k_codes, v_codes, params, n_heads, feature_flag)
+
+
+@torch.library.register_fake("matgptq_cuda::append_kv4")
+def _append_kv4_fake(qkv, positions, cos_table, sin_table, lengths, k_codes, v_codes, params, n_heads, feature_flag):
+    return qkv.new_empty((lengths.shape[0], qkv.shape[0] // lengths.shape[0], n_heads, 2 * k_codes.shape[3]))
+
+
+def attention_kv4(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, params: torch.Tensor, lengths: torch.Tensor, window: int,
+                  sinks: int, scale: float, feature_flag: int, weights: torch.Tensor | None = None) -> torch.Tensor:
+    """Addition: ``softmax(scale * q K^T) V`` of ``q [B, S, H, d]`` over a cache in 4 bits that holds the queries' own tokens as its last
+    ``S`` entries.  Query ``i`` is entry ``p = lengths[b] - S + i`` and sees entry ``j`` when ``j <= p`` and (``window == 0``, or
+    ``j > p - window``, or ``j < sinks``); one that sees nothing gives zeros.  ``weights`` fp32 ``[B, KV, capacity]``: the softmax weights of
+    each entry, summed over the queries and heads that share it, are added to it."""
+    return _ops.attention_kv4(q, k_codes, v_codes, params, lengths, window, sinks, scale, feature_flag, weights)
+
+
+@torch.library.register_fake("matgptq_cuda::attention_kv4")
+def _attention_kv4_fake(q, k_codes, v_codes, params, lengths, window, sinks, scale, feature_flag, weights=None):
+    return q.new_empty(q.shape)
+
+
+def evict_kv4(k_codes: torch.Tensor, v_codes: torch.Tensor, params: torch.Tensor, weights: torch.Tensor, lengths: torch.Tensor, keep: int,
+              slack: int, sinks: int, recent: int, feature_flag: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Addition: cuts every sequence of more than ``keep + slack`` entries back to ``keep``, in place: the first ``sinks``, the last
+    ``recent``, and of the others, head by head, those with the largest ``weights`` (ties: the lowest entry).  Returns the new lengths
+    int32 ``[B]`` and the old indices of the entries that stayed, int32 ``[B, KV, keep]`` (-1 where a sequence was not cut)."""
+    return _ops.evict_kv4(k_codes, v_codes, params, weights, lengths, keep, slack, sinks, recent, feature_flag)
+
+
+@torch.library.register_fake("matgptq_cuda::evict_kv4")
+def _evict_kv4_fake(k_codes, v_codes, params, weights, lengths, keep, slack, sinks, recent, feature_flag):
+    return lengths.new_empty(lengths.shape), lengths.new_empty((k_codes.shape[0], k_codes.shape[1], keep))
+
+
+def dequantize_kv4(k_codes: torch.Tensor, v_codes: torch.Tensor, params: torch.Tensor, lengths: torch.Tensor, count: int,
+                   feature_flag: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Addition: the last ``count`` entries of every sequence as dense K and V ``[B, KV, count, d]``, zeros in front where a sequence
+    has fewer."""
+    return _ops.dequantize_kv4(k_codes, v_codes, params, lengths, count, feature_flag)
+
+
+@torch.library.register_fake("matgptq_cuda::dequantize_kv4")
+def _dequantize_kv4_fake(k_codes, v_codes, params, lengths, count, feature_flag):
+    shape = (k_codes.shape[0], k_codes.shape[1], count, 2 * k_codes.shape[3])
+    return params.new_empty(shape), params.new_empty(shape)
 
 
 def matmul_matgptq_raw(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, n_out: int, n_in: int,

@@ -1,0 +1,115 @@
+"""The key/value cache in 4 bits in plain 64-bit operations: what the operators ``*_kv4`` are tested against.  Lists of sequences and
+heads are walked one by one; nothing here is shared with the library."""
+import math
+
+import torch
+
+
+def quantise_rows(x):
+    """Rows of 16-bit numbers ``[..., d]`` -> codes (int64), scale, minimum (float64, both representable in the type of ``x``)."""
+    x64 = x.double()
+    low, high = x64.min(-1, keepdim=True).values, x64.max(-1, keepdim=True).values
+    scale = ((high - low) / 15).to(x.dtype).double()
+    codes = torch.where(scale > 0, (x64 - low) / torch.where(scale > 0, scale, 1.0), 0.0).round().clamp(max=15).long()
+    return codes, scale, low
+
+
+def pack_k(codes):
+    """``[..., d]`` codes -> ``[..., d/2]`` bytes."""
+    return (codes[..., 0::2] + 16 * codes[..., 1::2]).to(torch.uint8)
+
+
+def unpack_k(k_codes):
+    out = torch.empty(*k_codes.shape[:-1], 2 * k_codes.shape[-1], dtype=torch.int64, device=k_codes.device)
+    out[..., 0::2] = k_codes.long() % 16
+    out[..., 1::2] = k_codes.long() // 16
+    return out
+
+
+def pack_v(codes):
+    """``[B, KV, capacity, d]`` codes -> ``[B, KV, capacity/2, d]`` bytes: two bytes of one entry, two of the other."""
+    rows = pack_k(codes)
+    out = torch.empty(*rows.shape[:2], rows.shape[2] // 2, 2 * rows.shape[3], dtype=torch.uint8, device=codes.device)
+    for which in range(2):
+        for byte in range(2):
+            out[..., 2 * which + byte::4] = rows[:, :, which::2, byte::2]
+    return out
+
+
+def unpack_v(v_codes):
+    rows = torch.empty(*v_codes.shape[:2], 2 * v_codes.shape[2], v_codes.shape[3] // 2, dtype=torch.uint8, device=v_codes.device)
+    for which in range(2):
+        for byte in range(2):
+            rows[:, :, which::2, byte::2] = v_codes[..., 2 * which + byte::4]
+    return unpack_k(rows)
+
+
+def dense(k_codes, v_codes, params):
+    """K and V of a whole cache in float64."""
+    p = params.double()
+    return p[..., 1:2] + p[..., 0:1] * unpack_k(k_codes), p[..., 3:4] + p[..., 2:3] * unpack_v(v_codes)
+
+
+def visible(length, seq, window, sinks, device=None):
+    """``[seq, length]``: which entries each query sees."""
+    at = torch.arange(length - seq, length, device=device)[:, None]
+    key = torch.arange(length, device=device)[None]
+    seen = key <= at
+    if window:
+        seen = seen & ((key > at - window) | (key < sinks))
+    return seen
+
+
+def attention(q, k_codes, v_codes, params, lengths, window, sinks, scale):
+    """``(out [B, S, H, d], added weights [B, KV, capacity], bound of |out - kernel| before its rounding, bound of the weights)``.
+
+    The bounds count the roundings of the operator: fp32 scores (``2**-20`` of the sums of magnitudes: products of codes are exact, the
+    tensor cores and what follows add about twenty times with 24 bits, q as scaled fp16 keeps ``2**-25`` of its largest value), ``p * v_scale``
+    to fp16 (``2**-11`` relative: ten fraction bits behind the leading one, off by half of the last at most, ``2**-25`` of the largest scale at the least, before the division by the sum), sums in fp32."""
+    b, seq, h, d = q.shape
+    kv, capacity = k_codes.shape[1], k_codes.shape[2]
+    group = h // kv
+    k_all, v_all = unpack_k(k_codes), unpack_v(v_codes)
+    out = torch.zeros(b, seq, h, d, dtype=torch.float64, device=q.device)
+    near = torch.zeros_like(out)
+    weights = torch.zeros(b, kv, capacity, dtype=torch.float64, device=q.device)
+    weights_near = torch.zeros_like(weights)
+    for i in range(b):
+        n = int(lengths[i])
+        if n == 0:
+            continue
+        seen = visible(n, seq, window, sinks, q.device)
+        for j in range(kv):
+            ks, kl, vs, vl = (params[i, j, :n, c].double() for c in range(4))
+            kc, vc = k_all[i, j, :n].double(), v_all[i, j, :n].double()
+            for g in range(group):
+                x = q[i, :, j * group + g].double()
+                score = scale * (x @ kc.T * ks + x.sum(-1, keepdim=True) * kl)
+                size = abs(scale) * (x.abs() @ kc.T * ks.abs() + x.abs().sum(-1, keepdim=True) * kl.abs())
+                top_q = x.abs().max(-1, keepdim=True).values
+                size = size * 2.0 ** -20 + abs(scale) * top_q * 2.0 ** -25 * (kc.sum(-1) * ks.abs() + d * kl.abs()) + 2.0 ** -22
+                score = torch.where(seen, score, -math.inf)
+                size = torch.where(seen, size, 0.0)
+                top = score.max(-1, keepdim=True).values
+                p = torch.where(seen, (score - torch.where(top > -math.inf, top, 0.0)).exp(), 0.0)
+                total = p.sum(-1, keepdim=True)
+                p = p / torch.where(total > 0, total, 1.0)
+                v = vl[:, None] + vs[:, None] * vc
+                out[i, :, j * group + g] = p @ v
+                off = 2 * size.max(-1, keepdim=True).values + 2.0 ** -20
+                floor = 2.0 ** -25 * vs.abs().max() * seen.sum(-1, keepdim=True) / torch.where(total > 0, total, 1.0)
+                near[i, :, j * group + g] = off * (p @ v.abs()) + 2.0 ** -11 * (p @ (vs[:, None] * (vc - 8).abs())) + 8 * floor * (total > 0) \
+                    + 2.0 ** -20 * (p @ (vl.abs() + 15 * vs.abs()))[:, None]
+                weights[i, j, :n] += p.sum(0)
+                weights_near[i, j, :n] += (p * off).sum(0)
+    return out, weights, near, weights_near
+
+
+def evict(weights, length, keep, slack, sinks, recent):
+    """The entries of one sequence and head that stay, in order, or None where it is not cut."""
+    if length <= keep + slack:
+        return None
+    w = [float(x) for x in weights[:length]]
+    # a NaN counts as the largest weight; ties go to the lowest entry
+    order = sorted(range(sinks, length - recent), key=lambda j: (0, 0.0, j) if w[j] != w[j] else (1, -w[j], j))
+    return sorted([*range(sinks), *order[:keep - sinks - recent], *range(length - recent, length)])
