@@ -7,7 +7,8 @@ Stands in for the two serving loops of the reference — vLLM with ``tensor_para
 bitwidths and CUDA-graph replay are under this package's control.  Every block linear goes through
 ``libmatgptq_b200`` (GEMV family for decode, tensor-core path for prefill); attention, RMSNorm, RoPE,
 embedding and the unquantised ``lm_head`` are plain torch ops (plumbing, as in the reference, which
-leaves them to vLLM / transformers).  Weights are random-init (no checkpoints exist here): master codes
+leaves them to vLLM / transformers).  With ``kv_bits=4`` the cache holds 4-bit codes and attention, its window and
+its eviction are this library's (``kv_cache.KV4Cache``).  Weights are random-init (no checkpoints exist here): master codes
 and scales are drawn per layer on the GPU from a seed (``matgptq_b200.synth``).
 
 Tensor parallelism: q/k/v and gate/up are column-parallel (out-features split), o and down are
@@ -23,6 +24,7 @@ import torch.distributed as dist
 import torch.nn.functional as F
 
 from . import _native, ops, synth
+from .kv_cache import KV4Cache
 
 
 @dataclass
@@ -118,8 +120,13 @@ class PackedLlama:
 
     def __init__(self, shape: LlamaShape, bits, *, group_size: int = 128, dtype: torch.dtype = torch.float16,
                  tp_rank: int = 0, tp_size: int = 1, seed: int = 0, batch: int = 1, max_seq: int = 256,
-                 device: torch.device | str = "cuda", keep_master: bool = False, pdl: bool = True, peer_allreduce=None):
-        """``peer_allreduce``: a ``tp_comm.PeerAllReduce`` of the tensor-parallel group.  With it the row-parallel
+                 device: torch.device | str = "cuda", keep_master: bool = False, pdl: bool = True, peer_allreduce=None,
+                 kv_bits: int = 16, kv_window: int = 0, kv_sinks: int = 0, kv_keep: int = 0, kv_slack: int = 0, kv_recent: int = 0):
+        """``kv_bits``: 16, or 4 for a cache of 4-bit codes (head dimension 64 or 128).  With 4 bits ``kv_window`` (0: none) and
+        ``kv_sinks`` limit what a token sees, and ``kv_keep`` (0: everything) cuts sequences of more than ``kv_keep + kv_slack`` entries back
+        to ``kv_keep`` after every step: the first ``kv_sinks``, the last ``kv_recent`` and those that were attended most.
+
+        ``peer_allreduce``: a ``tp_comm.PeerAllReduce`` of the tensor-parallel group.  With it the row-parallel
         layers (o, down) run the product fused with its all-reduce over peer memory for fewer than 32 rows; without
         it (and for larger batches) the product is followed by an NCCL all-reduce."""
         self.shape, self.dtype, self.dev = shape, dtype, torch.device(device)
@@ -156,8 +163,18 @@ class PackedLlama:
         inv = 1.0 / (shape.rope_theta ** (torch.arange(0, d, 2, device=self.dev, dtype=torch.float32) / d))
         ang = torch.arange(max_seq, device=self.dev, dtype=torch.float32)[:, None] * inv[None, :]
         self.cos, self.sin = ang.cos(), ang.sin()
-        self.k_cache = [torch.zeros(batch, self.kv_loc, max_seq, d, dtype=dtype, device=self.dev) for _ in range(shape.n_layers)]
-        self.v_cache = [torch.zeros_like(k) for k in self.k_cache]
+        if kv_bits not in (4, 16) or (kv_bits == 16 and (kv_window or kv_sinks or kv_keep or kv_slack or kv_recent)):
+            raise ValueError("kv_bits must be 16 or 4; a window, first entries and eviction need kv_bits=4")
+        if kv_keep and kv_sinks + kv_recent > kv_keep:
+            raise ValueError("kv_sinks and kv_recent must fit in kv_keep")
+        self.kv_window, self.kv_sinks, self.kv_keep, self.kv_slack, self.kv_recent = kv_window, kv_sinks, kv_keep, kv_slack, kv_recent
+        if kv_bits == 4:
+            self.cache4 = KV4Cache(shape.n_layers, batch, self.kv_loc, d, max_seq, dtype, self.dev, weights=kv_keep > 0)
+            self.k_cache, self.v_cache = [], []
+        else:
+            self.cache4 = None
+            self.k_cache = [torch.zeros(batch, self.kv_loc, max_seq, d, dtype=dtype, device=self.dev) for _ in range(shape.n_layers)]
+            self.v_cache = [torch.zeros_like(k) for k in self.k_cache]
 
     # -- pieces ------------------------------------------------------------------------------
     def linear(self, layer: int, which: str, x: torch.Tensor) -> torch.Tensor:
@@ -181,7 +198,8 @@ class PackedLlama:
 
     def forward(self, tokens: torch.Tensor, positions: torch.Tensor, fp32_logits: bool = True) -> torch.Tensor:
         """tokens [B, S] int64, positions [S] int64 (device) -> logits of the last position [B, vocab]
-        (fp32, or the model dtype with ``fp32_logits=False``)."""
+        (fp32, or the model dtype with ``fp32_logits=False``).  A 4-bit cache appends the tokens behind the entries it has
+        (``reset`` empties it); the 16-bit cache writes them at their positions."""
         B, S = tokens.shape
         d, H = self.shape.head_dim, self.shape.hidden
         lib = _native.load()
@@ -198,18 +216,25 @@ class PackedLlama:
 
         x = self.embed[tokens].reshape(rows, H)
         h = torch.empty_like(x)
-        q = torch.empty(B, self.h_loc, S, d, dtype=self.dtype, device=self.dev)
         act = torch.empty(rows, self.layers[0]["down"].n_in, dtype=self.dtype, device=self.dev)
-        mask = torch.empty(1, 1, S, self.max_seq, dtype=self.dtype, device=self.dev)
-        _native.check(lib.matgptq_b200_causal_mask(positions.data_ptr(), mask.data_ptr(), S, self.max_seq, flag, stream), "causal_mask")
+        if self.cache4 is not None:
+            self.cache4.advance(S)
+        else:
+            q = torch.empty(B, self.h_loc, S, d, dtype=self.dtype, device=self.dev)
+            mask = torch.empty(1, 1, S, self.max_seq, dtype=self.dtype, device=self.dev)
+            _native.check(lib.matgptq_b200_causal_mask(positions.data_ptr(), mask.data_ptr(), S, self.max_seq, flag, stream), "causal_mask")
         add_norm(x, None, self.layers[0]["ln1"], h)
         for li, L in enumerate(self.layers):
             qkv = self.linear(li, "qkv", h)
-            _native.check(lib.matgptq_b200_rope_kv(qkv.data_ptr(), positions.data_ptr(), self.cos.data_ptr(), self.sin.data_ptr(),
-                                                   q.data_ptr(), self.k_cache[li].data_ptr(), self.v_cache[li].data_ptr(),
-                                                   B, S, self.h_loc, self.kv_loc, d, self.max_seq, flag, stream), "rope_kv")
-            att = F.scaled_dot_product_attention(q, self.k_cache[li], self.v_cache[li], attn_mask=mask, enable_gqa=True)
-            att = att.transpose(1, 2).reshape(rows, self.h_loc * d)
+            if self.cache4 is not None:
+                q = self.cache4.append(li, qkv, positions, self.cos, self.sin, self.h_loc, self.pdl)
+                att = self.cache4.attend(li, q, self.kv_window, self.kv_sinks, pdl=self.pdl).view(rows, self.h_loc * d)
+            else:
+                _native.check(lib.matgptq_b200_rope_kv(qkv.data_ptr(), positions.data_ptr(), self.cos.data_ptr(), self.sin.data_ptr(),
+                                                       q.data_ptr(), self.k_cache[li].data_ptr(), self.v_cache[li].data_ptr(),
+                                                       B, S, self.h_loc, self.kv_loc, d, self.max_seq, flag, stream), "rope_kv")
+                att = F.scaled_dot_product_attention(q, self.k_cache[li], self.v_cache[li], attn_mask=mask, enable_gqa=True)
+                att = att.transpose(1, 2).reshape(rows, self.h_loc * d)
             o = self.row_parallel(li, "o", att)
             add_norm(x, o, L["ln2"], h)
             gu = self.linear(li, "gate_up", h)
@@ -217,6 +242,8 @@ class PackedLlama:
             dn = self.row_parallel(li, "down", act)
             nxt = self.layers[li + 1]["ln1"] if li + 1 < len(self.layers) else self.final_norm
             add_norm(x, dn, nxt, h)
+        if self.kv_keep:
+            self.cache4.evict(self.kv_keep, self.kv_slack, self.kv_sinks, self.kv_recent, pdl=self.pdl)
         last = h.view(B, S, H)[:, -1]
         logits = F.linear(last, self.lm_head)
         if fp32_logits:
@@ -230,12 +257,21 @@ class PackedLlama:
     def weight_bytes(self) -> int:
         return sum(L[k].weight_bytes() for L in self.layers for k in ("qkv", "o", "gate_up", "down"))
 
+    def reset(self) -> None:
+        """Empties a 4-bit cache (a 16-bit cache is written by position and needs no emptying)."""
+        if self.cache4 is not None:
+            self.cache4.reset()
+
+    def _cache_tensors(self) -> list[torch.Tensor]:
+        return self.cache4.tensors() if self.cache4 is not None else [*self.k_cache, *self.v_cache]
+
     # -- generation --------------------------------------------------------------------------
     @torch.no_grad()
     def generate(self, prompt: torch.Tensor, new_tokens: int, use_graph: bool = True) -> dict:
         """Greedy decode. Returns generated tokens [B, new_tokens] and device-timed prefill/decode seconds."""
         B, P = prompt.shape
         assert B == self.batch and P + new_tokens <= self.max_seq
+        self.reset()
         ev = [torch.cuda.Event(enable_timing=True) for _ in range(4)]
         ev[0].record()
         logits = self.forward(prompt, torch.arange(P, device=self.dev))
@@ -261,7 +297,8 @@ class PackedLlama:
 
         graph = None
         if use_graph and new_tokens > 2:
-            state = (tok.clone(), pos.clone(), step_idx.clone(), out.clone(), [k.clone() for k in self.k_cache], [v.clone() for v in self.v_cache])
+            state = [tok, pos, step_idx, out, *self._cache_tensors()]
+            saved, most = [t.clone() for t in state], self.cache4.most if self.cache4 is not None else 0
             s = torch.cuda.Stream(device=self.dev)
             s.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(s):
@@ -272,11 +309,10 @@ class PackedLlama:
                     step()
             torch.cuda.current_stream().wait_stream(s)
             # rewind everything the two trial steps touched
-            tok.copy_(state[0]); pos.copy_(state[1]); step_idx.copy_(state[2]); out.copy_(state[3])
-            for k, k0 in zip(self.k_cache, state[4]):
-                k.copy_(k0)
-            for v, v0 in zip(self.v_cache, state[5]):
-                v.copy_(v0)
+            for t, t0 in zip(state, saved):
+                t.copy_(t0)
+            if self.cache4 is not None:  # a replayed step does not count on the host: count all of them here
+                self.cache4.most = min(most + new_tokens - 1, self.kv_keep + self.kv_slack if self.kv_keep else self.max_seq)
         torch.cuda.synchronize()
         if self.tp_size > 1:
             dist.barrier()
