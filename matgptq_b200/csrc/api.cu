@@ -370,6 +370,9 @@ int matgptq_b200_device_status(int *status_out, int reset) {
   r = mg::kv4_attention_device_status(&k2, reset);
   if (r != MG_OK) return r;
   if (k == 0) k = k2;
+  r = mg::kv4_prompt_device_status(&k2, reset);
+  if (r != MG_OK) return r;
+  if (k == 0) k = k2;
   if (status_out) *status_out = a ? a : (b ? b : (d ? d : (f ? f : (k ? k : e))));
   return MG_OK;
 }

@@ -84,9 +84,10 @@ struct TsPlan {
 TsPlan gemm_ts_plan(int N, int K, int M, int group_size, int max_split, int sm_count, const int *clusters_at_once);
 int gemm_ts_device_status(int *status_out, int reset);
 
-// kv4.cu, kv4_attention.cu
+// kv4.cu, kv4_attention.cu, kv4_prompt.cu
 int kv4_device_status(int *status_out, int reset);
 int kv4_attention_device_status(int *status_out, int reset);
+int kv4_prompt_device_status(int *status_out, int reset);
 
 // selftest.cu
 int selftest_device_status(int *status_out, int reset);

@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 #include "../../include/matgptq_b200.h"
 #include "async.cuh"
@@ -23,48 +24,12 @@
 #include "helper_kernels.cuh"
 #include "host_util.h"
 #include "kernels.h"
-#include "kv4.cuh"
+#include "kv4_attention.cuh"
 #include "tc_common.cuh"
 
 namespace mg {
 
 MG_DEFINE_STATUS_ACCESSOR(kv4_attention_device_status)
-
-struct Kv4AttentionParams {
-  Kv4Cache cache;
-  const uint16_t *q;   // [B, S, H, D]
-  uint16_t *out;       // [B, S, H, D]
-  const int *lengths;  // [B]
-  float *weights;      // [B, KV, capacity] or null
-  float *lse;          // [B, KV, rows] or null: log2 of the sum of exp2(score), scores in units of log 2
-  int seq, heads, group;
-  int window, sinks;   // window 0: none
-  float scale_log2;    // softmax scale * log2(e)
-};
-
-// The blocks of 16 entries that rows of positions lo .. hi see: those that hold first entries, then those of the window.
-struct Kv4Range {
-  int first_blocks, window_block, blocks;
-  __device__ __forceinline__ int block(int i) const { return i < first_blocks ? i : window_block + (i - first_blocks); }
-};
-
-__device__ __forceinline__ Kv4Range kv4_range(int lo, int hi, int window, int sinks, int capacity) {
-  Kv4Range r;
-  const int end = min(hi + 1, capacity);  // entries 0 .. end - 1 at most
-  if (end <= 0) {
-    r.first_blocks = r.window_block = r.blocks = 0;
-    return r;
-  }
-  const int start = window > 0 ? max(0, lo - window + 1) : 0;
-  r.first_blocks = start > 0 ? (min(sinks, end) + 15) >> 4 : 0;
-  r.window_block = max(start >> 4, r.first_blocks);
-  r.blocks = r.first_blocks + max(0, ((end + 15) >> 4) - r.window_block);
-  return r;
-}
-
-__device__ __forceinline__ bool kv4_sees(int p, int j, int window, int sinks) {
-  return j <= p && (window == 0 || j > p - window || j < sinks);
-}
 
 // Rows r0 .. r0 + 7 of a key/value head as operands: lane (g, t) holds of row g the channels that lane t of a K row's words has,
 // in the order in which the masks take them out of a word; and the constants of the rows that its results are for, 2t and 2t + 1.
@@ -189,25 +154,8 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   return r;
 }
 
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Codes of two neighbours less 8, exact: 1024 + c and 1024 + 16 c are fp16 numbers with the code in their last bits.
-__device__ __forceinline__ uint32_t centred_low(uint32_t w) {
-  uint32_t r = (w & 0x000F000Fu) | 0x64006400u;
-  asm("add.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0xE408E408u));  // - 1032
-  return r;
-}
-__device__ __forceinline__ uint32_t centred_high(uint32_t w) {
-  uint32_t r = (w & 0x00F000F0u) | 0x64006400u;
-  asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(r) : "r"(0x2C002C00u), "r"(0xD480D480u));  // / 16 - 72
-  return r;
-}
-
 constexpr int kKv4Warps = 8;
+constexpr int kKv4FewRows = 32;  // of a key/value head; more go to the tensor-core kernel
 
 // Up to 8 NT rows of one key/value head and sequence per cluster; its warps share out the blocks of 16 entries, one range each.
 // Every warp keeps its own running maximum; they are joined in shared memory, then over the cluster's CTAs through distributed
@@ -230,7 +178,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attention_kernel(const Kv4
   const int length = kv4_length(p.lengths, b, p.cache.capacity);
   const size_t first = static_cast<size_t>(blockIdx.z) * p.cache.capacity;
   const int pos_lo = length - p.seq + r0 / p.group, pos_hi = length - p.seq + (min(r0 + R, total) - 1) / p.group;
-  const Kv4Range range = kv4_range(pos_lo, pos_hi, p.window, p.sinks, p.cache.capacity);
+  const Kv4Range range = kv4_range<16>(pos_lo, pos_hi, p.window, p.sinks, p.cache.capacity);
   const int units = ctas * kKv4Warps, unit = cta * kKv4Warps + warp;
   const int from = static_cast<int>(static_cast<long long>(range.blocks) * unit / units);
   const int to = static_cast<int>(static_cast<long long>(range.blocks) * (unit + 1) / units);
@@ -282,10 +230,10 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attention_kernel(const Kv4
       for (int e = 0; e < 2; ++e)
         if (j0 + g + 8 * e > pos_hi) vs[e] = vl[e] = 0.f;
     }
-    grow |= fmaxf(vs[0], vs[1]) > 16.f * v_unit;
+    grow |= fmaxf(fabsf(vs[0]), fabsf(vs[1])) > 16.f * v_unit;
     // Maximum and unit may lag by a factor of 16: both cancel in the end, and fp16 has the room.
     if (__any_sync(0xffffffffu, grow)) {
-      float top = fmaxf(vs[0], vs[1]);
+      float top = fmaxf(fabsf(vs[0]), fabsf(vs[1]));
 #pragma unroll
       for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
       float rescale = 1.f;
@@ -502,7 +450,8 @@ template <typename T, int D, int NT> int kv4_attention_launch(const Kv4Attention
 }
 
 template <typename T, int D> int kv4_attention_dispatch(const Kv4AttentionParams &p, cudaStream_t stream, bool pdl) {
-  const int st = p.seq * p.group <= 8 ? kv4_attention_launch<T, D, 1>(p, stream, pdl) : kv4_attention_launch<T, D, 2>(p, stream, pdl);
+  const int st = p.seq * p.group > kKv4FewRows ? kv4_prompt_launch(p, std::is_same<T, __nv_bfloat16>::value, pdl, stream)
+                 : p.seq * p.group <= 8 ? kv4_attention_launch<T, D, 1>(p, stream, pdl) : kv4_attention_launch<T, D, 2>(p, stream, pdl);
   if (st != MG_OK || p.weights == nullptr) return st;
   const dim3 grid((p.cache.capacity + 127) / 128, p.cache.batch * p.cache.kv_heads);
   return launch_helper(kv4_weights_kernel<T, D>, grid, 256, stream, true, p);

@@ -1,0 +1,544 @@
+// Attention over the 4-bit cache for many rows (the mathematics: kv4_attention.cu), on the tensor cores: a CTA takes 256 rows of one
+// key/value head and goes over tiles of 128 entries.
+//
+//   * four producer warps turn a tile's codes into operands in shared memory, once for both halves of the rows: K as fp16 subnormals
+//     (one mask per two codes; the codes that sit 4 bits up meet a q that was divided by 16), V centred; and its scales and minima as fp32;
+//   * one warp issues the MMAs: S = Q K^T (M 128 rows, N 128 entries) into tensor memory, and O += P V with P read from there;
+//   * two times four warps, a thread per row, take S from tensor memory, scale, mask and exponentiate it and put P = p v_scale back as
+//     fp16 over it.  While one half does that, the MMAs of the other run.
+//
+// The accumulator stays in tensor memory.  It is only rescaled when a row's maximum has grown by more than a factor of 2^8 (P then has
+// up to 2^8 of its unit, which fp16 holds), which after the first tiles is rare.  Fp32 work goes two numbers an instruction.
+// Every mbarrier wait is bounded; a warp that gives up hands nothing on, so that the others give up in turn; the issuing warp stays until
+// its MMAs have ended and tensor memory is freed on every path.
+#include <cuda_runtime.h>
+
+#include <cfloat>
+
+#include "../../include/matgptq_b200.h"
+#include "async.cuh"
+#include "helper_kernels.cuh"
+#include "host_util.h"
+#include "kernels.h"
+#include "kv4_attention.cuh"
+#include "tc_common.cuh"
+
+namespace mg {
+
+MG_DEFINE_STATUS_ACCESSOR(kv4_prompt_device_status)
+
+constexpr int kPrRows = 256, kPrTile = 128;   // rows of a CTA, entries of a tile
+constexpr int kPrWarps = 13;                  // 8 of softmax, 4 producers, 1 that issues
+// Shared memory: barriers, Q, two stages of K, V and params.
+constexpr int kPrBarKFull = 0, kPrBarVFull = 16, kPrBarEmpty = 32, kPrBarS = 48, kPrBarP = 64, kPrBarQ = 80, kPrBarEnd = 88, kPrTmemSlot = 96,
+              kPrUnit = 104 /* unit of P of each stage */, kPrMax = 112 /* four warps' maxima */;
+template <int D> struct PromptPlan {
+  static constexpr int q = 1024, q_bytes = 128 * D * 2;                    // per half
+  static constexpr int stages = q + 2 * q_bytes, k_bytes = kPrTile * D * 2;  // K and V have the same size
+  static constexpr int params = stages + 4 * k_bytes, param_bytes = 4 * kPrTile * 4;
+  static constexpr int end = params + 2 * param_bytes;
+};
+
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 32 columns of this warp's 32 lanes of tensor memory, and back; the caller waits
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
+      "%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+        "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
+        "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]),
+        "=r"(v[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]),
+      "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      "  .reg .pred p;\n"
+      "  setp.ne.b32 p, %4, 0;\n"
+      "  tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void sts_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void sts_f32(uint32_t addr, float a) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(a) : "memory"); }
+__device__ __forceinline__ float lds_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void lds_2x64(uint32_t addr, uint64_t &a, uint64_t &b) {
+  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(addr) : "memory");
+}
+
+// the lowest n of 32 bits
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+// What a thread keeps of its row
+struct PromptRow {
+  float unit, sum;   // log2 of a weight per score, score per minimum of K
+  float m;           // maximum so far, a whole number of log2
+  float v_unit;      // unit of P, and of the accumulator
+  uint64_t l2, fix2; // sums of the weights, and of the weights times the centres; two halves each
+};
+
+// A thread's row over a tile of 128 entries: S from tensor memory, P back over it.  Entry c of the tile is seen when c <= hi and
+// (c > lo or c < sk); WHOLE: all are.  `started`: the accumulator at t_o holds something.
+template <bool WHOLE, int D>
+__device__ __forceinline__ void prompt_tile(PromptRow &r, uint32_t t_s, uint32_t t_o, uint32_t par, float unit_now, bool started, int hi, int lo,
+                                            int sk) {
+  const uint64_t sum2 = pack2(r.sum, r.sum), unit2 = pack2(r.unit, r.unit);
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    union {
+      uint32_t u[32];
+      uint64_t d[16];
+    } s;
+    tmem_ld32(t_s + 32 * c, s.u);
+    uint32_t seen = 0xffffffffu;
+    if (!WHOLE) seen = bits_below(hi + 1 - 32 * c) & (~bits_below(lo + 1 - 32 * c) | bits_below(sk - 32 * c));
+    const uint32_t at = par + 32 * 4 * c;
+    tmem_wait_ld();
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      uint64_t ks[2], kl[2];
+      lds_2x64(at + i * 8, ks[0], ks[1]);
+      lds_2x64(at + kPrTile * 4 + i * 8, kl[0], kl[1]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        s.d[i + k] = fma2(ks[k], s.d[i + k], mul2(kl[k], sum2));
+        float x, y;
+        unpack2(s.d[i + k], x, y);
+        if (WHOLE || ((seen >> (2 * (i + k))) & 1u)) top = fmaxf(top, x);
+        if (WHOLE || ((seen >> (2 * (i + k) + 1)) & 1u)) top = fmaxf(top, y);
+      }
+    }
+    top *= r.unit;
+    // The maximum may lag by 2^8; whole numbers keep the factors powers of two, which P in fp16 takes without another rounding.
+    if (__any_sync(0xffffffffu, top > r.m + 8.f || r.v_unit != unit_now)) {
+      const float m_new = fmaxf(r.m, ceilf(top));
+      const float f = r.m == -INFINITY ? 0.f : exp2_approx(r.m - m_new);
+      r.m = m_new;
+      const uint64_t f2 = pack2(f, f);
+      r.l2 = mul2(r.l2, f2);
+      r.fix2 = mul2(r.fix2, f2);
+      const float g = f * (r.v_unit / unit_now);
+      if (started) {
+        // the accumulator is at rest: S of this tile was asked for after P V of the last one
+#pragma unroll 1
+        for (int col = 0; col < D; col += 16) {
+          uint32_t o[16];
+          tmem_ld16(t_o + col, o);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * g);
+          tmem_st16(t_o + col, o);
+        }
+      }
+      // the first 32 c entries' P, if any: its unit is this tile's already
+      tmem_wait_st();
+      const __half2 f16 = __float2half2_rn(f);
+#pragma unroll 1
+      for (int col = 0; col < 16 * c; col += 16) {
+        uint32_t o[16];
+        tmem_ld16(t_s + col, o);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const __half2 x = __hmul2(*reinterpret_cast<const __half2 *>(&o[i]), f16);
+          o[i] = *reinterpret_cast<const uint32_t *>(&x);
+        }
+        tmem_st16(t_s + col, o);
+      }
+      r.v_unit = unit_now;
+    }
+    const float shift = r.m == -INFINITY ? 0.f : -r.m;
+    const uint64_t shift2 = pack2(shift, shift);
+    uint32_t pv[16];
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      uint64_t vs[2], mid[2];
+      lds_2x64(at + 2 * kPrTile * 4 + i * 8, vs[0], vs[1]);
+      lds_2x64(at + 3 * kPrTile * 4 + i * 8, mid[0], mid[1]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float x, y;
+        unpack2(fma2(s.d[i + k], unit2, shift2), x, y);
+        x = exp2_approx(x);
+        y = exp2_approx(y);
+        if (!WHOLE) {  // hidden entries may hold a NaN: nothing of theirs is multiplied
+          float m0, m1, v0, v1;
+          unpack2(mid[k], m0, m1);
+          unpack2(vs[k], v0, v1);
+          if (!((seen >> (2 * (i + k))) & 1u)) x = 0.f, m0 = 0.f, v0 = 0.f;
+          if (!((seen >> (2 * (i + k) + 1)) & 1u)) y = 0.f, m1 = 0.f, v1 = 0.f;
+          mid[k] = pack2(m0, m1);
+          vs[k] = pack2(v0, v1);
+        }
+        const uint64_t p2 = pack2(x, y);
+        r.l2 = add2(r.l2, p2);
+        r.fix2 = fma2(p2, mid[k], r.fix2);
+        unpack2(mul2(p2, vs[k]), x, y);
+        const __half2 h = __floats2half2_rn(x, y);
+        pv[i + k] = *reinterpret_cast<const uint32_t *>(&h);
+      }
+    }
+    tmem_st16(t_s + 16 * c, pv);
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4AttentionParams p) {
+  using Plan = PromptPlan<D>;
+  extern __shared__ __align__(1024) unsigned char prompt_smem[];
+  const uint32_t base = smem_u32(prompt_smem);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  constexpr int kProducer = 8, kMma = 12;
+  if (warp == kMma) {
+    if (lane < 2) {
+      mbar_init(base + kPrBarKFull + 8 * lane, 4);
+      mbar_init(base + kPrBarVFull + 8 * lane, 4);
+      mbar_init(base + kPrBarEmpty + 8 * lane, 1);
+      mbar_init(base + kPrBarS + 8 * lane, 1);
+      mbar_init(base + kPrBarP + 8 * lane, 4);
+    }
+    if (lane == 0) {
+      mbar_init(base + kPrBarQ, 8);
+      mbar_init(base + kPrBarEnd, 1);
+    }
+    mbar_init_fence();
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(base + kPrTmemSlot) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(prompt_smem + kPrTmemSlot);
+  pdl_prologue();
+
+  const int b = blockIdx.y / p.cache.kv_heads, h = blockIdx.y - b * p.cache.kv_heads;
+  const int total = p.seq * p.group;
+  const int r0 = (gridDim.x - 1 - blockIdx.x) * kPrRows;  // the tiles with the most entries first
+  const int length = kv4_length(p.lengths, b, p.cache.capacity);
+  const size_t first = static_cast<size_t>(blockIdx.y) * p.cache.capacity;
+  const int pos_lo = length - p.seq + r0 / p.group, pos_hi = length - p.seq + (min(r0 + kPrRows, total) - 1) / p.group;
+  // the tiles that the rows see: those of first entries, then those of the window
+  const Kv4Range range = kv4_range<kPrTile>(pos_lo, pos_hi, p.window, p.sinks, p.cache.capacity);
+  const int tiles = range.blocks;
+  constexpr uint32_t kIdescS = 128, kChunkQ = 128 * 16, kChunkV = D * 16;
+  bool failed = false;
+
+  if (warp < kProducer) {
+    // ------------------------------------------------------------------ softmax: a thread per row
+    const int half = warp >> 2, quad = warp & 3;
+    const int row = r0 + threadIdx.x;  // of the key/value head
+    const bool live = row < total;
+    const int query = live ? row / p.group : 0;
+    const int pos = live ? length - p.seq + query : -1;
+    const int wg_lo = length - p.seq + (r0 + half * 128) / p.group;                                  // of this half's rows
+    const int wg_hi = length - p.seq + (min(r0 + half * 128 + 128, total) - 1) / p.group;
+    const size_t out_at = ((static_cast<size_t>(b) * p.seq + query) * p.heads + static_cast<size_t>(h) * p.group + (live ? row - query * p.group : 0)) * D;
+    // Q: scaled so that the largest value lies in [2^8, 2^9), which leaves the values divided by 16 their bits
+    float unit, sum = 0.f;
+    {
+      const uint16_t *src = p.q + out_at;
+      float top = 0.f;
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 raw = make_uint4(0, 0, 0, 0);
+        if (live) raw = *reinterpret_cast<const uint4 *>(src + 8 * c);
+        const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          top = fmaxf(top, fmaxf(fabsf(kv4_to_f<T>(static_cast<uint16_t>(u[i]))), fabsf(kv4_to_f<T>(static_cast<uint16_t>(u[i] >> 16)))));
+      }
+      const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 16), 253);
+      const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * (p.scale_log2 < 0.f ? -256.f : 256.f);
+      unit = __uint_as_float(static_cast<uint32_t>(e) << 23) * (fabsf(p.scale_log2) * 65536.f);  // 2^24 / 2^8
+      const uint32_t dst = base + Plan::q + half * Plan::q_bytes + (quad * 32 + lane) * 16;
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 raw = make_uint4(0, 0, 0, 0);
+        if (live) raw = *reinterpret_cast<const uint4 *>(src + 8 * c);
+        const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+        uint32_t x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float v = kv4_to_f<T>(static_cast<uint16_t>(u[i >> 1] >> (16 * (i & 1)))) * down;
+          const __half q16 = __float2half_rn(v);
+          sum += __half2float(q16);
+          x[i] = __half_as_ushort(i & 1 ? __float2half_rn(__half2float(q16) * 0.0625f) : q16);
+        }
+        sts_v4(dst + c * kChunkQ, x[0] | x[4] << 16, x[1] | x[5] << 16, x[2] | x[6] << 16, x[3] | x[7] << 16);
+      }
+      sum *= 0x1p-24f;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) mbar_arrive(base + kPrBarQ);
+
+    const uint32_t t_s = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * 128;
+    const uint32_t t_o = tmem + (static_cast<uint32_t>(quad * 32) << 16) + 256 + half * D;
+    PromptRow r = {unit, sum, -INFINITY, 0.f, 0, 0};
+    for (int t = 0; t < tiles; ++t) {
+      const int stage = t & 1;
+      if (!mbar_wait_chain(base + kPrBarS + 8 * half, t & 1) || !mbar_wait_chain(base + kPrBarVFull + 8 * stage, (t >> 1) & 1)) {
+        failed = true;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t par = base + Plan::params + stage * Plan::param_bytes;
+      const float unit_now = lds_f32(base + kPrUnit + 4 * stage);
+      const int j0 = range.block(t) * kPrTile;
+      const bool whole = j0 + kPrTile - 1 <= wg_lo && (p.window == 0 || j0 > wg_hi - p.window || j0 + kPrTile <= p.sinks);
+      const int hi = pos - j0, lo = p.window > 0 ? hi - p.window : -1, sk = p.sinks - j0;
+      if (whole)
+        prompt_tile<true, D>(r, t_s, t_o, par, unit_now, t > 0, hi, lo, sk);
+      else
+        prompt_tile<false, D>(r, t_s, t_o, par, unit_now, t > 0, hi, lo, sk);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(base + kPrBarP + 8 * half);
+    }
+    if (!failed && tiles > 0 && !mbar_wait_chain(base + kPrBarEnd, 0)) failed = true;
+    if (failed) {
+      report_status(kStatusMmaTimeout);
+    } else {
+      tc_fence_after();
+      float l0, l1, f0, f1;
+      unpack2(r.l2, l0, l1);
+      unpack2(r.fix2, f0, f1);
+      const float l = l0 + l1, fix = f0 + f1, inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
+      // column i D/4 + u of the accumulator is channel 4 u + i
+      constexpr int U = D / 4;
+#pragma unroll
+      for (int u0 = 0; u0 < U; u0 += 16) {
+        uint32_t o[4][16];
+        if (tiles > 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tmem_ld16(t_o + i * U + u0, o[i]);
+        }
+        if (live) {
+#pragma unroll
+          for (int u = 0; u < 16; u += 2) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              uint16_t c[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) c[i] = kv4_bits<T>(l == 0.f ? 0.f : fmaf(__uint_as_float(o[i][u + k]), r.v_unit, fix) * inv);
+              w[2 * k] = c[0] | static_cast<uint32_t>(c[1]) << 16;
+              w[2 * k + 1] = c[2] | static_cast<uint32_t>(c[3]) << 16;
+            }
+            *reinterpret_cast<uint4 *>(p.out + out_at + 4 * (u0 + u)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      if (p.lse != nullptr && live) p.lse[static_cast<size_t>(blockIdx.y) * total + row] = l == 0.f ? INFINITY : r.m + log2f(l);
+    }
+  } else if (warp < kMma) {
+    // ------------------------------------------------------------------ producers
+    const int pw = warp - kProducer, tid = threadIdx.x - kProducer * 32;
+    constexpr int KW = D / 8;            // words of a K row, one per thread
+    constexpr int U = D / 4;             // units of a V pair
+    constexpr int G = 32 / U;            // groups of 8 entries that a warp takes at once
+    constexpr int VP = 16 / (4 * G);     // passes over the 16 groups of a tile
+    uint32_t kw[KW], vw[VP][4];
+    uint2 par = make_uint2(0, 0);
+    const int unit_lane = lane & (U - 1), group0 = G * pw + (G == 2 ? lane >> 4 : 0);
+    auto load = [&](int t) {
+      const int j0 = range.block(t) * kPrTile;
+      const bool there = j0 + tid < p.cache.capacity;
+      const uint8_t *kr = p.cache.k + (first + j0 + (there ? tid : 0)) * (D / 2);
+#pragma unroll
+      for (int i = 0; i < KW; i += 4) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (there) x = *reinterpret_cast<const uint4 *>(kr + 4 * i);
+        kw[i] = x.x, kw[i + 1] = x.y, kw[i + 2] = x.z, kw[i + 3] = x.w;
+      }
+      // entries that no row sees may hold anything: their scales and minima are taken as zero
+      par = make_uint2(0, 0);
+      if (j0 + tid <= min(pos_hi, p.cache.capacity - 1)) par = *reinterpret_cast<const uint2 *>(p.cache.params + (first + j0 + tid) * 4);
+#pragma unroll
+      for (int v = 0; v < VP; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int pair = (j0 >> 1) + 4 * (group0 + 4 * G * v) + i;
+          vw[v][i] = 0;
+          if (2 * pair < p.cache.capacity) vw[v][i] = *reinterpret_cast<const uint32_t *>(p.cache.v + ((first >> 1) + pair) * D + 4 * unit_lane);
+        }
+    };
+    float v_unit = 0x1p-100f;
+    if (tiles > 0) load(0);
+    for (int t = 0; t < tiles; ++t) {
+      const int stage = t & 1;
+      // a warp that gives up goes on through the named barriers, which the others wait at, but hands nothing on
+      if (!failed && !mbar_wait_chain(base + kPrBarEmpty + 8 * stage, ((t >> 1) & 1) ^ 1)) failed = true;
+      const uint32_t k_at = base + Plan::stages + stage * 2 * Plan::k_bytes, v_at = k_at + Plan::k_bytes;
+#pragma unroll
+      for (int i = 0; i < KW; ++i) {
+        const uint32_t x = kw[i], y = x >> 8;
+        sts_v4(k_at + i * kChunkQ + tid * 16, x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0 && !failed) mbar_arrive(base + kPrBarKFull + 8 * stage);
+      // the unit of P: a power of two within a factor of 16 of the tile's largest v_scale, or larger
+      const float ks = kv4_to_f<T>(static_cast<uint16_t>(par.x)), kl = kv4_to_f<T>(static_cast<uint16_t>(par.x >> 16));
+      const float vs = kv4_to_f<T>(static_cast<uint16_t>(par.y)), vl = kv4_to_f<T>(static_cast<uint16_t>(par.y >> 16));
+      const float mine = fabsf(vs) <= FLT_MAX ? fabsf(vs) : 0.f;
+      const uint32_t top_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(mine));
+      if (lane == 0) sts_f32(base + kPrMax + 4 * pw, __uint_as_float(top_bits));
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, lds_f32(base + kPrMax + 4 * i));
+      if (top > 16.f * v_unit) v_unit = __uint_as_float(static_cast<uint32_t>(min(max(static_cast<int>(__float_as_uint(top) >> 23), 27), 250)) << 23);
+      const float v_per = __uint_as_float(static_cast<uint32_t>(254 - (__float_as_uint(v_unit) >> 23)) << 23);
+      const uint32_t at = base + Plan::params + stage * Plan::param_bytes + tid * 4;
+      sts_f32(at, ks);
+      sts_f32(at + kPrTile * 4, kl);
+      sts_f32(at + 2 * kPrTile * 4, vs * v_per);
+      sts_f32(at + 3 * kPrTile * 4, fmaf(8.f, vs, vl));
+      if (tid == 0) sts_f32(base + kPrUnit + 4 * stage, v_unit);
+#pragma unroll
+      for (int v = 0; v < VP; ++v) {
+        const uint32_t dst = v_at + (group0 + 4 * G * v) * kChunkV + unit_lane * 16;
+        const uint32_t *w = vw[v];
+        sts_v4(dst, centred_low(w[0]), centred_low(w[1]), centred_low(w[2]), centred_low(w[3]));
+        sts_v4(dst + U * 16, centred_high(w[0]), centred_high(w[1]), centred_high(w[2]), centred_high(w[3]));
+        sts_v4(dst + 2 * U * 16, centred_low(w[0] >> 8), centred_low(w[1] >> 8), centred_low(w[2] >> 8), centred_low(w[3] >> 8));
+        sts_v4(dst + 3 * U * 16, centred_high(w[0] >> 8), centred_high(w[1] >> 8), centred_high(w[2] >> 8), centred_high(w[3] >> 8));
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0 && !failed) mbar_arrive(base + kPrBarVFull + 8 * stage);
+      if (t + 1 < tiles) load(t + 1);
+      asm volatile("bar.sync 1, 128;" ::: "memory");  // the maxima have been read
+    }
+    if (failed) report_status(kStatusWeightCopyTimeout);
+  } else {
+    if (warp == kMma) {
+      // ---------------------------------------------------------------- MMAs
+      const uint32_t idesc_s = umma_instr_desc(0, kIdescS), idesc_o = umma_instr_desc(0, D);
+      const uint64_t dq = umma_smem_desc(base + Plan::q, kChunkQ, 128, 0);
+      const uint64_t dk = umma_smem_desc(base + Plan::stages, kChunkQ, 128, 0);
+      const uint64_t dv = umma_smem_desc(base + Plan::stages + Plan::k_bytes, kChunkV, 128, 0);
+      auto scores = [&](int half, int stage) {  // by one lane
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          umma_f16(tmem + half * 128, dq + half * (Plan::q_bytes >> 4) + k * (2 * kChunkQ >> 4),
+                   dk + stage * (2 * Plan::k_bytes >> 4) + k * (2 * kChunkQ >> 4), idesc_s, k > 0);
+        umma_commit(base + kPrBarS + 8 * half);
+      };
+      if (tiles > 0) {
+        if (!mbar_wait_chain(base + kPrBarQ, 0) || !mbar_wait_chain(base + kPrBarKFull, 0)) failed = true;
+        tc_fence_after();
+        if (!failed && elect_one()) {
+          scores(0, 0);
+          scores(1, 0);
+        }
+        __syncwarp();
+      }
+      for (int t = 0; t < tiles && !failed; ++t) {
+        const int stage = t & 1, next = stage ^ 1;
+        if (!mbar_wait_chain(base + kPrBarVFull + 8 * stage, (t >> 1) & 1)) {
+          failed = true;
+          break;
+        }
+        for (int half = 0; half < 2; ++half) {
+          if (!mbar_wait_chain(base + kPrBarP + 8 * half, t & 1) ||
+              (half == 0 && t + 1 < tiles && !mbar_wait_chain(base + kPrBarKFull + 8 * next, ((t + 1) >> 1) & 1))) {
+            failed = true;
+            break;
+          }
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < kPrTile / 16; ++k)
+              mma_ts(tmem + 256 + half * D, tmem + half * 128 + k * 8, dv + stage * (2 * Plan::k_bytes >> 4) + k * (2 * kChunkV >> 4), idesc_o,
+                     (t > 0 || k > 0) ? 1u : 0u);
+            if (half == 1) umma_commit(base + kPrBarEmpty + 8 * stage);
+            if (t + 1 < tiles) scores(half, next);
+          }
+          __syncwarp();
+        }
+      }
+      // nothing of this CTA may be in flight when it frees its memory
+      if (elect_one()) umma_commit(base + kPrBarEnd);
+      __syncwarp();
+      if (!mbar_wait_chain(base + kPrBarEnd, 0)) failed = true;
+      if (failed) report_status(kStatusMmaTimeout);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+namespace {
+
+template <typename T, int D> int launch_prompt(const Kv4AttentionParams &p, bool pdl, cudaStream_t stream) {
+  constexpr int smem = PromptPlan<D>::end;
+  static SharedMemoryOptIn opt_in;
+  const int st = opt_in.ensure(kv4_prompt_kernel<T, D>, smem);
+  if (st != MG_OK) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((p.seq * p.group + kPrRows - 1) / kPrRows, p.cache.batch * p.cache.kv_heads);
+  cfg.blockDim = dim3(kPrWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, p) == cudaSuccess ? MG_OK : MG_ERR_CUDA;
+}
+
+}  // namespace
+
+int kv4_prompt_launch(const Kv4AttentionParams &p, bool bf16, bool pdl, cudaStream_t stream) {
+  if (p.cache.dim == 64) return bf16 ? launch_prompt<__nv_bfloat16, 64>(p, pdl, stream) : launch_prompt<__half, 64>(p, pdl, stream);
+  return bf16 ? launch_prompt<__nv_bfloat16, 128>(p, pdl, stream) : launch_prompt<__half, 128>(p, pdl, stream);
+}
+
+}  // namespace mg
