@@ -274,7 +274,7 @@ int matgptq_b200_argmax(const void *logits, int64_t *out, int64_t rows, int64_t 
  *   k_codes [batch, n_kv_heads, capacity, head_dim/2] bytes: byte i holds channels 2i (low half) and 2i + 1
  *   v_codes [batch, n_kv_heads, capacity/2, head_dim] bytes: the rows of entries 2p and 2p + 1, in turns of two bytes
  *   params  [batch, n_kv_heads, capacity, 4] T: scale and minimum of K, scale and minimum of V
- * A code c stands for minimum + scale * c.  head_dim is 64 or 128, capacity a multiple of 64, batch * n_kv_heads at most 65535, the
+ * A code c stands for minimum + scale * c.  head_dim is 64 or 128, capacity a multiple of 64 up to 2^28, batch * n_kv_heads at most 65535, the
  * three pointers 16-byte aligned.
  * lengths[batch] (int32) counts the entries of each sequence, the tokens of the call among them: token i of `seq` is entry
  * lengths[b] - seq + i.  Where that is negative the token is padding (a prompt padded on the left): nothing is read or written for
@@ -303,9 +303,9 @@ int matgptq_b200_append_kv4(const matgptq_b200_kv4_cache *cache, const void *qkv
  * and sinks count entries.  A query that sees nothing gives zeros.  Head h reads key/value head h / (n_heads / n_kv_heads).
  * With weights[batch, n_kv_heads, capacity] (fp32, may be NULL) each entry's softmax weights, summed over the queries and heads that
  * share it, are added to what is there, in a fixed order; this needs matgptq_b200_attention_kv4_workspace_bytes(...) bytes of
- * workspace (its contents do not matter; one per call in flight).  K and V are not rounded; sums are fp32.
+ * workspace (16-byte aligned; its contents do not matter; one per call in flight).  K and V are not rounded; sums are fp32.
  */
-int64_t matgptq_b200_attention_kv4_workspace_bytes(int64_t batch, int64_t seq, int64_t n_heads, int with_weights);
+int64_t matgptq_b200_attention_kv4_workspace_bytes(const matgptq_b200_kv4_cache *cache, int64_t seq, int64_t n_heads, int with_weights);
 int matgptq_b200_attention_kv4(const matgptq_b200_kv4_cache *cache, const void *q, int64_t seq, int64_t n_heads, const int32_t *lengths,
                                int64_t window, int64_t sinks, float scale, float *weights, void *out, void *workspace,
                                int64_t workspace_bytes, uint32_t flags, void *stream);

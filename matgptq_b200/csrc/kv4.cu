@@ -320,7 +320,7 @@ namespace mg {
 
 int kv4_check_cache(const matgptq_b200_kv4_cache *c) {
   if (!c || !c->k_codes || !c->v_codes || !c->params) return MG_ERR_BAD_ARG;
-  if (c->batch < 0 || c->n_kv_heads <= 0 || c->n_kv_heads > (1 << 16) || c->capacity <= 0 || c->capacity > (1 << 30)) return MG_ERR_BAD_ARG;
+  if (c->batch < 0 || c->n_kv_heads <= 0 || c->n_kv_heads > (1 << 16) || c->capacity <= 0 || c->capacity > (1 << 28)) return MG_ERR_BAD_ARG;
   if (c->capacity % 64 != 0) return MG_ERR_BAD_ARG;
   if (c->batch > 65535 || c->batch * c->n_kv_heads > 65535) return MG_ERR_UNSUPPORTED;
   if (c->head_dim != 64 && c->head_dim != 128) return MG_ERR_UNSUPPORTED;

@@ -16,7 +16,6 @@
 
 #include <algorithm>
 #include <cfloat>
-#include <type_traits>
 
 #include "../../include/matgptq_b200.h"
 #include "async.cuh"
@@ -155,7 +154,6 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
 }
 
 constexpr int kKv4Warps = 8;
-constexpr int kKv4FewRows = 32;  // of a key/value head; more go to the tensor-core kernel
 
 // Up to 8 NT rows of one key/value head and sequence per cluster; its warps share out the blocks of 16 entries, one range each.
 // Every warp keeps its own running maximum; they are joined in shared memory, then over the cluster's CTAs through distributed
@@ -450,8 +448,7 @@ template <typename T, int D, int NT> int kv4_attention_launch(const Kv4Attention
 }
 
 template <typename T, int D> int kv4_attention_dispatch(const Kv4AttentionParams &p, cudaStream_t stream, bool pdl) {
-  const int st = p.seq * p.group > kKv4FewRows ? kv4_prompt_launch(p, std::is_same<T, __nv_bfloat16>::value, pdl, stream)
-                 : p.seq * p.group <= 8 ? kv4_attention_launch<T, D, 1>(p, stream, pdl) : kv4_attention_launch<T, D, 2>(p, stream, pdl);
+  const int st = p.seq * p.group <= 8 ? kv4_attention_launch<T, D, 1>(p, stream, pdl) : kv4_attention_launch<T, D, 2>(p, stream, pdl);
   if (st != MG_OK || p.weights == nullptr) return st;
   const dim3 grid((p.cache.capacity + 127) / 128, p.cache.batch * p.cache.kv_heads);
   return launch_helper(kv4_weights_kernel<T, D>, grid, 256, stream, true, p);
@@ -460,6 +457,7 @@ template <typename T, int D> int kv4_attention_dispatch(const Kv4AttentionParams
 }  // namespace
 
 int kv4_attention(const Kv4AttentionParams &p, bool bf16, bool pdl, cudaStream_t stream) {
+  if (p.seq * p.group > kKv4FewRows) return kv4_prompt_launch(p, bf16, pdl, stream);
   if (p.cache.dim == 64)
     return bf16 ? kv4_attention_dispatch<__nv_bfloat16, 64>(p, stream, pdl) : kv4_attention_dispatch<__half, 64>(p, stream, pdl);
   return bf16 ? kv4_attention_dispatch<__nv_bfloat16, 128>(p, stream, pdl) : kv4_attention_dispatch<__half, 128>(p, stream, pdl);
@@ -469,8 +467,10 @@ int kv4_attention(const Kv4AttentionParams &p, bool bf16, bool pdl, cudaStream_t
 
 extern "C" {
 
-int64_t matgptq_b200_attention_kv4_workspace_bytes(int64_t batch, int64_t seq, int64_t n_heads, int with_weights) {
-  return with_weights && batch > 0 && seq > 0 && n_heads > 0 ? batch * seq * n_heads * 4 : 0;
+int64_t matgptq_b200_attention_kv4_workspace_bytes(const matgptq_b200_kv4_cache *cache, int64_t seq, int64_t n_heads, int with_weights) {
+  if (!cache || !with_weights || cache->batch <= 0 || cache->n_kv_heads <= 0 || seq <= 0 || n_heads < cache->n_kv_heads) return 0;
+  const int64_t rows = seq * (n_heads / cache->n_kv_heads), heads = cache->batch * cache->n_kv_heads;
+  return rows <= mg::kKv4FewRows ? heads * rows * 4 : heads * ((rows + 127) / 128) * mg::kv4_row_tile_bytes(static_cast<int>(cache->head_dim));
 }
 
 int matgptq_b200_attention_kv4(const matgptq_b200_kv4_cache *cache, const void *q, int64_t seq, int64_t n_heads, const int32_t *lengths,
@@ -483,15 +483,17 @@ int matgptq_b200_attention_kv4(const matgptq_b200_kv4_cache *cache, const void *
   if (seq > (1 << 24) || n_heads > (1 << 16) || seq * (n_heads / cache->n_kv_heads) > (1 << 24)) return MG_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 != 0) return MG_ERR_ALIGNMENT;
   if (cache->batch == 0 || seq == 0) return MG_OK;
-  if (weights && (!workspace || workspace_bytes < matgptq_b200_attention_kv4_workspace_bytes(cache->batch, seq, n_heads, 1)))
-    return MG_ERR_BAD_ARG;
+  if (weights && (!workspace || workspace_bytes < matgptq_b200_attention_kv4_workspace_bytes(cache, seq, n_heads, 1))) return MG_ERR_BAD_ARG;
+  if (weights && reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return MG_ERR_ALIGNMENT;
   mg::Kv4AttentionParams p = {};
   p.cache = mg::kv4_cache(cache);
   p.q = static_cast<const uint16_t *>(q);
   p.out = static_cast<uint16_t *>(out);
   p.lengths = lengths;
   p.weights = weights;
-  p.lse = weights ? static_cast<float *>(workspace) : nullptr;
+  const bool few = seq * (n_heads / cache->n_kv_heads) <= mg::kKv4FewRows;
+  p.lse = weights && few ? static_cast<float *>(workspace) : nullptr;
+  p.row_tiles = weights && !few ? static_cast<uint8_t *>(workspace) : nullptr;
   p.seq = static_cast<int>(seq);
   p.heads = static_cast<int>(n_heads);
   p.group = static_cast<int>(n_heads / cache->n_kv_heads);

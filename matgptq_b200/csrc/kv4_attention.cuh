@@ -10,7 +10,8 @@ struct Kv4AttentionParams {
   uint16_t *out;       // [B, S, H, D]
   const int *lengths;  // [B]
   float *weights;      // [B, KV, capacity] or null
-  float *lse;          // [B, KV, rows] or null: log2 of the sum of exp2(score), scores in units of log 2
+  float *lse;          // few rows: [B, KV, rows] or null: log2 of the sum of exp2(score), scores in units of log 2
+  uint8_t *row_tiles;  // many rows: [B, KV, tiles of 128 rows, kv4_row_tile_bytes] or null
   int seq, heads, group;
   int window, sinks;   // window 0: none
   float scale_log2;    // softmax scale * log2(e)
@@ -57,6 +58,12 @@ __device__ __forceinline__ uint32_t centred_high(uint32_t w) {
   asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(r) : "r"(0x2C002C00u), "r"(0xD480D480u));  // / 16 - 72
   return r;
 }
+
+constexpr int kKv4FewRows = 32;  // of a key/value head, for kv4_attention.cu; more go to kv4_prompt.cu
+
+// What the second pass over many rows, for the weights, reads of 128 rows: q as the operand it is in shared memory, then three
+// numbers for each row: log2 of a weight per score, per minimum of K, and the log2 of the row's sum.
+__host__ __device__ constexpr int kv4_row_tile_bytes(int dim) { return 128 * dim * 2 + 3 * 128 * 4; }
 
 // kv4_prompt.cu
 int kv4_prompt_launch(const Kv4AttentionParams &p, bool bf16, bool pdl, cudaStream_t stream);

@@ -275,6 +275,10 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
     const int wg_lo = length - p.seq + (r0 + half * 128) / p.group;                                  // of this half's rows
     const int wg_hi = length - p.seq + (min(r0 + half * 128 + 128, total) - 1) / p.group;
     const size_t out_at = ((static_cast<size_t>(b) * p.seq + query) * p.heads + static_cast<size_t>(h) * p.group + (live ? row - query * p.group : 0)) * D;
+    // this row's tile for the pass that adds up the weights, where there is one
+    uint8_t *tile_out = nullptr;
+    if (p.row_tiles != nullptr && r0 + half * 128 < total)
+      tile_out = p.row_tiles + (static_cast<size_t>(blockIdx.y) * ((total + 127) / 128) + (r0 >> 7) + half) * kv4_row_tile_bytes(D);
     // Q: scaled so that the largest value lies in [2^8, 2^9), which leaves the values divided by 16 their bits
     float unit, sum = 0.f;
     {
@@ -306,7 +310,9 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
           sum += __half2float(q16);
           x[i] = __half_as_ushort(i & 1 ? __float2half_rn(__half2float(q16) * 0.0625f) : q16);
         }
-        sts_v4(dst + c * kChunkQ, x[0] | x[4] << 16, x[1] | x[5] << 16, x[2] | x[6] << 16, x[3] | x[7] << 16);
+        const uint4 chunk = make_uint4(x[0] | x[4] << 16, x[1] | x[5] << 16, x[2] | x[6] << 16, x[3] | x[7] << 16);
+        sts_v4(dst + c * kChunkQ, chunk.x, chunk.y, chunk.z, chunk.w);
+        if (tile_out != nullptr) *reinterpret_cast<uint4 *>(tile_out + c * kChunkQ + (quad * 32 + lane) * 16) = chunk;
       }
       sum *= 0x1p-24f;
     }
@@ -372,7 +378,12 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
           }
         }
       }
-      if (p.lse != nullptr && live) p.lse[static_cast<size_t>(blockIdx.y) * total + row] = l == 0.f ? INFINITY : r.m + log2f(l);
+      if (tile_out != nullptr) {
+        float *numbers = reinterpret_cast<float *>(tile_out + 128 * D * 2) + quad * 32 + lane;
+        numbers[0] = unit;
+        numbers[128] = sum * unit;
+        numbers[256] = !live || l == 0.f ? INFINITY : r.m + log2f(l);
+      }
     }
   } else if (warp < kMma) {
     // ------------------------------------------------------------------ producers
@@ -514,7 +525,204 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
   if (warp == kMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
+// weights[j] += sum over the rows that see entry j of exp2(score - log2 of the row's sum).  A CTA takes 128 entries and goes over the
+// tiles of 128 rows that kv4_prompt_kernel left: S^T = K Q^T puts an entry in each lane of tensor memory and the rows in its
+// columns, so that a thread adds up one entry's weights, in the order of the rows, with no other to wait for.  Four warps do that; the
+// fifth requests the tiles (one copy each, they are operands already) and issues the MMAs, two accumulators in turn.  What bounds it
+// are the exponentials (16 a cycle and SM) and what goes with them.
+constexpr int kPwWarps = 5, kPwMma = 4;
+constexpr int kPwBarK = 0, kPwBarQFull = 8, kPwBarQEmpty = 24, kPwBarSFull = 40, kPwBarSEmpty = 56, kPwBarEnd = 72, kPwTmemSlot = 80;
+template <int D> struct WeightsPlan {
+  static constexpr int k = 1024, k_bytes = 128 * D * 2, q = k + k_bytes, q_bytes = kv4_row_tile_bytes(D), end = q + 2 * q_bytes;
+};
+
+template <typename T, int D> __global__ void __launch_bounds__(kPwWarps * 32) kv4_prompt_weights_kernel(const Kv4AttentionParams p) {
+  using Plan = WeightsPlan<D>;
+  extern __shared__ __align__(1024) unsigned char weights_smem[];
+  const uint32_t base = smem_u32(weights_smem);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  if (warp == kPwMma) {
+    if (lane == 0) {
+      mbar_init(base + kPwBarK, 4);
+      mbar_init(base + kPwBarEnd, 1);
+    }
+    if (lane < 2) {
+      mbar_init(base + kPwBarQFull + 8 * lane, 1);
+      mbar_init(base + kPwBarQEmpty + 8 * lane, 5);  // the MMAs and four warps
+      mbar_init(base + kPwBarSFull + 8 * lane, 1);
+      mbar_init(base + kPwBarSEmpty + 8 * lane, 4);
+    }
+    mbar_init_fence();
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(base + kPwTmemSlot) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(weights_smem + kPwTmemSlot);
+  pdl_prologue();
+
+  const int b = blockIdx.y / p.cache.kv_heads;
+  const int total = p.seq * p.group, length = kv4_length(p.lengths, b, p.cache.capacity), behind = length - p.seq;
+  const size_t first = static_cast<size_t>(blockIdx.y) * p.cache.capacity;
+  const int j0 = blockIdx.x * 128;
+  // rows that see entry j: [from(j), to(j)); both grow with j, but for the first entries, which every later row sees
+  const auto from = [&](int j) { return min(max(j - behind, 0), p.seq) * p.group; };
+  const auto to = [&](int j) { return p.window > 0 && j >= p.sinks ? min(max(j + p.window - behind, 0), p.seq) * p.group : total; };
+  const int last = min(j0 + 127, length - 1);
+  const int row_lo = from(j0), row_hi = j0 >= length ? 0 : j0 < p.sinks ? total : to(last);
+  const int tile_lo = row_lo >> 7, tiles = row_hi > row_lo ? ((row_hi + 127) >> 7) - tile_lo : 0;
+  bool failed = false;
+  if (tiles > 0 && warp < kPwMma) {
+    const int tid = threadIdx.x, j = j0 + tid;
+    uint2 par = make_uint2(0, 0);  // entries behind the last one may hold anything: no row sees them
+    {
+      const bool there = j < p.cache.capacity;
+      const uint8_t *kr = p.cache.k + (first + (there ? j : j0)) * (D / 2);
+#pragma unroll
+      for (int i = 0; i < D / 8; i += 4) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(kr + 4 * i);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t x = w[k], y = x >> 8;
+          sts_v4(base + Plan::k + (i + k) * 2048 + tid * 16, x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u);
+        }
+      }
+      if (j < length) par = *reinterpret_cast<const uint2 *>(p.cache.params + (first + j) * 4);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) mbar_arrive(base + kPwBarK);
+    const float ks = kv4_to_f<T>(static_cast<uint16_t>(par.x)), kl = kv4_to_f<T>(static_cast<uint16_t>(par.x >> 16));
+    const uint64_t ks2 = pack2(ks, ks), kl2 = pack2(kl, kl);
+    const int mine_lo = from(j), mine_hi = j < length ? to(j) : 0;
+    uint64_t sum2 = 0;
+    for (int t = 0; t < tiles; ++t) {
+      const int stage = t & 1, parity = (t >> 1) & 1;
+      if (!mbar_wait_chain(base + kPwBarQFull + 8 * stage, parity) || !mbar_wait_chain(base + kPwBarSFull + 8 * stage, parity)) {
+        failed = true;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t t_s = tmem + (static_cast<uint32_t>(warp * 32) << 16) + stage * 128;
+      const uint32_t numbers = base + Plan::q + stage * Plan::q_bytes + 128 * D * 2;
+      const int row0 = (tile_lo + t) * 128;
+      const bool whole = __all_sync(0xffffffffu, mine_lo <= row0 && mine_hi >= row0 + 128);
+      uint64_t tile2 = 0;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t s[32];
+        tmem_ld32(t_s + 32 * c, s);
+        const uint32_t seen = whole ? 0xffffffffu : bits_below(mine_hi - row0 - 32 * c) & ~bits_below(mine_lo - row0 - 32 * c);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          uint64_t unit[2], low[2], lse[2];
+          const uint32_t at = numbers + (32 * c + i) * 4;
+          lds_2x64(at, unit[0], unit[1]);
+          lds_2x64(at + 512, low[0], low[1]);
+          lds_2x64(at + 1024, lse[0], lse[1]);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float x, y, lx, ly;
+            const uint64_t raw = mul2(ks2, pack2(__uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1])));
+            unpack2(lse[k], lx, ly);
+            unpack2(fma2(raw, unit[k], fma2(kl2, low[k], pack2(-lx, -ly))), x, y);
+            x = exp2_approx(x);
+            y = exp2_approx(y);
+            if (!((seen >> (i + 2 * k)) & 1u)) x = 0.f;
+            if (!((seen >> (i + 2 * k + 1)) & 1u)) y = 0.f;
+            tile2 = add2(tile2, pack2(x, y));
+          }
+        }
+      }
+      sum2 = add2(sum2, tile2);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(base + kPwBarSEmpty + 8 * stage);
+        mbar_arrive(base + kPwBarQEmpty + 8 * stage);
+      }
+    }
+    float x, y;
+    unpack2(sum2, x, y);
+    if (j < length && !failed) p.weights[first + j] += x + y;
+    if (failed) report_status(kStatusMmaTimeout);
+  } else if (tiles > 0) {
+    const uint32_t idesc = umma_instr_desc(0, 128);
+    const uint64_t dk = umma_smem_desc(base + Plan::k, 2048, 128, 0), dq = umma_smem_desc(base + Plan::q, 2048, 128, 0);
+    const uint8_t *src = p.row_tiles + (static_cast<size_t>(blockIdx.y) * ((total + 127) / 128) + tile_lo) * Plan::q_bytes;
+    const auto request = [&](int t) {  // by one lane
+      const uint32_t bar = base + kPwBarQFull + 8 * (t & 1);
+      mbar_arrive_expect_tx(bar, Plan::q_bytes);
+      bulk_copy_g2s(base + Plan::q + (t & 1) * Plan::q_bytes, src + static_cast<size_t>(t) * Plan::q_bytes, Plan::q_bytes, bar);
+    };
+    int requested = 0;
+    if (elect_one())
+      for (int t = 0; t < min(tiles, 2); ++t) request(t);
+    requested = min(tiles, 2);
+    __syncwarp();
+    if (!mbar_wait_chain(base + kPwBarK, 0)) failed = true;
+    for (int t = 0; t < tiles && !failed; ++t) {
+      const int stage = t & 1, parity = (t >> 1) & 1;
+      if (!mbar_wait_chain(base + kPwBarQFull + 8 * stage, parity) || !mbar_wait_chain(base + kPwBarSEmpty + 8 * stage, parity ^ 1)) {
+        failed = true;
+        break;
+      }
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          umma_f16(tmem + stage * 128, dk + k * (2 * 2048 >> 4), dq + stage * (Plan::q_bytes >> 4) + k * (2 * 2048 >> 4), idesc, k > 0);
+        umma_commit(base + kPwBarSFull + 8 * stage);
+        umma_commit(base + kPwBarQEmpty + 8 * stage);
+      }
+      __syncwarp();
+      // the tile after the next one, into the stage that the tile before this one leaves
+      if (t >= 1 && t + 1 < tiles) {
+        if (!mbar_wait_chain(base + kPwBarQEmpty + 8 * (stage ^ 1), ((t - 1) >> 1) & 1)) {
+          failed = true;
+          break;
+        }
+        if (elect_one()) request(t + 1);
+        requested = t + 2;
+        __syncwarp();
+      }
+    }
+    // nothing of this CTA may be in flight when it frees its memory
+    if (elect_one()) umma_commit(base + kPwBarEnd);
+    __syncwarp();
+    if (!mbar_wait_chain(base + kPwBarEnd, 0)) failed = true;
+    for (int t = max(0, requested - 2); t < requested; ++t)
+      if (!mbar_wait_chain(base + kPwBarQFull + 8 * (t & 1), (t >> 1) & 1)) failed = true;
+    if (failed) report_status(kStatusMmaTimeout);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kPwMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
+}
+
 namespace {
+
+template <typename T, int D> int launch_prompt_weights(const Kv4AttentionParams &p, cudaStream_t stream) {
+  constexpr int smem = WeightsPlan<D>::end;
+  static SharedMemoryOptIn opt_in;
+  const int st = opt_in.ensure(kv4_prompt_weights_kernel<T, D>, smem);
+  if (st != MG_OK) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((p.cache.capacity + 127) / 128, p.cache.batch * p.cache.kv_heads);
+  cfg.blockDim = dim3(kPwWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_prompt_weights_kernel<T, D>, p) == cudaSuccess ? MG_OK : MG_ERR_CUDA;
+}
 
 template <typename T, int D> int launch_prompt(const Kv4AttentionParams &p, bool pdl, cudaStream_t stream) {
   constexpr int smem = PromptPlan<D>::end;
@@ -531,7 +739,8 @@ template <typename T, int D> int launch_prompt(const Kv4AttentionParams &p, bool
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, p) == cudaSuccess ? MG_OK : MG_ERR_CUDA;
+  if (cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, p) != cudaSuccess) return MG_ERR_CUDA;
+  return p.weights != nullptr ? launch_prompt_weights<T, D>(p, stream) : MG_OK;
 }
 
 }  // namespace
