@@ -302,10 +302,11 @@ int matgptq_b200_append_kv4(const matgptq_b200_kv4_cache *cache, const void *qkv
  * entry p = lengths[b] - seq + i itself and sees entry j when j <= p and (window == 0, or j > p - window, or j < sinks).  Window
  * and sinks count entries.  A query that sees nothing gives zeros.  Head h reads key/value head h / (n_heads / n_kv_heads).
  * With weights[batch, n_kv_heads, capacity] (fp32, may be NULL) each entry's softmax weights, summed over the queries and heads that
- * share it, are added to what is there, in a fixed order; this needs matgptq_b200_attention_kv4_workspace_bytes(...) bytes of
- * workspace (16-byte aligned; its contents do not matter; one per call in flight).  K and V are not rounded; sums are fp32.
+ * share it, are added to what is there, in a fixed order.  The call needs matgptq_b200_attention_kv4_workspace_bytes(...) bytes of
+ * workspace (16-byte aligned, NULL where that is 0; its contents do not matter; one per call in flight).  K and V are not rounded; sums are fp32.
  */
-int64_t matgptq_b200_attention_kv4_workspace_bytes(const matgptq_b200_kv4_cache *cache, int64_t seq, int64_t n_heads, int with_weights);
+int64_t matgptq_b200_attention_kv4_workspace_bytes(const matgptq_b200_kv4_cache *cache, int64_t seq, int64_t n_heads, int64_t window,
+                                                   int64_t sinks, int with_weights);
 int matgptq_b200_attention_kv4(const matgptq_b200_kv4_cache *cache, const void *q, int64_t seq, int64_t n_heads, const int32_t *lengths,
                                int64_t window, int64_t sinks, float scale, float *weights, void *out, void *workspace,
                                int64_t workspace_bytes, uint32_t flags, void *stream);

@@ -60,7 +60,7 @@ SIGNATURES = {
     "matgptq_b200_argmax": (_c_int, [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_u32, _c_ptr]),
     "matgptq_b200_silu_mul": (_c_int, [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_u32, _c_ptr]),
     "matgptq_b200_append_kv4": (_c_int, [ctypes.POINTER(Kv4Cache), _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_u32, _c_ptr]),
-    "matgptq_b200_attention_kv4_workspace_bytes": (_c_i64, [ctypes.POINTER(Kv4Cache), _c_i64, _c_i64, _c_int]),
+    "matgptq_b200_attention_kv4_workspace_bytes": (_c_i64, [ctypes.POINTER(Kv4Cache), _c_i64, _c_i64, _c_i64, _c_i64, _c_int]),
     "matgptq_b200_attention_kv4": (_c_int, [ctypes.POINTER(Kv4Cache), _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, ctypes.c_float, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_u32, _c_ptr]),
     "matgptq_b200_evict_kv4": (_c_int, [ctypes.POINTER(Kv4Cache), _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_u32, _c_ptr]),
     "matgptq_b200_dequantize_kv4": (_c_int, [ctypes.POINTER(Kv4Cache), _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_u32, _c_ptr]),

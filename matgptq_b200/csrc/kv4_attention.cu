@@ -12,6 +12,8 @@
 // What is rounded is p v_scale, to fp16 (2^-11), as the operand of the second product, in units of a power of two near the largest
 // v_scale.  The codes of V are centred first: their mean would multiply that rounding, and the tensor cores would sum up numbers of
 // one sign, which over 131072 entries cost three bits of the result.  Row maximum and sums are fp32.
+//
+// This file: up to kKv4FewRows rows, as in decoding.  The entries are read once and that is what bounds it.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -34,8 +36,8 @@ MG_DEFINE_STATUS_ACCESSOR(kv4_attention_device_status)
 // in the order in which the masks take them out of a word; and the constants of the rows that its results are for, 2t and 2t + 1.
 template <int D> struct Kv4Rows {
   uint32_t q[D / 32][4];
-  float unit[2];  // score per k_scale * (q . c 2^-24)
-  float sum[2];   // score per k_min
+  float unit[2];  // log2 of a weight per score; scores are k_scale (q . c 2^-24) + k_min sum
+  float sum[2];
   int pos[2];     // position; before every entry where there is no such row
 };
 
@@ -64,9 +66,10 @@ __device__ __forceinline__ void kv4_load_rows(Kv4Rows<D> &rows, const Kv4Attenti
   }
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  // 2^-e with 2^e <= top < 2^(e+1), exact; a row of zeros stays as it is, one with an infinity keeps it
-  const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 1), 253);
-  const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23), up = __uint_as_float(static_cast<uint32_t>(e) << 23);
+  // a power of two that takes the largest value to [2^8, 2^9); a row of zeros stays as it is, one with an infinity keeps it
+  const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 16), 253);
+  const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * (p.scale_log2 < 0.f ? -256.f : 256.f);
+  const float up = __uint_as_float(static_cast<uint32_t>(e) << 23) * 65536.f;  // 2^24 / 2^8
   float sum = 0.f;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
@@ -75,7 +78,8 @@ __device__ __forceinline__ void kv4_load_rows(Kv4Rows<D> &rows, const Kv4Attenti
     for (int c = 0; c < 8; ++c) {
       const __half x = __float2half_rn(v[w][c] * down);
       sum += __half2float(x);
-      h2[c] = __half_as_ushort(x);
+      // the codes of odd channels are taken out 4 bits up
+      h2[c] = __half_as_ushort(c & 1 ? __float2half_rn(__half2float(x) * 0.0625f) : x);
     }
     rows.q[w][0] = h2[0] | h2[4] << 16;
     rows.q[w][1] = h2[2] | h2[6] << 16;
@@ -84,24 +88,19 @@ __device__ __forceinline__ void kv4_load_rows(Kv4Rows<D> &rows, const Kv4Attenti
   }
   sum += __shfl_xor_sync(0xffffffffu, sum, 1);
   sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-  const float per = up * p.scale_log2;
+  const float per = fmaxf(up * fabsf(p.scale_log2), FLT_MIN);  // never 0: what is hidden has a score of -infinity
+  sum *= 0x1p-24f;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const float f = __shfl_sync(0xffffffffu, per, (2 * t + k) * 4);
-    rows.unit[k] = f * 16777216.f;
-    rows.sum[k] = f * __shfl_sync(0xffffffffu, sum, (2 * t + k) * 4);
+    rows.unit[k] = __shfl_sync(0xffffffffu, per, (2 * t + k) * 4);
+    rows.sum[k] = __shfl_sync(0xffffffffu, sum, (2 * t + k) * 4);
     const int row = r0 + 2 * t + k;
     rows.pos[k] = row < total ? length - p.seq + row / p.group : -1;
   }
 }
 
-// What a lane (g, t) loads of a block of 16 entries: K words of entries g and g + 8, V words of the pairs t and t + 4, the params
-// of entries g and g + 8.
-template <int D> struct Kv4Block {
-  uint32_t k[2][D / 32], v[2][D / 32];
-  uint2 param[2];
-};
-
+// What a lane (g, t) takes of 16 entries: K words of entries g and g + 8, V words of the pairs t and t + 4, the params of entries
+// g and g + 8.
 template <int W> __device__ __forceinline__ void kv4_load_words(uint32_t (&dst)[W], const uint8_t *src) {
   if constexpr (W == 4) {
     const uint4 x = *reinterpret_cast<const uint4 *>(src);
@@ -112,25 +111,14 @@ template <int W> __device__ __forceinline__ void kv4_load_words(uint32_t (&dst)[
   }
 }
 
-template <int D, bool WITH_V = true>
-__device__ __forceinline__ void kv4_load_block(Kv4Block<D> &blk, const Kv4Cache &c, size_t first, int block) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const size_t e = first + static_cast<size_t>(block) * 16;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    kv4_load_words(blk.k[i], c.k + (e + g + 8 * i) * (D / 2) + t * (D / 8));
-    blk.param[i] = *reinterpret_cast<const uint2 *>(c.params + (e + g + 8 * i) * 4);
-    if constexpr (WITH_V) kv4_load_words(blk.v[i], c.v + ((e >> 1) + t + 4 * i) * D + g * (D / 8));
-  }
-}
-
-// Scores of 16 entries x 8 rows in units of log 2: s[0], s[1] entry g, rows 2t and 2t + 1; s[2], s[3] entry g + 8.
+// Scores of 16 entries x 8 rows in the rows' units: s[0], s[1] entry g, rows 2t and 2t + 1; s[2], s[3] entry g + 8.
 template <typename T, int D>
-__device__ __forceinline__ void kv4_scores(float (&s)[4], const Kv4Block<D> &blk, const Kv4Rows<D> &rows) {
-  float lo[4] = {0.f, 0.f, 0.f, 0.f}, hi[4] = {0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ void kv4_scores(float (&s)[4], const uint32_t (&k0)[D / 32], const uint32_t (&k1)[D / 32], const uint32_t (&kp)[2],
+                                           const Kv4Rows<D> &rows) {
+  float lo[4] = {0.f, 0.f, 0.f, 0.f}, hi[4] = {0.f, 0.f, 0.f, 0.f};  // two chains
 #pragma unroll
   for (int w = 0; w < D / 32; ++w) {
-    const uint32_t x = blk.k[0][w], y = blk.k[1][w], xs = x >> 8, ys = y >> 8;
+    const uint32_t x = k0[w], y = k1[w], xs = x >> 8, ys = y >> 8;
     const uint32_t a[4] = {x & 0x000F000Fu, y & 0x000F000Fu, xs & 0x000F000Fu, ys & 0x000F000Fu};
     const uint32_t c[4] = {x & 0x00F000F0u, y & 0x00F000F0u, xs & 0x00F000F0u, ys & 0x00F000F0u};
     mma16816<false>(lo, a, rows.q[w][0], rows.q[w][1]);
@@ -138,13 +126,14 @@ __device__ __forceinline__ void kv4_scores(float (&s)[4], const Kv4Block<D> &blk
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const float ks = kv4_to_f<T>(static_cast<uint16_t>(blk.param[i].x)), kl = kv4_to_f<T>(static_cast<uint16_t>(blk.param[i].x >> 16));
+    const float ks = kv4_to_f<T>(static_cast<uint16_t>(kp[i])), kl = kv4_to_f<T>(static_cast<uint16_t>(kp[i] >> 16));
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float dot = fmaf(hi[2 * i + k], 0.0625f, lo[2 * i + k]) * rows.unit[k];
-      s[2 * i + k] = fmaf(ks, dot, kl * rows.sum[k]);
-    }
+    for (int k = 0; k < 2; ++k) s[2 * i + k] = fmaf(ks, lo[2 * i + k] + hi[2 * i + k], kl * rows.sum[k]);
   }
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
@@ -153,128 +142,174 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   return r;
 }
 
-constexpr int kKv4Warps = 8;
+// ---- the work and who does it ---------------------------------------------------------------------------------------
+//
+// A segment is a tile of R = 8 or 16 rows of one key/value head of one sequence, its work the blocks of 32 entries that these rows
+// see.  Segments of few blocks get a CTA each.  Otherwise the blocks of all segments, one behind the other (sequence, tile, head), are
+// cut into equal shares, one for each CTA of a grid that fills the GPU, whatever the lengths: a share may begin and end inside a
+// segment, and the CTAs of a segment leave partial results, which kv4_finish_kernel joins in their order.  Lengths are known on the
+// device only, so every CTA works the cuts out by itself.
+constexpr int kStepWarps = 8;
+constexpr int kStepBlock = 32;       // entries of a block
+constexpr int kStepStages = 3;       // blocks in flight per warp
+constexpr int kStepCtas = 296;       // two on each SM of a B200
+constexpr int kStepLeast = kStepWarps;  // blocks of a share at least: one for each warp
+constexpr int kStepSequences = 1024;    // whose blocks are cut into shares, at most
+// Blocks of a segment up to which it is not cut.
+constexpr int kStepWhole = 64;
 
-// Up to 8 NT rows of one key/value head and sequence per cluster; its warps share out the blocks of 16 entries, one range each.
-// Every warp keeps its own running maximum; they are joined in shared memory, then over the cluster's CTAs through distributed
-// shared memory, in a fixed order.  blockIdx.x: the CTA of the cluster, y: tile of rows, z: sequence and head.
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kKv4Warps * 32) kv4_attention_kernel(const Kv4AttentionParams p) {
-  pdl_prologue();
-  constexpr int R = 8 * NT, W = D / 32;
-  extern __shared__ float smem[];
-  float *part = smem;                                  // [warps][R][D]
-  float *part_m = smem + kKv4Warps * R * D;            // [warps][R]
-  float *part_l = part_m + kKv4Warps * R;              // [warps][R]
-  float *cta_m = part_l + kKv4Warps * R;               // [R]
-  float *cta_l = cta_m + R;                            // [R]
+struct Kv4StepParams {
+  Kv4AttentionParams a;
+  float *ml;       // [slots][2][R]: maximum and sum of the partial result in a slot
+  float *partial;  // [slots][R][D]
+  int tiles;       // of rows
+  int whole;       // a CTA per segment
+};
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int cta = blockIdx.x, ctas = gridDim.x;
-  const int b = blockIdx.z / p.cache.kv_heads, h = blockIdx.z - b * p.cache.kv_heads;
-  const int total = p.seq * p.group, r0 = blockIdx.y * R;
-  const int length = kv4_length(p.lengths, b, p.cache.capacity);
-  const size_t first = static_cast<size_t>(blockIdx.z) * p.cache.capacity;
-  const int pos_lo = length - p.seq + r0 / p.group, pos_hi = length - p.seq + (min(r0 + R, total) - 1) / p.group;
-  const Kv4Range range = kv4_range<16>(pos_lo, pos_hi, p.window, p.sinks, p.cache.capacity);
-  const int units = ctas * kKv4Warps, unit = cta * kKv4Warps + warp;
-  const int from = static_cast<int>(static_cast<long long>(range.blocks) * unit / units);
-  const int to = static_cast<int>(static_cast<long long>(range.blocks) * (unit + 1) / units);
+template <int D> struct StepStage {
+  static constexpr int k = 0, v = kStepBlock * D / 2, params = 2 * v, bytes = params + kStepBlock * 8;
+};
 
-  Kv4Rows<D> rows[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) kv4_load_rows<T, D>(rows[n], p, b, h, r0 + 8 * n, total, length);
+template <int R> __device__ __forceinline__ Kv4Range step_range(const Kv4AttentionParams &p, int length, int tile) {
+  const int total = p.seq * p.group, r0 = tile * R;
+  return kv4_range<kStepBlock>(length - p.seq + r0 / p.group, length - p.seq + (min(r0 + R, total) - 1) / p.group, p.window, p.sinks, p.cache.capacity);
+}
 
-  float o[NT][2 * W][4], m[NT][2], l[NT][2], fix[NT][2];
+// before[b]: blocks of one head (all its tiles) of the sequences before b; before[batch]: of all.  All threads of the CTA.
+template <int R> __device__ __forceinline__ void step_prefix(const Kv4StepParams &p, int *before) {
+  __shared__ int warp_sum[kStepWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int carry = 0;
+  for (int b0 = 0; b0 < p.a.cache.batch; b0 += kStepWarps * 32) {
+    const int b = b0 + threadIdx.x;
+    int n = 0;
+    if (b < p.a.cache.batch) {
+      const int length = kv4_length(p.a.lengths, b, p.a.cache.capacity);
+      for (int tile = 0; tile < p.tiles; ++tile) n += step_range<R>(p.a, length, tile).blocks;
+    }
+    int sum = n;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int i = 0; i < 2 * W; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) m[n][k] = -INFINITY, l[n][k] = 0.f, fix[n][k] = 0.f;
+    for (int off = 1; off < 32; off <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, sum, off);
+      if (lane >= off) sum += x;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sum[warp] = sum;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < kStepWarps; ++w) {
+      if (w < warp) sum += warp_sum[w];
+      all += warp_sum[w];
+    }
+    if (b < p.a.cache.batch) before[b] = carry + sum - n;
+    carry += all;
   }
-  float v_unit = 0x1p-100f, v_per = 0x1p100f;  // p v_scale is rounded in these units, a power of two; the warp's largest v_scale sets it
+  if (threadIdx.x == 0) before[p.a.cache.batch] = carry;
+  __syncthreads();
+}
 
-  Kv4Block<D> cur, nxt;
-  if (from < to) kv4_load_block<D>(cur, p.cache, first, range.block(from));
-  for (int i = from; i < to; ++i) {
-    if (i + 1 < to) kv4_load_block<D>(nxt, p.cache, first, range.block(i + 1));
-    const int j0 = range.block(i) * 16;
-    const bool whole = j0 + 15 <= pos_lo && r0 + R <= total && (p.window == 0 || j0 > pos_hi - p.window || j0 + 16 <= p.sinks);
-    float s[NT][4];
-    float vs[2], vl[2];
+__device__ __forceinline__ int step_share(int blocks, int ctas) { return max((blocks + ctas - 1) / ctas, kStepLeast); }
+
+// What a warp has of its rows' sums so far
+template <int D, int NT> struct StepSums {
+  float o[NT][D / 16][4];    // sums of p v_scale (c - 8), in units of v_unit: channels along the lanes' g, rows along t
+  float m[NT][2], limit[NT][2], shift[NT][2];  // maximum in log2; the score above which it is raised; -m, 0 where nothing was seen
+  float l[NT][2], fix[NT][2];  // this lane's entries' part of the sums of p and of p (v_min + 8 v_scale)
+  float v_unit, v_per;         // p v_scale is rounded in these units, a power of two; the warp's largest v_scale sets it
+};
+
+// 32 entries from j0, in a stage of shared memory.  WHOLE: all rows see all of them.
+template <typename T, int D, int NT, bool WHOLE>
+__device__ __forceinline__ void step_block(StepSums<D, NT> &a, const Kv4Rows<D> (&rows)[NT], const uint8_t *blk, int j0, int pos_hi, int window, int sinks,
+                                           const Centring &centre) {
+  constexpr int W = D / 32;
+  using Stage = StepStage<D>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float s[2][NT][4], vs[2][2], vl[2][2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {  // 16 entries
+    uint32_t k0[W], k1[W], kp[2];
+    kv4_load_words(k0, blk + Stage::k + (16 * u + g) * (D / 2) + t * (D / 8));
+    kv4_load_words(k1, blk + Stage::k + (16 * u + 8 + g) * (D / 2) + t * (D / 8));
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      vs[e] = kv4_to_f<T>(static_cast<uint16_t>(cur.param[e].y));
-      vl[e] = kv4_to_f<T>(static_cast<uint16_t>(cur.param[e].y >> 16));
+      const uint2 x = *reinterpret_cast<const uint2 *>(blk + Stage::params + (16 * u + 8 * e + g) * 8);
+      kp[e] = x.x;
+      vs[u][e] = kv4_to_f<T>(static_cast<uint16_t>(x.y));
+      vl[u][e] = kv4_to_f<T>(static_cast<uint16_t>(x.y >> 16));
+      // entries that no row of the tile sees may hold anything
+      if (!WHOLE && j0 + 16 * u + 8 * e + g > pos_hi) vs[u][e] = vl[u][e] = 0.f;
     }
-    bool grow = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      kv4_scores<T, D>(s[n], cur, rows[n]);
-      if (!whole) {
+      kv4_scores<T, D>(s[u][n], k0, k1, kp, rows[n]);
+      if (!WHOLE) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (!kv4_sees(rows[n].pos[e & 1], j0 + g + 8 * (e >> 1), p.window, p.sinks)) s[n][e] = -INFINITY;
+          if (!kv4_sees(rows[n].pos[e & 1], j0 + 16 * u + g + 8 * (e >> 1), window, sinks)) s[u][n][e] = -INFINITY;
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) grow |= !(s[n][e] <= m[n][e & 1] + 4.f);
     }
-    // entries that no row of the warp's tile sees may hold anything
-    if (!whole) {
+  }
+  float top_v = fmaxf(fmaxf(fabsf(vs[0][0]), fabsf(vs[0][1])), fmaxf(fabsf(vs[1][0]), fabsf(vs[1][1])));
+  bool grow = top_v > 16.f * a.v_unit;
+  float top[NT][2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (j0 + g + 8 * e > pos_hi) vs[e] = vl[e] = 0.f;
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      top[n][k] = fmaxf(fmaxf(s[0][n][k], s[0][n][2 + k]), fmaxf(s[1][n][k], s[1][n][2 + k]));
+      grow |= top[n][k] > a.limit[n][k];
     }
-    grow |= fmaxf(fabsf(vs[0]), fabsf(vs[1])) > 16.f * v_unit;
-    // Maximum and unit may lag by a factor of 16: both cancel in the end, and fp16 has the room.
-    if (__any_sync(0xffffffffu, grow)) {
-      float top = fmaxf(fabsf(vs[0]), fabsf(vs[1]));
+  // Maximum and unit may lag by a factor of 16: both cancel in the end, and fp16 has the room.  (A NaN raises nothing: it makes the
+  // row's sum a NaN, which says all.)
+  if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-      for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-      float rescale = 1.f;
-      if (top > v_unit && top <= FLT_MAX) {
-        const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 27), 250);
-        const float unit_new = __uint_as_float(static_cast<uint32_t>(e) << 23);
-        rescale = v_unit * __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-        v_unit = unit_new;
-        v_per = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-      }
+    for (int off = 16; off >= 1; off >>= 1) top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, off));
+    float rescale = 1.f;
+    if (top_v > a.v_unit && top_v <= FLT_MAX) {
+      const int e = min(max(static_cast<int>(__float_as_uint(top_v) >> 23), 27), 250);
+      const float unit_new = __uint_as_float(static_cast<uint32_t>(e) << 23);
+      a.v_per = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+      rescale = a.v_unit * a.v_per;
+      a.v_unit = unit_new;
+    }
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          // a NaN counts as an infinity here: the row's results are NaN then
-          float x = s[n][k] == s[n][k] && s[n][2 + k] == s[n][2 + k] ? fmaxf(s[n][k], s[n][2 + k]) : INFINITY;
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          const float m_new = fmaxf(m[n][k], x);
-          const float f = m[n][k] == -INFINITY ? 0.f : exp2_approx(m[n][k] - m_new);
-          m[n][k] = m_new;
-          l[n][k] *= f;
-          fix[n][k] *= f;
+      for (int k = 0; k < 2; ++k) {
+        float x = top[n][k];
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)) * rows[n].unit[k];
+        const float m_new = fmaxf(a.m[n][k], x);
+        const float f = a.m[n][k] == -INFINITY ? 0.f : exp2_approx(a.m[n][k] - m_new);
+        a.m[n][k] = m_new;
+        a.shift[n][k] = m_new == -INFINITY ? 0.f : -m_new;
+        a.limit[n][k] = m_new == -INFINITY ? -INFINITY : (m_new + 4.f) / rows[n].unit[k];
+        a.l[n][k] *= f;
+        a.fix[n][k] *= f;
 #pragma unroll
-          for (int w = 0; w < 2 * W; ++w) {
-            o[n][w][k] *= f * rescale;
-            o[n][w][2 + k] *= f * rescale;
-          }
+        for (int w = 0; w < 2 * W; ++w) {
+          a.o[n][w][k] *= f * rescale;
+          a.o[n][w][2 + k] *= f * rescale;
         }
-    }
-    const float mid[2] = {fmaf(8.f, vs[0], vl[0]), fmaf(8.f, vs[1], vl[1])}, per[2] = {vs[0] * v_per, vs[1] * v_per};
+      }
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const float mid[2] = {fmaf(8.f, vs[u][0], vl[u][0]), fmaf(8.f, vs[u][1], vl[u][1])}, per[2] = {vs[u][0] * a.v_per, vs[u][1] * a.v_per};
     uint32_t pv[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
+        const int k = e & 1;
+        const float pe = exp2_approx(fmaf(s[u][n][e], rows[n].unit[k], a.shift[n][k]));
+        a.l[n][k] += pe;
         // hidden entries may hold a NaN: nothing of theirs is multiplied
-        const bool hidden = s[n][e] == -INFINITY;
-        const float pe = hidden ? 0.f : exp2_approx(s[n][e] - m[n][e & 1]);
-        l[n][e & 1] += pe;
-        fix[n][e & 1] = fmaf(pe, hidden ? 0.f : mid[e >> 1], fix[n][e & 1]);
+        const bool hidden = !WHOLE && s[u][n][e] == -INFINITY;
+        a.fix[n][k] = fmaf(pe, hidden ? 0.f : mid[e >> 1], a.fix[n][k]);
         x[e] = hidden ? 0.f : pe * per[e >> 1];
       }
 #pragma unroll
@@ -283,125 +318,311 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attention_kernel(const Kv4
         pv[n][e] = transpose_8x8(*reinterpret_cast<const uint32_t *>(&r));
       }
     }
+    uint32_t v0[W], v1[W];
+    kv4_load_words(v0, blk + Stage::v + (8 * u + t) * D + g * (D / 8));
+    kv4_load_words(v1, blk + Stage::v + (8 * u + 4 + t) * D + g * (D / 8));
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const uint32_t x = cur.v[0][w], y = cur.v[1][w], xs = x >> 8, ys = y >> 8;
-      const uint32_t a[4] = {centred_low(x), centred_high(x), centred_low(y), centred_high(y)};
-      const uint32_t c[4] = {centred_low(xs), centred_high(xs), centred_low(ys), centred_high(ys)};
+      const uint32_t x = v0[w], y = v1[w], xs = x >> 8, ys = y >> 8;
+      const uint32_t c0[4] = {centre.lower(x), centre.upper(x), centre.lower(y), centre.upper(y)};
+      const uint32_t c1[4] = {centre.lower(xs), centre.upper(xs), centre.lower(ys), centre.upper(ys)};
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        mma16816<false>(o[n][2 * w], a, pv[n][0], pv[n][1]);
-        mma16816<false>(o[n][2 * w + 1], c, pv[n][0], pv[n][1]);
+        mma16816<false>(a.o[n][2 * w], c0, pv[n][0], pv[n][1]);
+        mma16816<false>(a.o[n][2 * w + 1], c1, pv[n][0], pv[n][1]);
       }
     }
-    cur = nxt;
   }
-
-  // the warp's sums: lanes of equal t hold parts of the same rows' l and fix
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-#pragma unroll
-      for (int off = 4; off <= 16; off <<= 1) {
-        l[n][k] += __shfl_xor_sync(0xffffffffu, l[n][k], off);
-        fix[n][k] += __shfl_xor_sync(0xffffffffu, fix[n][k], off);
-      }
-      const int row = 8 * n + 2 * t + k;
-      if (g == 0) {
-        part_m[warp * R + row] = m[n][k];
-        part_l[warp * R + row] = l[n][k];
-      }
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        float4 x;  // channels D/8 g + 4 w + 0 .. 3
-        x.x = fmaf(o[n][2 * w][k], v_unit, fix[n][k]);
-        x.y = fmaf(o[n][2 * w][2 + k], v_unit, fix[n][k]);
-        x.z = fmaf(o[n][2 * w + 1][k], v_unit, fix[n][k]);
-        x.w = fmaf(o[n][2 * w + 1][2 + k], v_unit, fix[n][k]);
-        *reinterpret_cast<float4 *>(part + (warp * R + row) * D + (D / 8) * g + 4 * w) = x;
-      }
-    }
-  __syncthreads();
-  for (int r = threadIdx.x; r < R; r += kKv4Warps * 32) {
-    float top = -INFINITY, sum = 0.f;
-    for (int w = 0; w < kKv4Warps; ++w) top = fmaxf(top, part_m[w * R + r]);
-    for (int w = 0; w < kKv4Warps; ++w) {
-      const float f = part_m[w * R + r] == -INFINITY ? 0.f : exp2_approx(part_m[w * R + r] - top);
-      sum = fmaf(part_l[w * R + r], f, sum);
-      part_m[w * R + r] = f;
-    }
-    cta_m[r] = top;
-    cta_l[r] = sum;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < R * D; i += kKv4Warps * 32) {
-    const int r = i / D;
-    float sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kKv4Warps; ++w) {
-      const float f = part_m[w * R + r];
-      if (f != 0.f) sum = fmaf(part[w * R * D + i], f, sum);
-    }
-    part[i] = sum;
-  }
-  cluster_sync_all();
-  const uint32_t part_u32 = smem_u32(part), m_u32 = smem_u32(cta_m), l_u32 = smem_u32(cta_l);
-  auto remote = [](uint32_t addr, int c) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(addr, c)) : "memory");
-    return v;
-  };
-  for (int i = cta * kKv4Warps * 32 + threadIdx.x; i < R * D; i += ctas * kKv4Warps * 32) {
-    const int r = i / D, row = r0 + r;
-    float top = -INFINITY;
-    for (int c = 0; c < ctas; ++c) top = fmaxf(top, remote(m_u32 + 4 * r, c));
-    float sum = 0.f, norm = 0.f;
-    for (int c = 0; c < ctas; ++c) {
-      const float mc = remote(m_u32 + 4 * r, c);
-      if (mc == -INFINITY) continue;
-      const float f = exp2_approx(mc - top);
-      norm = fmaf(remote(l_u32 + 4 * r, c), f, norm);
-      sum = fmaf(remote(part_u32 + 4 * i, c), f, sum);
-    }
-    if (row < total) {
-      const int q = row / p.group;
-      const size_t at = ((static_cast<size_t>(b) * p.seq + q) * p.heads + static_cast<size_t>(h) * p.group + (row - q * p.group)) * D + (i - r * D);
-      p.out[at] = kv4_bits<T>(top == -INFINITY ? 0.f : sum / norm);  // a row that sees nothing: zeros
-      if (p.lse != nullptr && i % D == 0) p.lse[static_cast<size_t>(blockIdx.z) * total + row] = top == -INFINITY ? INFINITY : top + log2f(norm);
-    }
-  }
-  cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
 
-// weights[j] += sum over all rows of exp2(score - lse): a warp per block of 16 entries goes over the rows that see it, so that the
-// sum has one order and needs no atomics.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) kv4_weights_kernel(const Kv4AttentionParams p) {
+// One warp per 32 entries at a time: the warps of a CTA share out its part of a segment, each keeps a running maximum of its own.  A
+// warp's next blocks are on their way into its ring of stages while it works on one; a block is 32 x (D + 8) bytes in three places.
+// (With a bulk copy for each of the three a SM took in no more than 11 bytes a cycle, one copy in 130 cycles; cp.async has no such limit.)
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kStepWarps * 32, NT == 1 ? 2 : 1) kv4_step_kernel(const Kv4StepParams sp) {
   pdl_prologue();
+  const Kv4AttentionParams &p = sp.a;
+  constexpr int R = 8 * NT, W = D / 32;
+  using Stage = StepStage<D>;
+  extern __shared__ __align__(128) unsigned char step_smem[];
+  __shared__ int before[kStepSequences + 1];
+  __shared__ float part_m[kStepWarps][R], part_l[kStepWarps][R];
+  float *part = reinterpret_cast<float *>(step_smem);  // [warps][R][D], over the stages once these are done with
+
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int b = blockIdx.y / p.cache.kv_heads, h = blockIdx.y - b * p.cache.kv_heads;
-  const int total = p.seq * p.group, length = kv4_length(p.lengths, b, p.cache.capacity);
-  const size_t first = static_cast<size_t>(blockIdx.y) * p.cache.capacity;
-  const int block = blockIdx.x * 8 + warp, j0 = block * 16;
+  unsigned char *ring = step_smem + warp * kStepStages * Stage::bytes;
+  const uint32_t ring_u32 = smem_u32(ring);
+  const Centring centre;
+  const int kv = p.cache.kv_heads, total = p.seq * p.group;
+  int pos = 0, end = 1, share = 0;
+  if (!sp.whole) {
+    step_prefix<R>(sp, before);
+    const int all = before[p.cache.batch] * kv;
+    share = step_share(all, gridDim.x);
+    pos = min(static_cast<int>(blockIdx.x) * share, all);
+    end = min(pos + share, all);
+  }
+  while (pos < end) {
+    // ---- the piece of a segment that starts at pos
+    int b, tile = 0, h, offset = 0;
+    if (sp.whole) {
+      b = blockIdx.x / (sp.tiles * kv);
+      tile = (blockIdx.x - b * sp.tiles * kv) / kv;
+      h = blockIdx.x - (b * sp.tiles + tile) * kv;
+    } else {
+      int lo = 0, hi = p.cache.batch - 1;  // the last sequence that begins at pos or before, and has blocks
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (before[mid] * kv <= pos) lo = mid; else hi = mid - 1;
+      }
+      b = lo;
+      offset = pos - before[b] * kv;
+    }
+    const int length = kv4_length(p.lengths, b, p.cache.capacity);
+    Kv4Range range = step_range<R>(p, length, tile);
+    if (!sp.whole) {
+      while (offset >= range.blocks * kv) {
+        offset -= range.blocks * kv;
+        range = step_range<R>(p, length, ++tile);
+      }
+      h = offset / range.blocks;
+      offset -= h * range.blocks;
+    }
+    const int count = sp.whole ? range.blocks : min(range.blocks - offset, end - pos);
+    const bool complete = count == range.blocks;
+    const int segment = (b * sp.tiles + tile) * kv + h, slot = sp.whole ? segment : segment + blockIdx.x;
+    const int r0 = tile * R;
+    const int pos_lo = length - p.seq + r0 / p.group, pos_hi = length - p.seq + (min(r0 + R, total) - 1) / p.group;
+    const size_t first = (static_cast<size_t>(b) * kv + h) * p.cache.capacity;
+    const int from = offset + count * warp / kStepWarps, to = offset + count * (warp + 1) / kStepWarps;
+
+    // a block into a stage, 16 bytes a lane at a time; every call is a group of its own, with nothing in it behind the last block
+    const auto request = [&](int i, uint32_t stage) {
+      if (i < to) {
+        const size_t e = first + static_cast<size_t>(range.block(i)) * kStepBlock;
+        const uint32_t dst = ring_u32 + stage * Stage::bytes + lane * 16;
+        const uint8_t *k = p.cache.k + e * (D / 2) + lane * 16, *v = p.cache.v + e * (D / 2) + lane * 16;
+#pragma unroll
+        for (int c = 0; c < kStepBlock * D / 2; c += 512) {
+          cp_async16(dst + Stage::k + c, k + c);
+          cp_async16(dst + Stage::v + c, v + c);
+        }
+        if (lane < kStepBlock / 2) cp_async16(dst + Stage::params, reinterpret_cast<const uint8_t *>(p.cache.params) + e * 8 + lane * 16);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < kStepStages; ++i) request(from + i, i);
+
+    Kv4Rows<D> rows[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) kv4_load_rows<T, D>(rows[n], p, b, h, r0 + 8 * n, total, length);
+
+    StepSums<D, NT> a;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < 2 * W; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a.o[n][i][e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) a.m[n][k] = a.limit[n][k] = -INFINITY, a.shift[n][k] = a.l[n][k] = a.fix[n][k] = 0.f;
+    }
+    a.v_unit = 0x1p-100f, a.v_per = 0x1p100f;
+
+    uint32_t taken = 0;  // the stage that comes next
+    for (int i = from; i < to; ++i) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStepStages - 1) : "memory");
+      __syncwarp();  // the other lanes' bytes as well
+      const uint8_t *blk = ring + taken * Stage::bytes;
+      const int j0 = range.block(i) * kStepBlock;
+      if (j0 + kStepBlock - 1 <= pos_lo && r0 + R <= total && (p.window == 0 || j0 > pos_hi - p.window || j0 + kStepBlock <= p.sinks))
+        step_block<T, D, NT, true>(a, rows, blk, j0, pos_hi, p.window, p.sinks, centre);
+      else
+        step_block<T, D, NT, false>(a, rows, blk, j0, pos_hi, p.window, p.sinks, centre);
+      __syncwarp();  // every lane has read the stage
+      request(i + kStepStages, taken);
+      taken = taken == kStepStages - 1 ? 0 : taken + 1;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+    // ---- the warps' sums; lanes of equal t hold parts of the same rows' l and fix
+    __syncthreads();  // the stages are done with
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int off = 4; off <= 16; off <<= 1) {
+          a.l[n][k] += __shfl_xor_sync(0xffffffffu, a.l[n][k], off);
+          a.fix[n][k] += __shfl_xor_sync(0xffffffffu, a.fix[n][k], off);
+        }
+        const int row = 8 * n + 2 * t + k;
+        if (g == 0) {
+          part_m[warp][row] = a.m[n][k];
+          part_l[warp][row] = a.l[n][k];
+        }
+        if (from < to) {
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            float4 x;  // channels D/8 g + 4 w + 0 .. 3
+            x.x = fmaf(a.o[n][2 * w][k], a.v_unit, a.fix[n][k]);
+            x.y = fmaf(a.o[n][2 * w][2 + k], a.v_unit, a.fix[n][k]);
+            x.z = fmaf(a.o[n][2 * w + 1][k], a.v_unit, a.fix[n][k]);
+            x.w = fmaf(a.o[n][2 * w + 1][2 + k], a.v_unit, a.fix[n][k]);
+            *reinterpret_cast<float4 *>(part + (warp * R + row) * D + (D / 8) * g + 4 * w) = x;
+          }
+        }
+      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < R * D / 4; i += kStepWarps * 32) {
+      const int r = i / (D / 4), row = r0 + r;
+      float top = -INFINITY, norm = 0.f;
+#pragma unroll
+      for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, part_m[w][r]);
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kStepWarps; ++w) {
+        if (part_l[w][r] == 0.f) continue;  // nothing seen
+        const float f = exp2_approx(part_m[w][r] - top);
+        norm = fmaf(part_l[w][r], f, norm);
+        const float4 x = *reinterpret_cast<const float4 *>(part + (w * R) * D + 4 * i);
+        sum.x = fmaf(x.x, f, sum.x);
+        sum.y = fmaf(x.y, f, sum.y);
+        sum.z = fmaf(x.z, f, sum.z);
+        sum.w = fmaf(x.w, f, sum.w);
+      }
+      if ((!complete || p.weights != nullptr) && i % (D / 4) == 0) {
+        sp.ml[(static_cast<size_t>(slot) * 2) * R + r] = top;
+        sp.ml[(static_cast<size_t>(slot) * 2 + 1) * R + r] = norm;
+      }
+      if (!complete) {
+        *reinterpret_cast<float4 *>(sp.partial + static_cast<size_t>(slot) * R * D + 4 * i) = sum;
+      } else if (row < total) {
+        const float inv = norm == 0.f ? 0.f : 1.f / norm;  // a row that sees nothing: zeros
+        const int q = row / p.group;
+        const size_t at = ((static_cast<size_t>(b) * p.seq + q) * p.heads + static_cast<size_t>(h) * p.group + (row - q * p.group)) * D + (i % (D / 4)) * 4;
+        uint2 w;
+        w.x = kv4_bits<T>(sum.x * inv) | static_cast<uint32_t>(kv4_bits<T>(sum.y * inv)) << 16;
+        w.y = kv4_bits<T>(sum.z * inv) | static_cast<uint32_t>(kv4_bits<T>(sum.w * inv)) << 16;
+        *reinterpret_cast<uint2 *>(p.out + at) = w;
+      }
+    }
+    pos += sp.whole ? 1 : count;
+    if (pos < end) __syncthreads();  // before copies land where sums were
+  }
+}
+
+// What is left once every segment's blocks have been seen: joins the partial results of segments that were cut, and adds up the weights.
+// blockIdx.y: sequence and head; blockIdx.x: a part of a tile's results (256 numbers), and 128 entries whose weights are due.
+template <typename T, int D, int NT> __global__ void __launch_bounds__(kStepWarps * 32) kv4_finish_kernel(const Kv4StepParams sp, int ctas) {
+  pdl_prologue();
+  const Kv4AttentionParams &p = sp.a;
+  constexpr int R = 8 * NT, kParts = R * D / 256;
+  __shared__ int before[kStepSequences + 1];
+  __shared__ float factor[R][kStepCtas];  // of each partial result of a row
+  __shared__ float row_lse[kKv4FewRows];
+  __shared__ float4 quarter[4][64];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kv = p.cache.kv_heads, total = p.seq * p.group, b = blockIdx.y / kv, h = blockIdx.y - b * kv;
+  const int length = kv4_length(p.lengths, b, p.cache.capacity);
+  const bool weighs = p.weights != nullptr && static_cast<int>(blockIdx.x) * 128 < length;
+  if (!weighs && (sp.whole || static_cast<int>(blockIdx.x) >= kParts * sp.tiles)) return;
+  int share = 0, start = 0;
+  if (!sp.whole) {
+    step_prefix<R>(sp, before);
+    share = step_share(before[p.cache.batch] * kv, ctas);
+    start = before[b] * kv;
+  }
+  for (int tile = 0; tile < sp.tiles; ++tile) {
+    const int blocks = step_range<R>(p, length, tile).blocks, segment = (b * sp.tiles + tile) * kv + h;
+    const bool joins = !sp.whole && static_cast<int>(blockIdx.x) / kParts == tile;
+    int slot0 = segment, slots = 1;
+    if (!sp.whole && blocks > 0) {
+      const int at = start + h * blocks;
+      slot0 = segment + at / share;
+      slots = (at + blocks - 1) / share - at / share + 1;
+    }
+    start += blocks * kv;
+    // a sequence without entries has no block: a cut grid has not written its rows
+    const bool none = blocks == 0 && !sp.whole;
+    if (weighs || (joins && slots > 1)) {
+      __syncthreads();
+      for (int r = warp; r < R; r += kStepWarps) {
+        float top = -INFINITY, norm = 0.f;
+        if (!none) {
+          for (int i = lane; i < slots; i += 32) top = fmaxf(top, sp.ml[static_cast<size_t>(slot0 + i) * 2 * R + r]);
+#pragma unroll
+          for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          for (int i = lane; i < slots; i += 32) {
+            const float m = sp.ml[static_cast<size_t>(slot0 + i) * 2 * R + r];
+            const float l = sp.ml[(static_cast<size_t>(slot0 + i) * 2 + 1) * R + r], f = l == 0.f ? 0.f : exp2_approx(m - top);
+            factor[r][i] = f;
+            norm = fmaf(l, f, norm);
+          }
+#pragma unroll
+          for (int off = 16; off >= 1; off >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, off);
+        }
+        const float inv = norm == 0.f ? 0.f : 1.f / norm;  // a row that sees nothing: zeros
+        __syncwarp();
+        for (int i = lane; i < slots; i += 32) factor[r][i] *= inv;
+        if (lane == 0 && tile * R + r < total) row_lse[tile * R + r] = norm == 0.f ? INFINITY : top + log2f(norm);
+      }
+      __syncthreads();
+    }
+    if (joins && (slots > 1 || none)) {
+      // 64 times four numbers, four threads for each: every fourth partial result
+      const int i = (blockIdx.x % kParts) * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6, r = i / (D / 4), row = tile * R + r;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (!none) {
+#pragma unroll 4
+        for (int k = part; k < slots; k += 4) {
+          const float f = factor[r][k];
+          if (f == 0.f) continue;
+          const float4 x = *reinterpret_cast<const float4 *>(sp.partial + static_cast<size_t>(slot0 + k) * R * D + 4 * i);
+          sum.x = fmaf(x.x, f, sum.x);
+          sum.y = fmaf(x.y, f, sum.y);
+          sum.z = fmaf(x.z, f, sum.z);
+          sum.w = fmaf(x.w, f, sum.w);
+        }
+      }
+      quarter[part][threadIdx.x & 63] = sum;
+      __syncthreads();
+      if (part == 0 && row < total) {
+#pragma unroll
+        for (int k = 1; k < 4; ++k) {
+          const float4 x = quarter[k][threadIdx.x];
+          sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+        }
+        const int q = row / p.group;
+        const size_t at = ((static_cast<size_t>(b) * p.seq + q) * p.heads + static_cast<size_t>(h) * p.group + (row - q * p.group)) * D + (i % (D / 4)) * 4;
+        uint2 w;
+        w.x = kv4_bits<T>(sum.x) | static_cast<uint32_t>(kv4_bits<T>(sum.y)) << 16;
+        w.y = kv4_bits<T>(sum.z) | static_cast<uint32_t>(kv4_bits<T>(sum.w)) << 16;
+        *reinterpret_cast<uint2 *>(p.out + at) = w;
+      }
+    }
+  }
+  if (!weighs) return;
+  // weights[j] += sum over all rows of exp2(score - lse): a warp per 16 entries goes over the rows in their order
+  const int j0 = blockIdx.x * 128 + warp * 16, g = lane >> 2, t = lane & 3;
   if (j0 >= length) return;
-  // rows whose query is at j0 or behind; with a window, and past the first entries, only those it reaches
-  int lo = max(0, j0 - (length - p.seq)), hi = p.seq;
-  if (p.window > 0 && j0 >= p.sinks) hi = static_cast<int>(min(static_cast<long long>(hi), static_cast<long long>(j0) + 15 + p.window - (length - p.seq)));
-  if (lo >= hi) return;
-  Kv4Block<D> blk;
-  kv4_load_block<D, false>(blk, p.cache, first, block);
+  const size_t first = static_cast<size_t>(blockIdx.y) * p.cache.capacity;
+  uint32_t k0[D / 32], k1[D / 32], kp[2];
+  kv4_load_words(k0, p.cache.k + (first + j0 + g) * (D / 2) + t * (D / 8));
+  kv4_load_words(k1, p.cache.k + (first + j0 + 8 + g) * (D / 2) + t * (D / 8));
+#pragma unroll
+  for (int e = 0; e < 2; ++e) kp[e] = *reinterpret_cast<const uint32_t *>(p.cache.params + (first + j0 + 8 * e + g) * 4);
   float sum[2] = {0.f, 0.f};
-  const float *lse = p.lse + static_cast<size_t>(blockIdx.y) * total;
-  for (int r0 = lo * p.group; r0 < hi * p.group; r0 += 8) {
+  for (int r0 = 0; r0 < total; r0 += 8) {
     Kv4Rows<D> rows;
     kv4_load_rows<T, D>(rows, p, b, h, r0, total, length);
     float s[4];
-    kv4_scores<T, D>(s, blk, rows);
+    kv4_scores<T, D>(s, k0, k1, kp, rows);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int row = r0 + 2 * t + (e & 1);
-      if (row < total && kv4_sees(rows.pos[e & 1], j0 + g + 8 * (e >> 1), p.window, p.sinks)) sum[e >> 1] += exp2_approx(s[e] - lse[row]);
+      if (row < total && kv4_sees(rows.pos[e & 1], j0 + g + 8 * (e >> 1), p.window, p.sinks)) sum[e >> 1] += exp2_approx(fmaf(s[e], rows.unit[e & 1], -row_lse[row]));
     }
   }
 #pragma unroll
@@ -415,62 +636,94 @@ __global__ void __launch_bounds__(256) kv4_weights_kernel(const Kv4AttentionPara
 
 namespace {
 
-template <typename T, int D, int NT> int kv4_attention_launch(const Kv4AttentionParams &p, cudaStream_t stream, bool pdl) {
-  constexpr int R = 8 * NT;
-  constexpr int smem = (kKv4Warps * R * (D + 2) + 2 * R) * 4;
-  static SharedMemoryOptIn opt_in;
-  int st = opt_in.ensure(kv4_attention_kernel<T, D, NT>, smem);
-  if (st != MG_OK) return st;
-  int sms = 0;
-  st = current_device_sm_count(&sms);
-  if (st != MG_OK) return st;
-  const int tiles = (p.seq * p.group + R - 1) / R, bh = p.cache.batch * p.cache.kv_heads;
-  if (tiles > 65535) return MG_ERR_UNSUPPORTED;
-  const long long most = p.window > 0 ? static_cast<long long>(p.window) + p.sinks + p.seq + 32 : p.cache.capacity;
-  const long long blocks = (std::min<long long>(most, p.cache.capacity) + 15) / 16;
-  int ctas = 1;
-  while (ctas < 8 && static_cast<long long>(tiles) * bh * ctas < 2 * sms && ctas * kKv4Warps < blocks) ctas *= 2;
+struct StepPlan {
+  int rows, tiles, segments, blocks;  // rows of a tile; blocks of a segment at most
+  bool whole;
+  int64_t slots, ml_bytes, partial_bytes;
+};
+
+StepPlan step_plan(const Kv4Cache &c, int seq, int group, int window, int sinks, bool weights) {
+  StepPlan s;
+  s.rows = seq * group <= 8 ? 8 : 16;
+  s.tiles = (seq * group + s.rows - 1) / s.rows;
+  s.segments = c.batch * c.kv_heads * s.tiles;
+  const int all = (c.capacity + kStepBlock - 1) / kStepBlock;
+  // a window of w entries and the s rows' own lie in at most (w + s - 2) / 32 + 2 blocks
+  s.blocks = window > 0 ? std::min(all, (window + seq - 2) / kStepBlock + 2 + (sinks + kStepBlock - 1) / kStepBlock) : all;
+  s.whole = s.blocks <= kStepWhole || c.batch > kStepSequences || s.segments >= 4 * kStepCtas;
+  s.slots = s.whole ? s.segments : s.segments + kStepCtas;
+  s.ml_bytes = s.whole && !weights ? 0 : s.slots * 2 * s.rows * 4;
+  s.partial_bytes = s.whole ? 0 : s.slots * s.rows * c.dim * 4;
+  return s;
+}
+
+template <typename Kernel, typename... Args>
+int launch_step(Kernel kernel, dim3 grid, int smem, cudaStream_t stream, bool pdl, Args... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, tiles, bh);
-  cfg.blockDim = dim3(kKv4Warps * 32);
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kStepWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kv4_attention_kernel<T, D, NT>, p) == cudaSuccess ? MG_OK : MG_ERR_CUDA;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? MG_OK : MG_ERR_CUDA;
 }
 
-template <typename T, int D> int kv4_attention_dispatch(const Kv4AttentionParams &p, cudaStream_t stream, bool pdl) {
-  const int st = p.seq * p.group <= 8 ? kv4_attention_launch<T, D, 1>(p, stream, pdl) : kv4_attention_launch<T, D, 2>(p, stream, pdl);
-  if (st != MG_OK || p.weights == nullptr) return st;
-  const dim3 grid((p.cache.capacity + 127) / 128, p.cache.batch * p.cache.kv_heads);
-  return launch_helper(kv4_weights_kernel<T, D>, grid, 256, stream, true, p);
+template <typename T, int D, int NT> int kv4_step(const Kv4StepParams &p, const StepPlan &plan, cudaStream_t stream, bool pdl) {
+  constexpr int ring = kStepWarps * kStepStages * StepStage<D>::bytes, part = kStepWarps * 8 * NT * D * 4, smem = ring > part ? ring : part;
+  static SharedMemoryOptIn opt_in;
+  int st = opt_in.ensure(kv4_step_kernel<T, D, NT>, smem);
+  if (st != MG_OK) return st;
+  const long long most = static_cast<long long>(plan.segments) * plan.blocks;
+  const int ctas = plan.whole ? plan.segments : static_cast<int>(std::min<long long>(kStepCtas, (most + kStepLeast - 1) / kStepLeast));
+  st = launch_step(kv4_step_kernel<T, D, NT>, dim3(ctas), smem, stream, pdl, p);
+  if (st != MG_OK || (plan.whole && p.a.weights == nullptr)) return st;
+  const int parts = plan.whole ? 1 : 8 * NT * D / 256 * plan.tiles;
+  const int entries = p.a.weights != nullptr ? (p.a.cache.capacity + 127) / 128 : 1;
+  return launch_step(kv4_finish_kernel<T, D, NT>, dim3(std::max(parts, entries), p.a.cache.batch * p.a.cache.kv_heads), 0, stream, true, p, ctas);
 }
+
+template <typename T, int D> int kv4_step_rows(const Kv4StepParams &p, const StepPlan &plan, cudaStream_t stream, bool pdl) {
+  return plan.rows == 8 ? kv4_step<T, D, 1>(p, plan, stream, pdl) : kv4_step<T, D, 2>(p, plan, stream, pdl);
+}
+
+int kv4_few_rows(const Kv4AttentionParams &a, void *workspace, bool bf16, bool pdl, cudaStream_t stream) {
+  const StepPlan plan = step_plan(a.cache, a.seq, a.group, a.window, a.sinks, a.weights != nullptr);
+  Kv4StepParams p = {};
+  p.a = a;
+  p.ml = static_cast<float *>(workspace);
+  p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + plan.ml_bytes);
+  p.tiles = plan.tiles;
+  p.whole = plan.whole;
+  if (a.cache.dim == 64) return bf16 ? kv4_step_rows<__nv_bfloat16, 64>(p, plan, stream, pdl) : kv4_step_rows<__half, 64>(p, plan, stream, pdl);
+  return bf16 ? kv4_step_rows<__nv_bfloat16, 128>(p, plan, stream, pdl) : kv4_step_rows<__half, 128>(p, plan, stream, pdl);
+}
+
+// a window or first entries past the capacity reach everything; kept small so that positions +- window stay in 32 bits
+int kv4_window(const Kv4Cache &c, int64_t window) { return static_cast<int>(window > c.capacity ? 0 : window); }
+int kv4_sinks(const Kv4Cache &c, int64_t sinks) { return static_cast<int>(sinks > c.capacity ? c.capacity : sinks); }
 
 }  // namespace
-
-int kv4_attention(const Kv4AttentionParams &p, bool bf16, bool pdl, cudaStream_t stream) {
-  if (p.seq * p.group > kKv4FewRows) return kv4_prompt_launch(p, bf16, pdl, stream);
-  if (p.cache.dim == 64)
-    return bf16 ? kv4_attention_dispatch<__nv_bfloat16, 64>(p, stream, pdl) : kv4_attention_dispatch<__half, 64>(p, stream, pdl);
-  return bf16 ? kv4_attention_dispatch<__nv_bfloat16, 128>(p, stream, pdl) : kv4_attention_dispatch<__half, 128>(p, stream, pdl);
-}
 
 }  // namespace mg
 
 extern "C" {
 
-int64_t matgptq_b200_attention_kv4_workspace_bytes(const matgptq_b200_kv4_cache *cache, int64_t seq, int64_t n_heads, int with_weights) {
-  if (!cache || !with_weights || cache->batch <= 0 || cache->n_kv_heads <= 0 || seq <= 0 || n_heads < cache->n_kv_heads) return 0;
-  const int64_t rows = seq * (n_heads / cache->n_kv_heads), heads = cache->batch * cache->n_kv_heads;
-  return rows <= mg::kKv4FewRows ? heads * rows * 4 : heads * ((rows + 127) / 128) * mg::kv4_row_tile_bytes(static_cast<int>(cache->head_dim));
+int64_t matgptq_b200_attention_kv4_workspace_bytes(const matgptq_b200_kv4_cache *cache, int64_t seq, int64_t n_heads, int64_t window,
+                                                   int64_t sinks, int with_weights) {
+  if (mg::kv4_check_cache(cache) != MG_OK || cache->batch == 0 || seq <= 0 || n_heads <= 0 || n_heads % cache->n_kv_heads != 0 || window < 0 ||
+      sinks < 0 || seq > (1 << 24) || n_heads > (1 << 16))
+    return 0;
+  const int64_t rows = seq * (n_heads / cache->n_kv_heads);
+  if (rows > mg::kKv4FewRows)
+    return with_weights ? cache->batch * cache->n_kv_heads * ((rows + 127) / 128) * mg::kv4_row_tile_bytes(static_cast<int>(cache->head_dim)) : 0;
+  const mg::Kv4Cache c = mg::kv4_cache(cache);
+  const mg::StepPlan plan = mg::step_plan(c, static_cast<int>(seq), static_cast<int>(rows / seq), mg::kv4_window(c, window), mg::kv4_sinks(c, sinks),
+                                          with_weights != 0);
+  return plan.ml_bytes + plan.partial_bytes;
 }
 
 int matgptq_b200_attention_kv4(const matgptq_b200_kv4_cache *cache, const void *q, int64_t seq, int64_t n_heads, const int32_t *lengths,
@@ -481,27 +734,27 @@ int matgptq_b200_attention_kv4(const matgptq_b200_kv4_cache *cache, const void *
   if (!q || !lengths || !out) return MG_ERR_BAD_ARG;
   if (seq < 0 || n_heads <= 0 || n_heads % cache->n_kv_heads != 0 || window < 0 || sinks < 0) return MG_ERR_BAD_ARG;
   if (seq > (1 << 24) || n_heads > (1 << 16) || seq * (n_heads / cache->n_kv_heads) > (1 << 24)) return MG_ERR_UNSUPPORTED;
-  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 != 0) return MG_ERR_ALIGNMENT;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) % 16 != 0) return MG_ERR_ALIGNMENT;
   if (cache->batch == 0 || seq == 0) return MG_OK;
-  if (weights && (!workspace || workspace_bytes < matgptq_b200_attention_kv4_workspace_bytes(cache, seq, n_heads, 1))) return MG_ERR_BAD_ARG;
-  if (weights && reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return MG_ERR_ALIGNMENT;
+  const int64_t need = matgptq_b200_attention_kv4_workspace_bytes(cache, seq, n_heads, window, sinks, weights != nullptr);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return MG_ERR_BAD_ARG;
   mg::Kv4AttentionParams p = {};
   p.cache = mg::kv4_cache(cache);
   p.q = static_cast<const uint16_t *>(q);
   p.out = static_cast<uint16_t *>(out);
   p.lengths = lengths;
   p.weights = weights;
-  const bool few = seq * (n_heads / cache->n_kv_heads) <= mg::kKv4FewRows;
-  p.lse = weights && few ? static_cast<float *>(workspace) : nullptr;
-  p.row_tiles = weights && !few ? static_cast<uint8_t *>(workspace) : nullptr;
   p.seq = static_cast<int>(seq);
   p.heads = static_cast<int>(n_heads);
   p.group = static_cast<int>(n_heads / cache->n_kv_heads);
-  // a window or first entries past the capacity reach everything; kept small so that positions +- window stay in 32 bits
-  p.window = static_cast<int>(window > cache->capacity ? 0 : window);
-  p.sinks = static_cast<int>(sinks > cache->capacity ? cache->capacity : sinks);
+  p.window = mg::kv4_window(p.cache, window);
+  p.sinks = mg::kv4_sinks(p.cache, sinks);
   p.scale_log2 = scale * 1.44269504088896340736f;
-  return mg::kv4_attention(p, (flags & MATGPTQ_B200_FLAG_BF16) != 0, (flags & MATGPTQ_B200_FLAG_PDL) != 0, static_cast<cudaStream_t>(stream));
+  const bool bf16 = (flags & MATGPTQ_B200_FLAG_BF16) != 0, pdl = (flags & MATGPTQ_B200_FLAG_PDL) != 0;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  if (p.seq * p.group <= mg::kKv4FewRows) return mg::kv4_few_rows(p, workspace, bf16, pdl, cs);
+  p.row_tiles = weights ? static_cast<uint8_t *>(workspace) : nullptr;
+  return mg::kv4_prompt_launch(p, bf16, pdl, cs);
 }
 
 }  // extern "C"

@@ -10,7 +10,6 @@ struct Kv4AttentionParams {
   uint16_t *out;       // [B, S, H, D]
   const int *lengths;  // [B]
   float *weights;      // [B, KV, capacity] or null
-  float *lse;          // few rows: [B, KV, rows] or null: log2 of the sum of exp2(score), scores in units of log 2
   uint8_t *row_tiles;  // many rows: [B, KV, tiles of 128 rows, kv4_row_tile_bytes] or null
   int seq, heads, group;
   int window, sinks;   // window 0: none
@@ -47,17 +46,48 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// Codes of two neighbours less 8, exact: 1024 + c and 1024 + 16 c are fp16 numbers with the code in their last bits.
-__device__ __forceinline__ uint32_t centred_low(uint32_t w) {
-  uint32_t r = (w & 0x000F000Fu) | 0x64006400u;
-  asm("add.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0xE408E408u));  // - 1032
+// Two fp32 numbers an instruction
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ uint32_t centred_high(uint32_t w) {
-  uint32_t r = (w & 0x00F000F0u) | 0x64006400u;
-  asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(r) : "r"(0x2C002C00u), "r"(0xD480D480u));  // / 16 - 72
+__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Codes of two neighbours less 8, exact: 1024 + c and 1024 + 16 c are fp16 numbers with the code in their last bits.  The constants are
+// made once, as registers: an instruction takes one literal.
+struct Centring {
+  uint32_t magic, low, sixteenth, high;  // 1024, -1032, 1 / 16, -72; twice each
+  __device__ __forceinline__ Centring() {
+    asm volatile("mov.b32 %0, 0x64006400;\n\tmov.b32 %1, 0xE408E408;\n\tmov.b32 %2, 0x2C002C00;\n\tmov.b32 %3, 0xD480D480;"
+                 : "=r"(magic), "=r"(low), "=r"(sixteenth), "=r"(high));
+  }
+  __device__ __forceinline__ uint32_t lower(uint32_t w) const {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;\n\tadd.rn.f16x2 %0, %0, %3;" : "=&r"(r) : "r"(w), "r"(magic), "r"(low));
+    return r;
+  }
+  __device__ __forceinline__ uint32_t upper(uint32_t w) const {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, 0x00F000F0, %2, 0xEA;\n\tfma.rn.f16x2 %0, %0, %3, %4;" : "=&r"(r) : "r"(w), "r"(magic), "r"(sixteenth), "r"(high));
+    return r;
+  }
+};
 
 constexpr int kKv4FewRows = 32;  // of a key/value head, for kv4_attention.cu; more go to kv4_prompt.cu
 

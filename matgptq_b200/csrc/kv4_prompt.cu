@@ -39,28 +39,6 @@ template <int D> struct PromptPlan {
   static constexpr int end = params + 2 * param_bytes;
 };
 
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
 // 32 columns of this warp's 32 lanes of tensor memory, and back; the caller waits
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *v) {
   asm volatile(
@@ -418,6 +396,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
         }
     };
     float v_unit = 0x1p-100f;
+    const Centring centre;
     if (tiles > 0) load(0);
     for (int t = 0; t < tiles; ++t) {
       const int stage = t & 1;
@@ -454,10 +433,10 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
       for (int v = 0; v < VP; ++v) {
         const uint32_t dst = v_at + (group0 + 4 * G * v) * kChunkV + unit_lane * 16;
         const uint32_t *w = vw[v];
-        sts_v4(dst, centred_low(w[0]), centred_low(w[1]), centred_low(w[2]), centred_low(w[3]));
-        sts_v4(dst + U * 16, centred_high(w[0]), centred_high(w[1]), centred_high(w[2]), centred_high(w[3]));
-        sts_v4(dst + 2 * U * 16, centred_low(w[0] >> 8), centred_low(w[1] >> 8), centred_low(w[2] >> 8), centred_low(w[3] >> 8));
-        sts_v4(dst + 3 * U * 16, centred_high(w[0] >> 8), centred_high(w[1] >> 8), centred_high(w[2] >> 8), centred_high(w[3] >> 8));
+        sts_v4(dst, centre.lower(w[0]), centre.lower(w[1]), centre.lower(w[2]), centre.lower(w[3]));
+        sts_v4(dst + U * 16, centre.upper(w[0]), centre.upper(w[1]), centre.upper(w[2]), centre.upper(w[3]));
+        sts_v4(dst + 2 * U * 16, centre.lower(w[0] >> 8), centre.lower(w[1] >> 8), centre.lower(w[2] >> 8), centre.lower(w[3] >> 8));
+        sts_v4(dst + 3 * U * 16, centre.upper(w[0] >> 8), centre.upper(w[1] >> 8), centre.upper(w[2] >> 8), centre.upper(w[3] >> 8));
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();

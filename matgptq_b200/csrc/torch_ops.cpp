@@ -371,7 +371,7 @@ Tensor attention_kv4(const Tensor &q, const Tensor &k_codes, const Tensor &v_cod
   const Tensor x = dense16(q);
   Tensor out = empty_on({cache.batch, seq, heads, cache.head_dim}, type_of(flags), dev);
   if (out.numel() == 0) return out;
-  const int64_t need = lib.attention_kv4_workspace_bytes(&cache, seq, heads, weights.has_value());
+  const int64_t need = lib.attention_kv4_workspace_bytes(&cache, seq, heads, window, sinks, weights.has_value());
   const Tensor ws = need > 0 ? empty_on({need}, at::kByte, dev) : Tensor();
   check_status(lib.attention_kv4(&cache, x.const_data_ptr(), seq, heads, lengths.const_data_ptr<int32_t>(), window, sinks,
                                  static_cast<float>(scale), weights ? weights->data_ptr<float>() : nullptr, out.data_ptr(),

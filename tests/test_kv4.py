@@ -95,12 +95,24 @@ def test_c_abi_refuses_bad_arguments(lib):
     assert lib.matgptq_b200_dequantize_kv4(c, p, 4, None, p, 0, None) == 1
     assert lib.matgptq_b200_dequantize_kv4(c, p, 4, p, odd, 0, None) == 4
     assert lib.matgptq_b200_dequantize_kv4(c, p, 0, None, None, 0, None) == 0
-    assert lib.matgptq_b200_attention_kv4_workspace_bytes(c, 5, H, 0) == 0
-    assert lib.matgptq_b200_attention_kv4_workspace_bytes(None, 5, H, 1) == 0
+    assert lib.matgptq_b200_attention_kv4_workspace_bytes(c, 5, H, 0, 0, 0) == 0
+    assert lib.matgptq_b200_attention_kv4_workspace_bytes(None, 5, H, 0, 0, 1) == 0
     for seq in (1, 5, 16, 17, 500):
-        need = lib.matgptq_b200_attention_kv4_workspace_bytes(c, seq, H, 1)
+        need = lib.matgptq_b200_attention_kv4_workspace_bytes(c, seq, H, 0, 0, 1)
         assert need >= B * seq * H * 4
+        assert lib.matgptq_b200_attention_kv4_workspace_bytes(c, seq, H, 9, 1, 1) >= B * seq * H * 4
         assert attend(seq=seq, weights=p, ws=p, ws_bytes=need - 1) == 1 and attend(seq=seq, weights=p, ws=odd, ws_bytes=need) == 4
+
+
+def test_long_caches_need_a_workspace(lib):
+    """Few rows over many entries: the work is cut into shares, whose partial results go through the workspace."""
+    p = 1 << 23
+    c = native_cache(capacity=1 << 17)
+    need = lib.matgptq_b200_attention_kv4_workspace_bytes(c, 1, H, 0, 0, 0)
+    assert need > 0
+    attend = lambda ws, n: lib.matgptq_b200_attention_kv4(c, p, 1, H, p, 0, 0, 1.0, None, p, ws, n, 0, None)  # noqa: E731
+    assert attend(None, need) == 1 and attend(p, need - 1) == 1 and attend(p + 8, need) == 4
+    assert lib.matgptq_b200_attention_kv4_workspace_bytes(c, 1, H, 100, 4, 0) == 0  # a window that one CTA takes as a whole
 
 
 def test_cache_refuses_bad_shapes():
