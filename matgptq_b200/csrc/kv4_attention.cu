@@ -145,21 +145,21 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
 // ---- the work and who does it ---------------------------------------------------------------------------------------
 //
 // A segment is a tile of R = 8 or 16 rows of one key/value head of one sequence, its work the blocks of 32 entries that these rows
-// see.  Segments of few blocks get a CTA each.  Otherwise the blocks of all segments, one behind the other (sequence, tile, head), are
-// cut into equal shares, one for each CTA of a grid that fills the GPU, whatever the lengths: a share may begin and end inside a
-// segment, and the CTAs of a segment leave partial results, which kv4_finish_kernel joins in their order.  Lengths are known on the
-// device only, so every CTA works the cuts out by itself.
+// see.  Segments of few blocks get a CTA each.  Otherwise a segment is cut into pieces of equal size, none larger than a share that
+// makes about `kStepCtas` pieces of all the work; each piece is a CTA, leaves a partial result, and kv4_finish_kernel joins them in
+// their order.  Lengths are known on the device only: every CTA works out by itself which piece is its own, and the grid is as large as
+// the pieces can become.  (A CTA that goes on into the next segment, for shares that are all equal, has the latencies of a second
+// beginning and end one after the other: 16384 entries of 8 heads 19.6 us.)
 constexpr int kStepWarps = 8;
 constexpr int kStepBlock = 32;       // entries of a block
 constexpr int kStepStages = 3;       // blocks in flight per warp
 constexpr int kStepCtas = 296;       // two on each SM of a B200
 constexpr int kStepLeast = kStepWarps;  // blocks of a share at least: one for each warp
-constexpr int kStepSequences = 1024;    // whose blocks are cut into shares, at most
-// Blocks of a segment up to which it is not cut.
-constexpr int kStepWhole = 64;
+constexpr int kStepWhole = 64;          // blocks of a segment up to which it is not cut
 
 struct Kv4StepParams {
   Kv4AttentionParams a;
+  int2 *pieces;    // [segments]: first slot and number of pieces of each segment that has blocks
   float *ml;       // [slots][2][R]: maximum and sum of the partial result in a slot
   float *partial;  // [slots][R][D]
   int tiles;       // of rows
@@ -175,40 +175,70 @@ template <int R> __device__ __forceinline__ Kv4Range step_range(const Kv4Attenti
   return kv4_range<kStepBlock>(length - p.seq + r0 / p.group, length - p.seq + (min(r0 + R, total) - 1) / p.group, p.window, p.sinks, p.cache.capacity);
 }
 
-// before[b]: blocks of one head (all its tiles) of the sequences before b; before[batch]: of all.  All threads of the CTA.
-template <int R> __device__ __forceinline__ void step_prefix(const Kv4StepParams &p, int *before) {
-  __shared__ int warp_sum[kStepWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int carry = 0;
-  for (int b0 = 0; b0 < p.a.cache.batch; b0 += kStepWarps * 32) {
-    const int b = b0 + threadIdx.x;
-    int n = 0;
-    if (b < p.a.cache.batch) {
-      const int length = kv4_length(p.a.lengths, b, p.a.cache.capacity);
-      for (int tile = 0; tile < p.tiles; ++tile) n += step_range<R>(p.a, length, tile).blocks;
-    }
-    int sum = n;
+__device__ __forceinline__ int warp_sum(int x) {
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, sum, off);
-      if (lane >= off) sum += x;
-    }
-    __syncthreads();
-    if (lane == 31) warp_sum[warp] = sum;
-    __syncthreads();
-    int all = 0;
-    for (int w = 0; w < kStepWarps; ++w) {
-      if (w < warp) sum += warp_sum[w];
-      all += warp_sum[w];
-    }
-    if (b < p.a.cache.batch) before[b] = carry + sum - n;
-    carry += all;
-  }
-  if (threadIdx.x == 0) before[p.a.cache.batch] = carry;
-  __syncthreads();
+  for (int off = 16; off >= 1; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+  return x;
 }
 
-__device__ __forceinline__ int step_share(int blocks, int ctas) { return max((blocks + ctas - 1) / ctas, kStepLeast); }
+// The piece of CTA `cta`: its segment (b, tile, h), which of its segment's pieces it is, and how many these are; false where there are
+// fewer pieces than CTAs.  Pieces are numbered by sequence, tile and head; a warp looks at 32 sequences at a time.
+struct StepPiece {
+  int b, tile, h, index, pieces, length;
+};
+template <int R> __device__ __forceinline__ bool step_find(StepPiece &s, const Kv4StepParams &p, int cta) {
+  const int kv = p.a.cache.kv_heads, batch = p.a.cache.batch, lane = threadIdx.x & 31;
+  if (p.whole) {
+    s.b = cta / (p.tiles * kv);
+    s.tile = (cta - s.b * p.tiles * kv) / kv;
+    s.h = cta - (s.b * p.tiles + s.tile) * kv;
+    s.index = 0;
+    s.pieces = 1;
+    s.length = kv4_length(p.a.lengths, s.b, p.a.cache.capacity);
+    return true;
+  }
+  int all = 0;  // blocks
+  for (int b0 = 0; b0 < batch; b0 += 32) {
+    if (b0 + lane < batch) {
+      const int length = kv4_length(p.a.lengths, b0 + lane, p.a.cache.capacity);
+      for (int tile = 0; tile < p.tiles; ++tile) all += step_range<R>(p.a, length, tile).blocks;
+    }
+  }
+  all = warp_sum(all) * kv;
+  const int share = max((all + kStepCtas - 1) / kStepCtas, kStepLeast);
+  const auto cut = [&](int blocks) { return (blocks + share - 1) / share; };
+  int before = 0;
+  for (int b0 = 0; b0 < batch; b0 += 32) {
+    int length = 0, mine = 0;
+    if (b0 + lane < batch) {
+      length = kv4_length(p.a.lengths, b0 + lane, p.a.cache.capacity);
+      for (int tile = 0; tile < p.tiles; ++tile) mine += cut(step_range<R>(p.a, length, tile).blocks) * kv;
+    }
+    int up_to = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, up_to, off);
+      if (lane >= off) up_to += x;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, before + up_to > cta);
+    if (past != 0) {
+      const int l = __ffs(past) - 1;  // the sequence that the piece is in
+      s.b = b0 + l;
+      s.length = __shfl_sync(0xffffffffu, length, l);
+      int at = cta - before - __shfl_sync(0xffffffffu, up_to - mine, l);
+      for (s.tile = 0; s.tile < p.tiles; ++s.tile) {
+        s.pieces = cut(step_range<R>(p.a, s.length, s.tile).blocks);
+        if (at < s.pieces * kv) break;
+        at -= s.pieces * kv;
+      }
+      s.h = at / s.pieces;
+      s.index = at - s.h * s.pieces;
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, up_to, 31);
+  }
+  return false;
+}
 
 // What a warp has of its rows' sums so far
 template <int D, int NT> struct StepSums {
@@ -345,161 +375,203 @@ __global__ void __launch_bounds__(kStepWarps * 32, NT == 1 ? 2 : 1) kv4_step_ker
   constexpr int R = 8 * NT, W = D / 32;
   using Stage = StepStage<D>;
   extern __shared__ __align__(128) unsigned char step_smem[];
-  __shared__ int before[kStepSequences + 1];
   __shared__ float part_m[kStepWarps][R], part_l[kStepWarps][R];
   float *part = reinterpret_cast<float *>(step_smem);  // [warps][R][D], over the stages once these are done with
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   unsigned char *ring = step_smem + warp * kStepStages * Stage::bytes;
   const uint32_t ring_u32 = smem_u32(ring);
-  const Centring centre;
   const int kv = p.cache.kv_heads, total = p.seq * p.group;
-  int pos = 0, end = 1, share = 0;
-  if (!sp.whole) {
-    step_prefix<R>(sp, before);
-    const int all = before[p.cache.batch] * kv;
-    share = step_share(all, gridDim.x);
-    pos = min(static_cast<int>(blockIdx.x) * share, all);
-    end = min(pos + share, all);
+  StepPiece piece;
+  if (!step_find<R>(piece, sp, blockIdx.x)) return;
+  const int b = piece.b, tile = piece.tile, h = piece.h, length = piece.length, slot = blockIdx.x;
+  const Kv4Range range = step_range<R>(p, length, tile);
+  const bool complete = piece.pieces == 1;
+  const int r0 = tile * R;
+  const int pos_lo = length - p.seq + r0 / p.group, pos_hi = length - p.seq + (min(r0 + R, total) - 1) / p.group;
+  const size_t first = (static_cast<size_t>(b) * kv + h) * p.cache.capacity;
+  const int lo = static_cast<int>(static_cast<long long>(range.blocks) * piece.index / piece.pieces);
+  const int count = static_cast<int>(static_cast<long long>(range.blocks) * (piece.index + 1) / piece.pieces) - lo;
+  const int from = lo + count * warp / kStepWarps, to = lo + count * (warp + 1) / kStepWarps;
+  if (!sp.whole && piece.index == 0 && threadIdx.x == 0) sp.pieces[(b * sp.tiles + tile) * kv + h] = make_int2(slot, piece.pieces);
+
+  // a block into a stage, 16 bytes a lane at a time; every call is a group of its own, with nothing in it behind the last block
+  const auto request = [&](int i, uint32_t stage) {
+    if (i < to) {
+      const size_t e = first + static_cast<size_t>(range.block(i)) * kStepBlock;
+      const uint32_t dst = ring_u32 + stage * Stage::bytes + lane * 16;
+      const uint8_t *k = p.cache.k + e * (D / 2) + lane * 16, *v = p.cache.v + e * (D / 2) + lane * 16;
+#pragma unroll
+      for (int c = 0; c < kStepBlock * D / 2; c += 512) {
+        cp_async16(dst + Stage::k + c, k + c);
+        cp_async16(dst + Stage::v + c, v + c);
+      }
+      if (lane < kStepBlock / 2) cp_async16(dst + Stage::params, reinterpret_cast<const uint8_t *>(p.cache.params) + e * 8 + lane * 16);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kStepStages; ++i) request(from + i, i);
+
+  Kv4Rows<D> rows[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) kv4_load_rows<T, D>(rows[n], p, b, h, r0 + 8 * n, total, length);
+
+  StepSums<D, NT> a;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int i = 0; i < 2 * W; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a.o[n][i][e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) a.m[n][k] = a.limit[n][k] = -INFINITY, a.shift[n][k] = a.l[n][k] = a.fix[n][k] = 0.f;
   }
-  while (pos < end) {
-    // ---- the piece of a segment that starts at pos
-    int b, tile = 0, h, offset = 0;
-    if (sp.whole) {
-      b = blockIdx.x / (sp.tiles * kv);
-      tile = (blockIdx.x - b * sp.tiles * kv) / kv;
-      h = blockIdx.x - (b * sp.tiles + tile) * kv;
-    } else {
-      int lo = 0, hi = p.cache.batch - 1;  // the last sequence that begins at pos or before, and has blocks
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (before[mid] * kv <= pos) lo = mid; else hi = mid - 1;
+  a.v_unit = 0x1p-100f, a.v_per = 0x1p100f;
+
+  const Centring centre;
+  uint32_t taken = 0;  // the stage that comes next
+  for (int i = from; i < to; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStepStages - 1) : "memory");
+    __syncwarp();  // the other lanes' bytes as well
+    const uint8_t *blk = ring + taken * Stage::bytes;
+    const int j0 = range.block(i) * kStepBlock;
+    // (rows that there are not count for nothing, whatever they see)
+    if (j0 + kStepBlock - 1 <= pos_lo && (p.window == 0 || j0 > pos_hi - p.window || j0 + kStepBlock <= p.sinks))
+      step_block<T, D, NT, true>(a, rows, blk, j0, pos_hi, p.window, p.sinks, centre);
+    else
+      step_block<T, D, NT, false>(a, rows, blk, j0, pos_hi, p.window, p.sinks, centre);
+    __syncwarp();  // every lane has read the stage
+    request(i + kStepStages, taken);
+    taken = taken == kStepStages - 1 ? 0 : taken + 1;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+  // ---- the warps' sums; lanes of equal t hold parts of the same rows' l and fix
+  __syncthreads();  // the stages are done with
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int off = 4; off <= 16; off <<= 1) {
+        a.l[n][k] += __shfl_xor_sync(0xffffffffu, a.l[n][k], off);
+        a.fix[n][k] += __shfl_xor_sync(0xffffffffu, a.fix[n][k], off);
       }
-      b = lo;
-      offset = pos - before[b] * kv;
-    }
-    const int length = kv4_length(p.lengths, b, p.cache.capacity);
-    Kv4Range range = step_range<R>(p, length, tile);
-    if (!sp.whole) {
-      while (offset >= range.blocks * kv) {
-        offset -= range.blocks * kv;
-        range = step_range<R>(p, length, ++tile);
+      const int row = 8 * n + 2 * t + k;
+      if (g == 0) {
+        part_m[warp][row] = a.m[n][k];
+        part_l[warp][row] = a.l[n][k];
       }
-      h = offset / range.blocks;
-      offset -= h * range.blocks;
-    }
-    const int count = sp.whole ? range.blocks : min(range.blocks - offset, end - pos);
-    const bool complete = count == range.blocks;
-    const int segment = (b * sp.tiles + tile) * kv + h, slot = sp.whole ? segment : segment + blockIdx.x;
-    const int r0 = tile * R;
-    const int pos_lo = length - p.seq + r0 / p.group, pos_hi = length - p.seq + (min(r0 + R, total) - 1) / p.group;
-    const size_t first = (static_cast<size_t>(b) * kv + h) * p.cache.capacity;
-    const int from = offset + count * warp / kStepWarps, to = offset + count * (warp + 1) / kStepWarps;
-
-    // a block into a stage, 16 bytes a lane at a time; every call is a group of its own, with nothing in it behind the last block
-    const auto request = [&](int i, uint32_t stage) {
-      if (i < to) {
-        const size_t e = first + static_cast<size_t>(range.block(i)) * kStepBlock;
-        const uint32_t dst = ring_u32 + stage * Stage::bytes + lane * 16;
-        const uint8_t *k = p.cache.k + e * (D / 2) + lane * 16, *v = p.cache.v + e * (D / 2) + lane * 16;
+      if (from < to) {
 #pragma unroll
-        for (int c = 0; c < kStepBlock * D / 2; c += 512) {
-          cp_async16(dst + Stage::k + c, k + c);
-          cp_async16(dst + Stage::v + c, v + c);
+        for (int w = 0; w < W; ++w) {
+          float4 x;  // channels D/8 g + 4 w + 0 .. 3
+          x.x = fmaf(a.o[n][2 * w][k], a.v_unit, a.fix[n][k]);
+          x.y = fmaf(a.o[n][2 * w][2 + k], a.v_unit, a.fix[n][k]);
+          x.z = fmaf(a.o[n][2 * w + 1][k], a.v_unit, a.fix[n][k]);
+          x.w = fmaf(a.o[n][2 * w + 1][2 + k], a.v_unit, a.fix[n][k]);
+          *reinterpret_cast<float4 *>(part + (warp * R + row) * D + (D / 8) * g + 4 * w) = x;
         }
-        if (lane < kStepBlock / 2) cp_async16(dst + Stage::params, reinterpret_cast<const uint8_t *>(p.cache.params) + e * 8 + lane * 16);
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-#pragma unroll
-    for (int i = 0; i < kStepStages; ++i) request(from + i, i);
-
-    Kv4Rows<D> rows[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) kv4_load_rows<T, D>(rows[n], p, b, h, r0 + 8 * n, total, length);
-
-    StepSums<D, NT> a;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int i = 0; i < 2 * W; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a.o[n][i][e] = 0.f;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) a.m[n][k] = a.limit[n][k] = -INFINITY, a.shift[n][k] = a.l[n][k] = a.fix[n][k] = 0.f;
     }
-    a.v_unit = 0x1p-100f, a.v_per = 0x1p100f;
-
-    uint32_t taken = 0;  // the stage that comes next
-    for (int i = from; i < to; ++i) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStepStages - 1) : "memory");
-      __syncwarp();  // the other lanes' bytes as well
-      const uint8_t *blk = ring + taken * Stage::bytes;
-      const int j0 = range.block(i) * kStepBlock;
-      if (j0 + kStepBlock - 1 <= pos_lo && r0 + R <= total && (p.window == 0 || j0 > pos_hi - p.window || j0 + kStepBlock <= p.sinks))
-        step_block<T, D, NT, true>(a, rows, blk, j0, pos_hi, p.window, p.sinks, centre);
-      else
-        step_block<T, D, NT, false>(a, rows, blk, j0, pos_hi, p.window, p.sinks, centre);
-      __syncwarp();  // every lane has read the stage
-      request(i + kStepStages, taken);
-      taken = taken == kStepStages - 1 ? 0 : taken + 1;
+  __syncthreads();
+  for (int i = threadIdx.x; i < R * D / 4; i += kStepWarps * 32) {
+    const int r = i / (D / 4), row = r0 + r;
+    float top = -INFINITY, norm = 0.f;
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, part_m[w][r]);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w) {
+      if (part_l[w][r] == 0.f) continue;  // nothing seen
+      const float f = exp2_approx(part_m[w][r] - top);
+      norm = fmaf(part_l[w][r], f, norm);
+      const float4 x = *reinterpret_cast<const float4 *>(part + (w * R) * D + 4 * i);
+      sum.x = fmaf(x.x, f, sum.x);
+      sum.y = fmaf(x.y, f, sum.y);
+      sum.z = fmaf(x.z, f, sum.z);
+      sum.w = fmaf(x.w, f, sum.w);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if ((!complete || p.weights != nullptr) && i % (D / 4) == 0) {
+      sp.ml[(static_cast<size_t>(slot) * 2) * R + r] = top;
+      sp.ml[(static_cast<size_t>(slot) * 2 + 1) * R + r] = norm;
+    }
+    if (!complete) {
+      *reinterpret_cast<float4 *>(sp.partial + static_cast<size_t>(slot) * R * D + 4 * i) = sum;
+    } else if (row < total) {
+      const float inv = norm == 0.f ? 0.f : 1.f / norm;  // a row that sees nothing: zeros
+      const int q = row / p.group;
+      const size_t at = ((static_cast<size_t>(b) * p.seq + q) * p.heads + static_cast<size_t>(h) * p.group + (row - q * p.group)) * D + (i % (D / 4)) * 4;
+      uint2 w;
+      w.x = kv4_bits<T>(sum.x * inv) | static_cast<uint32_t>(kv4_bits<T>(sum.y * inv)) << 16;
+      w.y = kv4_bits<T>(sum.z * inv) | static_cast<uint32_t>(kv4_bits<T>(sum.w * inv)) << 16;
+      *reinterpret_cast<uint2 *>(p.out + at) = w;
+    }
+  }
+}
 
-    // ---- the warps' sums; lanes of equal t hold parts of the same rows' l and fix
-    __syncthreads();  // the stages are done with
+// What is left once every piece has been seen: joins the partial results of segments that were cut, and adds up the weights.
+// blockIdx.y: sequence and head; blockIdx.x: a part of a tile's results (256 numbers), and 128 entries whose weights are due.
+template <typename T, int D, int NT> __global__ void __launch_bounds__(kStepWarps * 32) kv4_finish_kernel(const Kv4StepParams sp) {
+  pdl_prologue();
+  const Kv4AttentionParams &p = sp.a;
+  constexpr int R = 8 * NT, kParts = R * D / 256;
+  __shared__ float row_lse[kKv4FewRows];
+  __shared__ float4 quarter[3][64];
+  __shared__ float quarter_m[3][64], quarter_l[3][64];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kv = p.cache.kv_heads, total = p.seq * p.group, b = blockIdx.y / kv, h = blockIdx.y - b * kv;
+  const int part = blockIdx.x, tile = part / kParts;
+  const bool joins = !sp.whole && tile < sp.tiles;
+  int2 pieces = make_int2(0, 1);
+  if (joins) pieces = sp.pieces[(b * sp.tiles + tile) * kv + h];
+  const int length = kv4_length(p.lengths, b, p.cache.capacity);
+  if (joins) {
+    // a sequence without entries has no piece: its rows have not been written
+    if (step_range<R>(p, length, tile).blocks == 0) pieces.y = 0;
+    if (pieces.y != 1) {
+      // 64 times four numbers, four threads for each: every fourth partial result
+      const int i = (part - tile * kParts) * 64 + (threadIdx.x & 63), fourth = threadIdx.x >> 6, r = i / (D / 4), row = tile * R + r;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      float m = -INFINITY, l = 0.f;
+      const auto add = [&](float m1, float l1, float4 x) {
+        if (l1 == 0.f) return;
+        const float top = fmaxf(m, m1), f = l == 0.f ? 0.f : exp2_approx(m - top), f1 = exp2_approx(m1 - top);
+        m = top;
+        l = fmaf(l, f, l1 * f1);
+        sum.x = fmaf(sum.x, f, x.x * f1);
+        sum.y = fmaf(sum.y, f, x.y * f1);
+        sum.z = fmaf(sum.z, f, x.z * f1);
+        sum.w = fmaf(sum.w, f, x.w * f1);
+      };
+      constexpr int kAhead = 5;
+      for (int k = fourth; k < pieces.y; k += 4 * kAhead) {
+        float4 x[kAhead];
+        float m1[kAhead], l1[kAhead];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-#pragma unroll
-        for (int off = 4; off <= 16; off <<= 1) {
-          a.l[n][k] += __shfl_xor_sync(0xffffffffu, a.l[n][k], off);
-          a.fix[n][k] += __shfl_xor_sync(0xffffffffu, a.fix[n][k], off);
-        }
-        const int row = 8 * n + 2 * t + k;
-        if (g == 0) {
-          part_m[warp][row] = a.m[n][k];
-          part_l[warp][row] = a.l[n][k];
-        }
-        if (from < to) {
-#pragma unroll
-          for (int w = 0; w < W; ++w) {
-            float4 x;  // channels D/8 g + 4 w + 0 .. 3
-            x.x = fmaf(a.o[n][2 * w][k], a.v_unit, a.fix[n][k]);
-            x.y = fmaf(a.o[n][2 * w][2 + k], a.v_unit, a.fix[n][k]);
-            x.z = fmaf(a.o[n][2 * w + 1][k], a.v_unit, a.fix[n][k]);
-            x.w = fmaf(a.o[n][2 * w + 1][2 + k], a.v_unit, a.fix[n][k]);
-            *reinterpret_cast<float4 *>(part + (warp * R + row) * D + (D / 8) * g + 4 * w) = x;
+        for (int u = 0; u < kAhead; ++u) {
+          const size_t slot = pieces.x + k + 4 * u;
+          l1[u] = 0.f;
+          if (k + 4 * u < pieces.y) {
+            m1[u] = sp.ml[slot * 2 * R + r];
+            l1[u] = sp.ml[(slot * 2 + 1) * R + r];
+            x[u] = *reinterpret_cast<const float4 *>(sp.partial + slot * R * D + 4 * i);
           }
         }
-      }
-    __syncthreads();
-    for (int i = threadIdx.x; i < R * D / 4; i += kStepWarps * 32) {
-      const int r = i / (D / 4), row = r0 + r;
-      float top = -INFINITY, norm = 0.f;
 #pragma unroll
-      for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, part_m[w][r]);
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int u = 0; u < kAhead; ++u) add(m1[u], l1[u], x[u]);
+      }
+      if (fourth > 0) {
+        quarter[fourth - 1][threadIdx.x & 63] = sum;
+        quarter_m[fourth - 1][threadIdx.x & 63] = m;
+        quarter_l[fourth - 1][threadIdx.x & 63] = l;
+      }
+      __syncthreads();
+      if (fourth == 0 && row < total) {
 #pragma unroll
-      for (int w = 0; w < kStepWarps; ++w) {
-        if (part_l[w][r] == 0.f) continue;  // nothing seen
-        const float f = exp2_approx(part_m[w][r] - top);
-        norm = fmaf(part_l[w][r], f, norm);
-        const float4 x = *reinterpret_cast<const float4 *>(part + (w * R) * D + 4 * i);
-        sum.x = fmaf(x.x, f, sum.x);
-        sum.y = fmaf(x.y, f, sum.y);
-        sum.z = fmaf(x.z, f, sum.z);
-        sum.w = fmaf(x.w, f, sum.w);
-      }
-      if ((!complete || p.weights != nullptr) && i % (D / 4) == 0) {
-        sp.ml[(static_cast<size_t>(slot) * 2) * R + r] = top;
-        sp.ml[(static_cast<size_t>(slot) * 2 + 1) * R + r] = norm;
-      }
-      if (!complete) {
-        *reinterpret_cast<float4 *>(sp.partial + static_cast<size_t>(slot) * R * D + 4 * i) = sum;
-      } else if (row < total) {
-        const float inv = norm == 0.f ? 0.f : 1.f / norm;  // a row that sees nothing: zeros
+        for (int k = 0; k < 3; ++k) add(quarter_m[k][threadIdx.x], quarter_l[k][threadIdx.x], quarter[k][threadIdx.x]);
+        const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
         const int q = row / p.group;
         const size_t at = ((static_cast<size_t>(b) * p.seq + q) * p.heads + static_cast<size_t>(h) * p.group + (row - q * p.group)) * D + (i % (D / 4)) * 4;
         uint2 w;
@@ -508,102 +580,31 @@ __global__ void __launch_bounds__(kStepWarps * 32, NT == 1 ? 2 : 1) kv4_step_ker
         *reinterpret_cast<uint2 *>(p.out + at) = w;
       }
     }
-    pos += sp.whole ? 1 : count;
-    if (pos < end) __syncthreads();  // before copies land where sums were
   }
-}
-
-// What is left once every segment's blocks have been seen: joins the partial results of segments that were cut, and adds up the weights.
-// blockIdx.y: sequence and head; blockIdx.x: a part of a tile's results (256 numbers), and 128 entries whose weights are due.
-template <typename T, int D, int NT> __global__ void __launch_bounds__(kStepWarps * 32) kv4_finish_kernel(const Kv4StepParams sp, int ctas) {
-  pdl_prologue();
-  const Kv4AttentionParams &p = sp.a;
-  constexpr int R = 8 * NT, kParts = R * D / 256;
-  __shared__ int before[kStepSequences + 1];
-  __shared__ float factor[R][kStepCtas];  // of each partial result of a row
-  __shared__ float row_lse[kKv4FewRows];
-  __shared__ float4 quarter[4][64];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kv = p.cache.kv_heads, total = p.seq * p.group, b = blockIdx.y / kv, h = blockIdx.y - b * kv;
-  const int length = kv4_length(p.lengths, b, p.cache.capacity);
-  const bool weighs = p.weights != nullptr && static_cast<int>(blockIdx.x) * 128 < length;
-  if (!weighs && (sp.whole || static_cast<int>(blockIdx.x) >= kParts * sp.tiles)) return;
-  int share = 0, start = 0;
-  if (!sp.whole) {
-    step_prefix<R>(sp, before);
-    share = step_share(before[p.cache.batch] * kv, ctas);
-    start = before[b] * kv;
+  if (p.weights == nullptr || part * 128 >= length) return;
+  // the rows' sums: a warp per row
+  for (int row = warp; row < total; row += kStepWarps) {
+    const int segment = (b * sp.tiles + row / R) * kv + h, r = row % R;
+    int2 of = make_int2(segment, 1);
+    if (!sp.whole) of = sp.pieces[segment];
+    if (step_range<R>(p, length, row / R).blocks == 0) of.y = 0;
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < of.y; i += 32) {
+      const float m1 = sp.ml[static_cast<size_t>(of.x + i) * 2 * R + r], l1 = sp.ml[(static_cast<size_t>(of.x + i) * 2 + 1) * R + r];
+      if (l1 == 0.f) continue;
+      const float top = fmaxf(m, m1);
+      l = (l == 0.f ? 0.f : l * exp2_approx(m - top)) + l1 * exp2_approx(m1 - top);
+      m = top;
+    }
+    float top = m;
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    l = l == 0.f ? 0.f : l * exp2_approx(m - top);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    if (lane == 0) row_lse[row] = l == 0.f ? INFINITY : top + log2f(l);
   }
-  for (int tile = 0; tile < sp.tiles; ++tile) {
-    const int blocks = step_range<R>(p, length, tile).blocks, segment = (b * sp.tiles + tile) * kv + h;
-    const bool joins = !sp.whole && static_cast<int>(blockIdx.x) / kParts == tile;
-    int slot0 = segment, slots = 1;
-    if (!sp.whole && blocks > 0) {
-      const int at = start + h * blocks;
-      slot0 = segment + at / share;
-      slots = (at + blocks - 1) / share - at / share + 1;
-    }
-    start += blocks * kv;
-    // a sequence without entries has no block: a cut grid has not written its rows
-    const bool none = blocks == 0 && !sp.whole;
-    if (weighs || (joins && slots > 1)) {
-      __syncthreads();
-      for (int r = warp; r < R; r += kStepWarps) {
-        float top = -INFINITY, norm = 0.f;
-        if (!none) {
-          for (int i = lane; i < slots; i += 32) top = fmaxf(top, sp.ml[static_cast<size_t>(slot0 + i) * 2 * R + r]);
-#pragma unroll
-          for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-          for (int i = lane; i < slots; i += 32) {
-            const float m = sp.ml[static_cast<size_t>(slot0 + i) * 2 * R + r];
-            const float l = sp.ml[(static_cast<size_t>(slot0 + i) * 2 + 1) * R + r], f = l == 0.f ? 0.f : exp2_approx(m - top);
-            factor[r][i] = f;
-            norm = fmaf(l, f, norm);
-          }
-#pragma unroll
-          for (int off = 16; off >= 1; off >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, off);
-        }
-        const float inv = norm == 0.f ? 0.f : 1.f / norm;  // a row that sees nothing: zeros
-        __syncwarp();
-        for (int i = lane; i < slots; i += 32) factor[r][i] *= inv;
-        if (lane == 0 && tile * R + r < total) row_lse[tile * R + r] = norm == 0.f ? INFINITY : top + log2f(norm);
-      }
-      __syncthreads();
-    }
-    if (joins && (slots > 1 || none)) {
-      // 64 times four numbers, four threads for each: every fourth partial result
-      const int i = (blockIdx.x % kParts) * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6, r = i / (D / 4), row = tile * R + r;
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (!none) {
-#pragma unroll 4
-        for (int k = part; k < slots; k += 4) {
-          const float f = factor[r][k];
-          if (f == 0.f) continue;
-          const float4 x = *reinterpret_cast<const float4 *>(sp.partial + static_cast<size_t>(slot0 + k) * R * D + 4 * i);
-          sum.x = fmaf(x.x, f, sum.x);
-          sum.y = fmaf(x.y, f, sum.y);
-          sum.z = fmaf(x.z, f, sum.z);
-          sum.w = fmaf(x.w, f, sum.w);
-        }
-      }
-      quarter[part][threadIdx.x & 63] = sum;
-      __syncthreads();
-      if (part == 0 && row < total) {
-#pragma unroll
-        for (int k = 1; k < 4; ++k) {
-          const float4 x = quarter[k][threadIdx.x];
-          sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
-        }
-        const int q = row / p.group;
-        const size_t at = ((static_cast<size_t>(b) * p.seq + q) * p.heads + static_cast<size_t>(h) * p.group + (row - q * p.group)) * D + (i % (D / 4)) * 4;
-        uint2 w;
-        w.x = kv4_bits<T>(sum.x) | static_cast<uint32_t>(kv4_bits<T>(sum.y)) << 16;
-        w.y = kv4_bits<T>(sum.z) | static_cast<uint32_t>(kv4_bits<T>(sum.w)) << 16;
-        *reinterpret_cast<uint2 *>(p.out + at) = w;
-      }
-    }
-  }
-  if (!weighs) return;
+  __syncthreads();
   // weights[j] += sum over all rows of exp2(score - lse): a warp per 16 entries goes over the rows in their order
   const int j0 = blockIdx.x * 128 + warp * 16, g = lane >> 2, t = lane & 3;
   if (j0 >= length) return;
@@ -637,9 +638,9 @@ template <typename T, int D, int NT> __global__ void __launch_bounds__(kStepWarp
 namespace {
 
 struct StepPlan {
-  int rows, tiles, segments, blocks;  // rows of a tile; blocks of a segment at most
+  int rows, tiles, segments;  // rows of a tile
   bool whole;
-  int64_t slots, ml_bytes, partial_bytes;
+  int64_t slots, pieces_bytes, ml_bytes, partial_bytes;
 };
 
 StepPlan step_plan(const Kv4Cache &c, int seq, int group, int window, int sinks, bool weights) {
@@ -649,9 +650,11 @@ StepPlan step_plan(const Kv4Cache &c, int seq, int group, int window, int sinks,
   s.segments = c.batch * c.kv_heads * s.tiles;
   const int all = (c.capacity + kStepBlock - 1) / kStepBlock;
   // a window of w entries and the s rows' own lie in at most (w + s - 2) / 32 + 2 blocks
-  s.blocks = window > 0 ? std::min(all, (window + seq - 2) / kStepBlock + 2 + (sinks + kStepBlock - 1) / kStepBlock) : all;
-  s.whole = s.blocks <= kStepWhole || c.batch > kStepSequences || s.segments >= 4 * kStepCtas;
+  const int blocks = window > 0 ? std::min(all, (window + seq - 2) / kStepBlock + 2 + (sinks + kStepBlock - 1) / kStepBlock) : all;
+  s.whole = blocks <= kStepWhole || s.segments >= 4 * kStepCtas;
+  // pieces of all segments: blocks / share and one for what is left over, each; shares are at least all blocks / kStepCtas
   s.slots = s.whole ? s.segments : s.segments + kStepCtas;
+  s.pieces_bytes = s.whole ? 0 : (s.segments * 8 + 15) / 16 * 16;
   s.ml_bytes = s.whole && !weights ? 0 : s.slots * 2 * s.rows * 4;
   s.partial_bytes = s.whole ? 0 : s.slots * s.rows * c.dim * 4;
   return s;
@@ -677,13 +680,11 @@ template <typename T, int D, int NT> int kv4_step(const Kv4StepParams &p, const 
   static SharedMemoryOptIn opt_in;
   int st = opt_in.ensure(kv4_step_kernel<T, D, NT>, smem);
   if (st != MG_OK) return st;
-  const long long most = static_cast<long long>(plan.segments) * plan.blocks;
-  const int ctas = plan.whole ? plan.segments : static_cast<int>(std::min<long long>(kStepCtas, (most + kStepLeast - 1) / kStepLeast));
-  st = launch_step(kv4_step_kernel<T, D, NT>, dim3(ctas), smem, stream, pdl, p);
+  st = launch_step(kv4_step_kernel<T, D, NT>, dim3(static_cast<unsigned>(plan.slots)), smem, stream, pdl, p);
   if (st != MG_OK || (plan.whole && p.a.weights == nullptr)) return st;
   const int parts = plan.whole ? 1 : 8 * NT * D / 256 * plan.tiles;
   const int entries = p.a.weights != nullptr ? (p.a.cache.capacity + 127) / 128 : 1;
-  return launch_step(kv4_finish_kernel<T, D, NT>, dim3(std::max(parts, entries), p.a.cache.batch * p.a.cache.kv_heads), 0, stream, true, p, ctas);
+  return launch_step(kv4_finish_kernel<T, D, NT>, dim3(std::max(parts, entries), p.a.cache.batch * p.a.cache.kv_heads), 0, stream, true, p);
 }
 
 template <typename T, int D> int kv4_step_rows(const Kv4StepParams &p, const StepPlan &plan, cudaStream_t stream, bool pdl) {
@@ -694,8 +695,9 @@ int kv4_few_rows(const Kv4AttentionParams &a, void *workspace, bool bf16, bool p
   const StepPlan plan = step_plan(a.cache, a.seq, a.group, a.window, a.sinks, a.weights != nullptr);
   Kv4StepParams p = {};
   p.a = a;
-  p.ml = static_cast<float *>(workspace);
-  p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + plan.ml_bytes);
+  p.pieces = static_cast<int2 *>(workspace);
+  p.ml = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + plan.pieces_bytes);
+  p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + plan.pieces_bytes + plan.ml_bytes);
   p.tiles = plan.tiles;
   p.whole = plan.whole;
   if (a.cache.dim == 64) return bf16 ? kv4_step_rows<__nv_bfloat16, 64>(p, plan, stream, pdl) : kv4_step_rows<__half, 64>(p, plan, stream, pdl);
@@ -723,7 +725,7 @@ int64_t matgptq_b200_attention_kv4_workspace_bytes(const matgptq_b200_kv4_cache 
   const mg::Kv4Cache c = mg::kv4_cache(cache);
   const mg::StepPlan plan = mg::step_plan(c, static_cast<int>(seq), static_cast<int>(rows / seq), mg::kv4_window(c, window), mg::kv4_sinks(c, sinks),
                                           with_weights != 0);
-  return plan.ml_bytes + plan.partial_bytes;
+  return plan.pieces_bytes + plan.ml_bytes + plan.partial_bytes;
 }
 
 int matgptq_b200_attention_kv4(const matgptq_b200_kv4_cache *cache, const void *q, int64_t seq, int64_t n_heads, const int32_t *lengths,
