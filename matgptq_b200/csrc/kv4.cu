@@ -34,6 +34,14 @@ template <typename T> __device__ __forceinline__ T turned(float x, float a, floa
   return from_f<T>(static_cast<float>(static_cast<double>(x) * a + static_cast<double>(y) * b));
 }
 
+// rint(x / scale) for the fp32 quotient rounded once, 0 <= x / scale < 32: the approximate quotient is off by less than 2^-17, and only
+// a quotient that near a border is divided for.
+__device__ __forceinline__ float nearest_code(float x, float scale, float per) {
+  const float q = x * per, code = rintf(q);
+  return fabsf(q - code) < 0.5f - 0x1p-16f ? code : rintf(__fdiv_rn(x, scale));
+}
+
+// blockIdx.x over the 16-byte pieces of a token's row, blockIdx.y walks the tokens
 template <typename T>
 __global__ void __launch_bounds__(256) append_kv4_kernel(const T *__restrict__ qkv, const long long *__restrict__ positions,
                                                          long long position_stride, const float *__restrict__ cos_t,
@@ -41,86 +49,87 @@ __global__ void __launch_bounds__(256) append_kv4_kernel(const T *__restrict__ q
                                                          const int *__restrict__ lengths, T *__restrict__ q_out, Kv4Cache cache, int seq,
                                                          int heads) {
   pdl_prologue();
-  const int lanes = cache.dim >> 3;  // of a row: 8 or 16
+  const int lanes = cache.dim >> 3, shift = cache.dim == 128 ? 4 : 3;  // of a row: 8 or 16
   const int all = heads + 2 * cache.kv_heads;
-  const long long rows = static_cast<long long>(cache.batch) * seq * all;
-  const long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) / lanes;
-  const int c0 = (threadIdx.x & (lanes - 1)) * 8;
-  const bool live = row < rows;
-  const long long safe = live ? row : 0;
-  const int head = static_cast<int>(safe % all);
-  const long long token = safe / all;
-  const int b = static_cast<int>(token / seq), s = static_cast<int>(token - static_cast<long long>(b) * seq);
-  const long long slot = static_cast<long long>(lengths[b]) - seq + s;
-  const bool padding = slot < 0;
-  bool outside = !padding && slot >= cache.capacity;
+  const int at = blockIdx.x * 256 + threadIdx.x, c0 = (at & (lanes - 1)) * 8;
+  const bool live = (at >> shift) < all;
+  const int head = live ? at >> shift : 0;
+  for (int row = blockIdx.y; row < cache.batch * seq; row += gridDim.y) {
+    const long long token = row;
+    const int b = row / seq, s = row - b * seq;
+    const long long slot = static_cast<long long>(lengths[b]) - seq + s;
+    const bool padding = slot < 0;
+    bool outside = !padding && slot >= cache.capacity;
 
-  uint4 raw = make_uint4(0, 0, 0, 0);
-  if (live && !padding) raw = *reinterpret_cast<const uint4 *>(qkv + (token * all + head) * cache.dim + c0);
-  T *e = reinterpret_cast<T *>(&raw);
-  if (head < heads + cache.kv_heads && live && !padding) {
-    const long long pos = positions[b * position_stride + s];
-    if (pos < 0 || pos >= n_positions) {
-      outside = true;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (live && !padding) raw = *reinterpret_cast<const uint4 *>(qkv + (token * all + head) * cache.dim + c0);
+    T *e = reinterpret_cast<T *>(&raw);
+    if (head < heads + cache.kv_heads && live && !padding) {
+      const long long pos = positions[b * position_stride + s];
+      if (pos < 0 || pos >= n_positions) {
+        outside = true;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = from_f<T>(NAN);
-    } else {
-      const float4 cs = *reinterpret_cast<const float4 *>(cos_t + pos * (cache.dim >> 1) + (c0 >> 1));
-      const float4 sn = *reinterpret_cast<const float4 *>(sin_t + pos * (cache.dim >> 1) + (c0 >> 1));
-      const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
+        for (int i = 0; i < 8; ++i) e[i] = from_f<T>(NAN);
+      } else {
+        const float4 cs = *reinterpret_cast<const float4 *>(cos_t + pos * (cache.dim >> 1) + (c0 >> 1));
+        const float4 sn = *reinterpret_cast<const float4 *>(sin_t + pos * (cache.dim >> 1) + (c0 >> 1));
+        const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const float x = to_f(e[2 * p]), y = to_f(e[2 * p + 1]);
-        e[2 * p] = turned<T>(x, cv[p], y, -sv[p]);
-        e[2 * p + 1] = turned<T>(y, cv[p], x, sv[p]);
+        for (int p = 0; p < 4; ++p) {
+          const float x = to_f(e[2 * p]), y = to_f(e[2 * p + 1]);
+          e[2 * p] = turned<T>(x, cv[p], y, -sv[p]);
+          e[2 * p + 1] = turned<T>(y, cv[p], x, sv[p]);
+        }
       }
     }
-  }
-  if (outside) report_status(kStatusCacheRange);
+    if (outside) report_status(kStatusCacheRange);
 
-  float x[8], low = FLT_MAX, high = -FLT_MAX;
-  bool odd = false;
+    float x[8], low = FLT_MAX, high = -FLT_MAX;
+    bool odd = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[i] = to_f(e[i]);
-    odd |= !(fabsf(x[i]) <= FLT_MAX);
-    low = fminf(low, x[i]);
-    high = fmaxf(high, x[i]);
-  }
-  if (odd) high = INFINITY;
-  for (int off = lanes >> 1; off >= 1; off >>= 1) {  // whole warps come here: rows of one warp differ, lanes of one row do not
-    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, off));
-    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, off));
-  }
-  if (!live) return;
-  if (head < heads) {
-    *reinterpret_cast<uint4 *>(q_out + (token * heads + head) * cache.dim + c0) = raw;
-    return;
-  }
-  if (padding || slot >= cache.capacity) return;
-  const float range = __fsub_rn(high, low);
-  const T scale16 = from_f<T>(range <= FLT_MAX ? __fdiv_rn(range, 15.f) : NAN);
-  const float scale = to_f(scale16);
-  uint32_t word = 0;
+    for (int i = 0; i < 8; ++i) {
+      x[i] = to_f(e[i]);
+      odd |= !(fabsf(x[i]) <= FLT_MAX);
+      low = fminf(low, x[i]);
+      high = fmaxf(high, x[i]);
+    }
+    if (odd) high = INFINITY;
+    for (int off = lanes >> 1; off >= 1; off >>= 1) {  // whole warps come here: rows of one warp differ, lanes of one row do not
+      low = fminf(low, __shfl_xor_sync(0xffffffffu, low, off));
+      high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, off));
+    }
+    if (!live) continue;
+    if (head < heads) {
+      *reinterpret_cast<uint4 *>(q_out + (token * heads + head) * cache.dim + c0) = raw;
+      continue;
+    }
+    if (padding || slot >= cache.capacity) continue;
+    const float range = __fsub_rn(high, low);
+    const T scale16 = from_f<T>(range <= FLT_MAX ? __fdiv_rn(range, 15.f) : NAN);
+    const float scale = to_f(scale16);
+    float per;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(per) : "f"(scale));
+    uint32_t word = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float c = scale > 0.f ? fminf(15.f, rintf(__fdiv_rn(__fsub_rn(x[i], low), scale))) : 0.f;
-    word |= static_cast<uint32_t>(c) << (4 * i);
-  }
-  const bool is_v = head >= heads + cache.kv_heads;
-  const size_t entry = (static_cast<size_t>(b) * cache.kv_heads + (head - heads - (is_v ? cache.kv_heads : 0))) * cache.capacity + slot;
-  if (is_v) {
-    uint16_t *units = reinterpret_cast<uint16_t *>(cache.v + (entry >> 1) * cache.dim) + (entry & 1) + (c0 >> 1);
-    units[0] = static_cast<uint16_t>(word);
-    units[2] = static_cast<uint16_t>(word >> 16);
-  } else {
-    *reinterpret_cast<uint32_t *>(cache.k + entry * (cache.dim >> 1) + (c0 >> 1)) = word;
-  }
-  if (c0 == 0) {
-    const T low16 = from_f<T>(low);
-    const uint32_t both = static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(&scale16)) |
-                          static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(&low16)) << 16;
-    *reinterpret_cast<uint32_t *>(cache.params + entry * 4 + (is_v ? 2 : 0)) = both;
+    for (int i = 0; i < 8; ++i) {
+      const float c = scale > 0.f ? fminf(15.f, nearest_code(__fsub_rn(x[i], low), scale, per)) : 0.f;
+      word |= static_cast<uint32_t>(c) << (4 * i);
+    }
+    const bool is_v = head >= heads + cache.kv_heads;
+    const size_t entry = (static_cast<size_t>(b) * cache.kv_heads + (head - heads - (is_v ? cache.kv_heads : 0))) * cache.capacity + slot;
+    if (is_v) {
+      uint16_t *units = reinterpret_cast<uint16_t *>(cache.v + (entry >> 1) * cache.dim) + (entry & 1) + (c0 >> 1);
+      units[0] = static_cast<uint16_t>(word);
+      units[2] = static_cast<uint16_t>(word >> 16);
+    } else {
+      *reinterpret_cast<uint32_t *>(cache.k + entry * (cache.dim >> 1) + (c0 >> 1)) = word;
+    }
+    if (c0 == 0) {
+      const T low16 = from_f<T>(low);
+      const uint32_t both = static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(&scale16)) |
+                            static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(&low16)) << 16;
+      *reinterpret_cast<uint32_t *>(cache.params + entry * 4 + (is_v ? 2 : 0)) = both;
+    }
   }
 }
 
@@ -129,36 +138,44 @@ __global__ void __launch_bounds__(256) append_kv4_kernel(const T *__restrict__ q
 // The last `count` entries of every sequence as dense rows of the model's type, zeros in front where a sequence has fewer: eight
 // channels of one entry's K and V a thread.  One multiply-add in fp32 (the product is exact: 4 bits x 11) and one rounding.
 // Bound by memory: 4 d bytes written for d + 8 read.
+// A thread takes eight channels of a V pair's two entries; blockIdx.x over these, blockIdx.y over sequences and heads.
+template <typename T> __device__ __forceinline__ uint4 dense_row(uint32_t word, float scale, float low) {
+  uint4 out;
+  T *e = reinterpret_cast<T *>(&out);
+#pragma unroll
+  for (int c = 0; c < 8; ++c) e[c] = from_f<T>(__fmaf_rn(scale, static_cast<float>((word >> (4 * c)) & 15u), low));
+  return out;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) dequantize_kv4_kernel(Kv4Cache cache, const int *__restrict__ lengths, int count, T *__restrict__ k_out,
                                                              T *__restrict__ v_out) {
   pdl_prologue();
-  const int lanes = cache.dim >> 3;
-  const long long rows = static_cast<long long>(cache.batch) * cache.kv_heads * count;
-  const long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) / lanes;
-  if (row >= rows) return;
+  const int lanes = cache.dim >> 3, shift = cache.dim == 128 ? 4 : 3;
+  const int bh = blockIdx.y, b = bh / cache.kv_heads;
+  const int before = kv4_length(lengths, b, cache.capacity) - count;  // entry of row 0; negative: rows of zeros come first
   const int c0 = (threadIdx.x & (lanes - 1)) * 8;
-  const long long bh = row / count;
-  const int i = static_cast<int>(row - bh * count), b = static_cast<int>(bh / cache.kv_heads);
-  const int slot = kv4_length(lengths, b, cache.capacity) - count + i;
-  uint4 k4 = make_uint4(0, 0, 0, 0), v4 = k4;
-  if (slot >= 0) {
-    const size_t entry = static_cast<size_t>(bh) * cache.capacity + slot;
-    const uint32_t kw = *reinterpret_cast<const uint32_t *>(cache.k + entry * (cache.dim >> 1) + (c0 >> 1));
-    const uint16_t *units = reinterpret_cast<const uint16_t *>(cache.v + (entry >> 1) * cache.dim) + (entry & 1) + (c0 >> 1);
-    const uint32_t vw = units[0] | static_cast<uint32_t>(units[2]) << 16;
-    const uint2 p = *reinterpret_cast<const uint2 *>(cache.params + entry * 4);
-    const float ks = kv4_to_f<T>(static_cast<uint16_t>(p.x)), kl = kv4_to_f<T>(static_cast<uint16_t>(p.x >> 16));
-    const float vs = kv4_to_f<T>(static_cast<uint16_t>(p.y)), vl = kv4_to_f<T>(static_cast<uint16_t>(p.y >> 16));
-    T *ke = reinterpret_cast<T *>(&k4), *ve = reinterpret_cast<T *>(&v4);
+  const int first = (before & ~1) + 2 * static_cast<int>((static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> shift);  // entry, even
+  const size_t head = static_cast<size_t>(bh) * cache.capacity;
+  uint32_t k[2] = {0, 0};
+  uint2 v = make_uint2(0, 0), p[2] = {make_uint2(0, 0), make_uint2(0, 0)};
+  if (first >= 0 && first < cache.capacity) {
+    v = *reinterpret_cast<const uint2 *>(cache.v + ((head + first) >> 1) * cache.dim + c0);
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      ke[c] = from_f<T>(__fmaf_rn(ks, static_cast<float>((kw >> (4 * c)) & 15u), kl));
-      ve[c] = from_f<T>(__fmaf_rn(vs, static_cast<float>((vw >> (4 * c)) & 15u), vl));
+    for (int i = 0; i < 2; ++i) {
+      k[i] = *reinterpret_cast<const uint32_t *>(cache.k + (head + first + i) * (cache.dim >> 1) + (c0 >> 1));
+      p[i] = *reinterpret_cast<const uint2 *>(cache.params + (head + first + i) * 4);
     }
   }
-  *reinterpret_cast<uint4 *>(k_out + row * cache.dim + c0) = k4;
-  *reinterpret_cast<uint4 *>(v_out + row * cache.dim + c0) = v4;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = first + i - before;
+    if (row < 0 || row >= count) continue;
+    const size_t at = (static_cast<size_t>(bh) * count + row) * cache.dim + c0;
+    *reinterpret_cast<uint4 *>(k_out + at) = dense_row<T>(k[i], kv4_to_f<T>(static_cast<uint16_t>(p[i].x)), kv4_to_f<T>(static_cast<uint16_t>(p[i].x >> 16)));
+    *reinterpret_cast<uint4 *>(v_out + at) = dense_row<T>(__byte_perm(v.x, v.y, i ? 0x7632 : 0x5410), kv4_to_f<T>(static_cast<uint16_t>(p[i].y)),
+                                                          kv4_to_f<T>(static_cast<uint16_t>(p[i].y >> 16)));
+  }
 }
 
 // ---- thinning out -----------------------------------------------------------------------------------------------------
@@ -167,7 +184,7 @@ __global__ void __launch_bounds__(256) dequantize_kv4_kernel(Kv4Cache cache, con
 // ones with the largest weights, ties to the lowest index, all in their order.  evict_kv4_select_kernel, a CTA per sequence and
 // head, finds the smallest weight that stays by four passes over the weights' bits (8 at a time, from the top), writes the indices
 // that stay and moves the weights; evict_kv4_move_kernel moves codes and scales.
-constexpr int kEvictThreads = 1024;
+constexpr int kEvictThreads = 1024, kEvictCached = 16;
 
 // larger weights have larger keys; a NaN counts as the largest weight, -0 as 0
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -196,19 +213,47 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_kv4_select_kernel(floa
   __shared__ uint32_t s_prefix;
   __shared__ int s_want;
   uint32_t prefix = 0;  // the top bits of the smallest key that stays
+  // the first keys of every thread stay in registers over the passes
+  uint32_t cached[kEvictCached];
+#pragma unroll
+  for (int k = 0; k < kEvictCached; ++k) {
+    const int j = first + tid + k * kEvictThreads;
+    if (j < last) cached[k] = weight_key(w[j]);
+  }
   for (int shift = 24; shift >= 0; shift -= 8) {
     for (int i = tid; i < 256; i += kEvictThreads) hist[i] = 0;
     __syncthreads();
-    for (int j = first + tid; j < last; j += kEvictThreads) {
-      const uint32_t key = weight_key(w[j]);
+    const auto count = [&](uint32_t key) {
       if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1);
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < kEvictCached; ++k)
+      if (first + tid + k * kEvictThreads < last) count(cached[k]);
+    for (int j = first + tid + kEvictCached * kEvictThreads; j < last; j += kEvictThreads) count(weight_key(w[j]));
     __syncthreads();
-    if (tid == 0) {
-      int above = 0, digit = 255;
-      for (; digit > 0 && above + hist[digit] < want; --digit) above += hist[digit];
-      s_prefix = prefix | static_cast<uint32_t>(digit) << shift;
-      s_want = want - above;
+    if (warp == 0) {  // lane l: the digits 255 - 8 l down to 248 - 8 l
+      int mine[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += mine[i] = hist[255 - 8 * lane - i];
+      int above = sum;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, above, off);
+        if (lane >= off) above += x;
+      }
+      // the first digit at which `want` is reached, the lowest one where it never is
+      const unsigned reached = __ballot_sync(0xffffffffu, above >= want);
+      if (lane == (reached ? __ffs(reached) - 1 : 31)) {
+        above -= sum;
+        int digit = -1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (digit < 0 && (i == 7 || above + mine[i] >= want)) digit = 255 - 8 * lane - i;
+          if (digit < 0) above += mine[i];
+        }
+        s_prefix = prefix | static_cast<uint32_t>(digit) << shift;
+        s_want = want - above;
+      }
     }
     __syncthreads();
     prefix = s_prefix;
@@ -257,8 +302,9 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_kv4_select_kernel(floa
 }
 
 // A CTA moves one column slice (32 bytes of the K rows, 32 bytes of the V pairs, or the params) of one sequence and head: entry
-// i comes from kept[i] >= i, and what a step reads is read before the step writes, so nothing is overwritten that is still needed.
-constexpr int kMoveThreads = 512;
+// i comes from kept[i] >= i, and what a step reads is read before the step writes, so nothing is overwritten that is still needed.  A
+// step is as many entries as its threads can hold, since it costs a round trip to memory.
+constexpr int kMoveThreads = 512, kMoveEach = 8;
 
 __global__ void __launch_bounds__(kMoveThreads) evict_kv4_move_kernel(Kv4Cache cache, const int *__restrict__ kept, int keep) {
   pdl_prologue();
@@ -271,45 +317,75 @@ __global__ void __launch_bounds__(kMoveThreads) evict_kv4_move_kernel(Kv4Cache c
   if (slice < k_slices) {
     const int row_bytes = cache.dim >> 1;
     uint8_t *base = cache.k + first * row_bytes + slice * 32 + (tid & 1) * 16;
-    for (int i0 = 0; i0 < keep; i0 += kMoveThreads / 2) {
-      const int i = i0 + (tid >> 1);
-      const int from = i < keep ? src[i] : i;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (from != i) v = *reinterpret_cast<const uint4 *>(base + static_cast<size_t>(from) * row_bytes);
+    for (int i0 = tid >> 1; i0 - (tid >> 1) < keep; i0 += kMoveEach * kMoveThreads / 2) {
+      uint4 v[kMoveEach];
+      int from[kMoveEach];
+#pragma unroll
+      for (int k = 0; k < kMoveEach; ++k) {
+        const int i = i0 + k * kMoveThreads / 2;
+        from[k] = i < keep ? src[i] : i;
+      }
+#pragma unroll
+      for (int k = 0; k < kMoveEach; ++k)
+        if (from[k] != i0 + k * kMoveThreads / 2) v[k] = *reinterpret_cast<const uint4 *>(base + static_cast<size_t>(from[k]) * row_bytes);
       __syncthreads();
-      if (from != i) *reinterpret_cast<uint4 *>(base + static_cast<size_t>(i) * row_bytes) = v;
+#pragma unroll
+      for (int k = 0; k < kMoveEach; ++k) {
+        const int i = i0 + k * kMoveThreads / 2;
+        if (from[k] != i) *reinterpret_cast<uint4 *>(base + static_cast<size_t>(i) * row_bytes) = v[k];
+      }
     }
   } else if (slice < k_slices + v_slices) {
     // a pair at a time: each word takes the half of one entry's unit and the half of another's
     uint8_t *base = cache.v + (first >> 1) * cache.dim + (slice - k_slices) * 32 + (tid & 1) * 16;
     const int pairs = (keep + 1) >> 1;
-    for (int p0 = 0; p0 < pairs; p0 += kMoveThreads / 2) {
-      const int p = p0 + (tid >> 1);
-      const bool live = p < pairs;
-      const int a = live ? src[2 * p] : 0;
-      const int c = live && 2 * p + 1 < keep ? src[2 * p + 1] : 2 * p + 1;  // behind the last entry: as it was
-      const bool moves = live && (a != 2 * p || c != 2 * p + 1);
-      uint32_t out[4] = {0, 0, 0, 0};
-      if (moves) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(base + static_cast<size_t>(a >> 1) * cache.dim);
-        const uint4 y = *reinterpret_cast<const uint4 *>(base + static_cast<size_t>(c >> 1) * cache.dim);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-        const unsigned pick = (a & 1 ? 0x32u : 0x10u) | ((c & 1 ? 0x76u : 0x54u) << 8);
+    constexpr int kEach = kMoveEach / 2;
+    for (int p0 = tid >> 1; p0 - (tid >> 1) < pairs; p0 += kEach * kMoveThreads / 2) {
+      int a[kEach], c[kEach];
+      uint4 x[kEach], y[kEach];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) out[i] = __byte_perm(xs[i], ys[i], pick);
+      for (int k = 0; k < kEach; ++k) {
+        const int p = p0 + k * kMoveThreads / 2;
+        a[k] = p < pairs ? src[2 * p] : 2 * p;
+        c[k] = 2 * p + 1 < keep ? src[2 * p + 1] : 2 * p + 1;  // behind the last entry: as it was
+      }
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) {
+        const int p = p0 + k * kMoveThreads / 2;
+        if (a[k] != 2 * p || c[k] != 2 * p + 1) {
+          x[k] = *reinterpret_cast<const uint4 *>(base + static_cast<size_t>(a[k] >> 1) * cache.dim);
+          y[k] = *reinterpret_cast<const uint4 *>(base + static_cast<size_t>(c[k] >> 1) * cache.dim);
+        }
       }
       __syncthreads();
-      if (moves) *reinterpret_cast<uint4 *>(base + static_cast<size_t>(p) * cache.dim) = make_uint4(out[0], out[1], out[2], out[3]);
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) {
+        const int p = p0 + k * kMoveThreads / 2;
+        if (a[k] != 2 * p || c[k] != 2 * p + 1) {
+          const unsigned pick = (a[k] & 1 ? 0x32u : 0x10u) | ((c[k] & 1 ? 0x76u : 0x54u) << 8);
+          *reinterpret_cast<uint4 *>(base + static_cast<size_t>(p) * cache.dim) =
+              make_uint4(__byte_perm(x[k].x, y[k].x, pick), __byte_perm(x[k].y, y[k].y, pick), __byte_perm(x[k].z, y[k].z, pick),
+                         __byte_perm(x[k].w, y[k].w, pick));
+        }
+      }
     }
   } else {
     uint2 *base = reinterpret_cast<uint2 *>(cache.params) + first;
-    for (int i0 = 0; i0 < keep; i0 += kMoveThreads) {
-      const int i = i0 + tid;
-      const int from = i < keep ? src[i] : i;
-      uint2 v = make_uint2(0, 0);
-      if (from != i) v = base[from];
+    for (int i0 = tid; i0 - tid < keep; i0 += kMoveEach * kMoveThreads) {
+      int from[kMoveEach];
+      uint2 v[kMoveEach];
+#pragma unroll
+      for (int k = 0; k < kMoveEach; ++k) {
+        const int i = i0 + k * kMoveThreads;
+        from[k] = i < keep ? src[i] : i;
+      }
+#pragma unroll
+      for (int k = 0; k < kMoveEach; ++k)
+        if (from[k] != i0 + k * kMoveThreads) v[k] = base[from[k]];
       __syncthreads();
-      if (from != i) base[i] = v;
+#pragma unroll
+      for (int k = 0; k < kMoveEach; ++k)
+        if (from[k] != i0 + k * kMoveThreads) base[i0 + k * kMoveThreads] = v[k];
     }
   }
 }
@@ -360,12 +436,14 @@ int matgptq_b200_append_kv4(const matgptq_b200_kv4_cache *cache, const void *qkv
   if (seq < 0 || seq > (1 << 30) || n_heads <= 0 || n_heads > (1 << 20) || n_positions <= 0 || position_stride < 0) return MG_ERR_BAD_ARG;
   if (misaligned({qkv, cos_table, sin_table, q_out})) return MG_ERR_ALIGNMENT;
   const Kv4Cache c = mg::kv4_cache(cache);
-  const long long threads = cache->batch * seq * (n_heads + 2 * cache->n_kv_heads) * (c.dim / 8);
-  if (threads == 0) return MG_OK;
-  if ((threads + 255) / 256 > INT32_MAX) return MG_ERR_UNSUPPORTED;
+  const long long tokens = cache->batch * seq;
+  if (tokens == 0) return MG_OK;
+  if (tokens > INT32_MAX) return MG_ERR_UNSUPPORTED;
+  const long long x = ((n_heads + 2 * cache->n_kv_heads) * (c.dim / 8) + 255) / 256, most = (148LL * 64 + x - 1) / x;
+  const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(tokens < most ? tokens : most));
   const auto go = [&](auto tag) {
     using T = decltype(tag);
-    return mg::launch_helper(mg::append_kv4_kernel<T>, dim3(static_cast<unsigned>((threads + 255) / 256)), 256, static_cast<cudaStream_t>(stream),
+    return mg::launch_helper(mg::append_kv4_kernel<T>, grid, 256, static_cast<cudaStream_t>(stream),
                              (flags & MATGPTQ_B200_FLAG_PDL) != 0, static_cast<const T *>(qkv), reinterpret_cast<const long long *>(positions),
                              static_cast<long long>(position_stride), cos_table, sin_table, static_cast<long long>(n_positions),
                              static_cast<const int *>(lengths), static_cast<T *>(q_out), c, static_cast<int>(seq), static_cast<int>(n_heads));
@@ -380,12 +458,12 @@ int matgptq_b200_dequantize_kv4(const matgptq_b200_kv4_cache *cache, const int32
   if (!lengths || count < 0 || count > (1 << 30) || (count > 0 && (!k_out || !v_out))) return MG_ERR_BAD_ARG;
   if (misaligned({k_out, v_out})) return MG_ERR_ALIGNMENT;
   const Kv4Cache c = mg::kv4_cache(cache);
-  const long long threads = cache->batch * cache->n_kv_heads * count * (c.dim / 8);
-  if (threads == 0) return MG_OK;
-  if ((threads + 255) / 256 > INT32_MAX) return MG_ERR_UNSUPPORTED;
+  if (cache->batch == 0 || count == 0) return MG_OK;
+  // the pairs that `count` entries lie in, one more than half where they begin in the middle of one
+  const dim3 grid(static_cast<unsigned>(((count / 2 + 1) * (c.dim / 8) + 255) / 256), static_cast<unsigned>(cache->batch * cache->n_kv_heads));
   const auto go = [&](auto tag) {
     using T = decltype(tag);
-    return mg::launch_helper(mg::dequantize_kv4_kernel<T>, dim3(static_cast<unsigned>((threads + 255) / 256)), 256,
+    return mg::launch_helper(mg::dequantize_kv4_kernel<T>, grid, 256,
                              static_cast<cudaStream_t>(stream), (flags & MATGPTQ_B200_FLAG_PDL) != 0, c, static_cast<const int *>(lengths),
                              static_cast<int>(count), static_cast<T *>(k_out), static_cast<T *>(v_out));
   };

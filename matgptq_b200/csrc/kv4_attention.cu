@@ -512,7 +512,10 @@ __global__ void __launch_bounds__(kStepWarps * 32, NT == 1 ? 2 : 1) kv4_step_ker
 }
 
 // What is left once every piece has been seen: joins the partial results of segments that were cut, and adds up the weights.
-// blockIdx.y: sequence and head; blockIdx.x: a part of a tile's results (256 numbers), and 128 entries whose weights are due.
+// blockIdx.y: sequence and head; blockIdx.x: a part of a tile's results (256 numbers), and kFinishEntries entries whose weights are due.
+// Every step is a round trip to memory, so what does not hang on another is asked for at once.
+constexpr int kFinishEach = 4, kFinishEntries = kStepWarps * 16 * kFinishEach;
+
 template <typename T, int D, int NT> __global__ void __launch_bounds__(kStepWarps * 32) kv4_finish_kernel(const Kv4StepParams sp) {
   pdl_prologue();
   const Kv4AttentionParams &p = sp.a;
@@ -527,6 +530,21 @@ template <typename T, int D, int NT> __global__ void __launch_bounds__(kStepWarp
   int2 pieces = make_int2(0, 1);
   if (joins) pieces = sp.pieces[(b * sp.tiles + tile) * kv + h];
   const int length = kv4_length(p.lengths, b, p.cache.capacity);
+  const size_t first = static_cast<size_t>(blockIdx.y) * p.cache.capacity;
+  const int g = lane >> 2, t = lane & 3;
+  const bool weighs = p.weights != nullptr && part * kFinishEntries < length;
+  const auto entry = [&](int u) { return part * kFinishEntries + (u * kStepWarps + warp) * 16; };  // the first of 16 that this warp weighs
+  uint32_t k0[kFinishEach][D / 32], k1[kFinishEach][D / 32], kp[kFinishEach][2];
+  if (weighs) {
+#pragma unroll
+    for (int u = 0; u < kFinishEach; ++u) {
+      if (entry(u) >= length) continue;
+      kv4_load_words(k0[u], p.cache.k + (first + entry(u) + g) * (D / 2) + t * (D / 8));
+      kv4_load_words(k1[u], p.cache.k + (first + entry(u) + 8 + g) * (D / 2) + t * (D / 8));
+#pragma unroll
+      for (int e = 0; e < 2; ++e) kp[u][e] = *reinterpret_cast<const uint32_t *>(p.cache.params + (first + entry(u) + 8 * e + g) * 4);
+    }
+  }
   if (joins) {
     // a sequence without entries has no piece: its rows have not been written
     if (step_range<R>(p, length, tile).blocks == 0) pieces.y = 0;
@@ -581,7 +599,7 @@ template <typename T, int D, int NT> __global__ void __launch_bounds__(kStepWarp
       }
     }
   }
-  if (p.weights == nullptr || part * 128 >= length) return;
+  if (!weighs) return;
   // the rows' sums: a warp per row
   for (int row = warp; row < total; row += kStepWarps) {
     const int segment = (b * sp.tiles + row / R) * kv + h, r = row % R;
@@ -605,34 +623,35 @@ template <typename T, int D, int NT> __global__ void __launch_bounds__(kStepWarp
     if (lane == 0) row_lse[row] = l == 0.f ? INFINITY : top + log2f(l);
   }
   __syncthreads();
-  // weights[j] += sum over all rows of exp2(score - lse): a warp per 16 entries goes over the rows in their order
-  const int j0 = blockIdx.x * 128 + warp * 16, g = lane >> 2, t = lane & 3;
-  if (j0 >= length) return;
-  const size_t first = static_cast<size_t>(blockIdx.y) * p.cache.capacity;
-  uint32_t k0[D / 32], k1[D / 32], kp[2];
-  kv4_load_words(k0, p.cache.k + (first + j0 + g) * (D / 2) + t * (D / 8));
-  kv4_load_words(k1, p.cache.k + (first + j0 + 8 + g) * (D / 2) + t * (D / 8));
+  // weights[j] += sum over all rows of exp2(score - lse), in the order of the rows
+  float sum[kFinishEach][2];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) kp[e] = *reinterpret_cast<const uint32_t *>(p.cache.params + (first + j0 + 8 * e + g) * 4);
-  float sum[2] = {0.f, 0.f};
+  for (int u = 0; u < kFinishEach; ++u) sum[u][0] = sum[u][1] = 0.f;
   for (int r0 = 0; r0 < total; r0 += 8) {
     Kv4Rows<D> rows;
     kv4_load_rows<T, D>(rows, p, b, h, r0, total, length);
-    float s[4];
-    kv4_scores<T, D>(s, k0, k1, kp, rows);
+    float lse[2];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int row = r0 + 2 * t + (e & 1);
-      if (row < total && kv4_sees(rows.pos[e & 1], j0 + g + 8 * (e >> 1), p.window, p.sinks)) sum[e >> 1] += exp2_approx(fmaf(s[e], rows.unit[e & 1], -row_lse[row]));
+    for (int k = 0; k < 2; ++k) lse[k] = r0 + 2 * t + k < total ? row_lse[r0 + 2 * t + k] : INFINITY;
+#pragma unroll
+    for (int u = 0; u < kFinishEach; ++u) {
+      if (entry(u) >= length) continue;
+      float s[4];
+      kv4_scores<T, D>(s, k0[u], k1[u], kp[u], rows);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (kv4_sees(rows.pos[e & 1], entry(u) + g + 8 * (e >> 1), p.window, p.sinks)) sum[u][e >> 1] += exp2_approx(fmaf(s[e], rows.unit[e & 1], -lse[e & 1]));
     }
   }
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
-    sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
-    const int j = j0 + g + 8 * e;
-    if (t == 0 && j < length) p.weights[first + j] += sum[e];
-  }
+  for (int u = 0; u < kFinishEach; ++u)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      sum[u][e] += __shfl_xor_sync(0xffffffffu, sum[u][e], 1);
+      sum[u][e] += __shfl_xor_sync(0xffffffffu, sum[u][e], 2);
+      const int j = entry(u) + g + 8 * e;
+      if (t == 0 && j < length) p.weights[first + j] += sum[u][e];
+    }
 }
 
 namespace {
@@ -683,7 +702,7 @@ template <typename T, int D, int NT> int kv4_step(const Kv4StepParams &p, const 
   st = launch_step(kv4_step_kernel<T, D, NT>, dim3(static_cast<unsigned>(plan.slots)), smem, stream, pdl, p);
   if (st != MG_OK || (plan.whole && p.a.weights == nullptr)) return st;
   const int parts = plan.whole ? 1 : 8 * NT * D / 256 * plan.tiles;
-  const int entries = p.a.weights != nullptr ? (p.a.cache.capacity + 127) / 128 : 1;
+  const int entries = p.a.weights != nullptr ? (p.a.cache.capacity + kFinishEntries - 1) / kFinishEntries : 1;
   return launch_step(kv4_finish_kernel<T, D, NT>, dim3(std::max(parts, entries), p.a.cache.batch * p.a.cache.kv_heads), 0, stream, true, p);
 }
 
