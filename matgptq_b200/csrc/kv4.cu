@@ -23,15 +23,30 @@ MG_DEFINE_STATUS_ACCESSOR(kv4_device_status)
 // with fp32 differences and quotients, each rounded once.  A code is the nearest one for the scale as it is kept.
 // A row with an infinity, a NaN or a range beyond fp32 gets a NaN for its scale, so that what reads it comes out as NaN.
 // Bound by memory for prompts (reads 2 bytes and writes 2 or 0.5 bytes per element), by latency for single tokens.
-// x a + y b rounded to fp32 and then to T, as if computed without any other error: a code next to a border, and with the smallest
-// value of a row all of its codes, would go by the last bit.  The fp32 result is off by less than `off`; where that leaves T in doubt
-// (one value in 2000 in fp16, one in 16000 in bf16) 64 bits decide.
-template <typename T> __device__ __forceinline__ T turned(float x, float a, float y, float b) {
-  const float product = __fmul_rn(y, b), r = __fmaf_rn(x, a, product);
-  const float off = __fmaf_rn(0x1p-23f, fabsf(r), __fmaf_rn(0x1p-23f, fabsf(product), FLT_MIN));
-  const T low = from_f<T>(r - off), high = from_f<T>(r + off);
-  if (*reinterpret_cast<const uint16_t *>(&low) == *reinterpret_cast<const uint16_t *>(&high)) return low;
-  return from_f<T>(static_cast<float>(static_cast<double>(x) * a + static_cast<double>(y) * b));
+// Two numbers x a + y b, each rounded to fp32 and then to T as if computed without any other error: a code next to a border, and with
+// the smallest value of a row all of its codes, would go by the last bit.  The fp32 results are off by less than `off`; where that leaves
+// T in doubt (one value in 2000 in fp16, one in 16000 in bf16) 64 bits decide, out of line: the compiler computes them for all otherwise.
+static __device__ __noinline__ float turned_exactly(float x, float a, float y, float b) {
+  return static_cast<float>(static_cast<double>(x) * a + static_cast<double>(y) * b);
+}
+template <typename T> __device__ __forceinline__ uint32_t two_bits(float a, float b) {
+  return kv4_bits<T>(a) | static_cast<uint32_t>(kv4_bits<T>(b)) << 16;
+}
+template <> __device__ __forceinline__ uint32_t two_bits<__half>(float a, float b) {
+  const __half2 r = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+template <> __device__ __forceinline__ uint32_t two_bits<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+// the pair (x, y) turned by the angle of cosine c and sine s
+template <typename T> __device__ __forceinline__ uint32_t turned(float x, float y, float c, float s) {
+  const float p0 = __fmul_rn(y, -s), r0 = __fmaf_rn(x, c, p0), p1 = __fmul_rn(x, s), r1 = __fmaf_rn(y, c, p1);
+  const float off0 = __fmaf_rn(0x1p-23f, fabsf(r0) + fabsf(p0), FLT_MIN), off1 = __fmaf_rn(0x1p-23f, fabsf(r1) + fabsf(p1), FLT_MIN);
+  const uint32_t low = two_bits<T>(r0 - off0, r1 - off1), high = two_bits<T>(r0 + off0, r1 + off1);
+  if (low == high) return low;
+  return two_bits<T>(turned_exactly(x, c, y, -s), turned_exactly(y, c, x, s));
 }
 
 // rint(x / scale) for the fp32 quotient rounded once, 0 <= x / scale < 32: the approximate quotient is off by less than 2^-17, and only
@@ -62,33 +77,33 @@ __global__ void __launch_bounds__(256) append_kv4_kernel(const T *__restrict__ q
     bool outside = !padding && slot >= cache.capacity;
 
     uint4 raw = make_uint4(0, 0, 0, 0);
+    uint32_t *pair = reinterpret_cast<uint32_t *>(&raw);
     if (live && !padding) raw = *reinterpret_cast<const uint4 *>(qkv + (token * all + head) * cache.dim + c0);
-    T *e = reinterpret_cast<T *>(&raw);
     if (head < heads + cache.kv_heads && live && !padding) {
       const long long pos = positions[b * position_stride + s];
       if (pos < 0 || pos >= n_positions) {
         outside = true;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = from_f<T>(NAN);
+        for (int i = 0; i < 4; ++i) pair[i] = two_bits<T>(NAN, NAN);
       } else {
         const float4 cs = *reinterpret_cast<const float4 *>(cos_t + pos * (cache.dim >> 1) + (c0 >> 1));
         const float4 sn = *reinterpret_cast<const float4 *>(sin_t + pos * (cache.dim >> 1) + (c0 >> 1));
         const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-          const float x = to_f(e[2 * p]), y = to_f(e[2 * p + 1]);
-          e[2 * p] = turned<T>(x, cv[p], y, -sv[p]);
-          e[2 * p + 1] = turned<T>(y, cv[p], x, sv[p]);
+          pair[p] = turned<T>(kv4_to_f<T>(static_cast<uint16_t>(pair[p])), kv4_to_f<T>(static_cast<uint16_t>(pair[p] >> 16)), cv[p], sv[p]);
         }
       }
     }
     if (outside) report_status(kStatusCacheRange);
 
+    if (live && head < heads) *reinterpret_cast<uint4 *>(q_out + (token * heads + head) * cache.dim + c0) = raw;
+    if (__all_sync(0xffffffffu, !live || head < heads)) continue;  // nothing to quantise in this warp
     float x[8], low = FLT_MAX, high = -FLT_MAX;
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      x[i] = to_f(e[i]);
+      x[i] = kv4_to_f<T>(static_cast<uint16_t>(pair[i >> 1] >> (16 * (i & 1))));
       odd |= !(fabsf(x[i]) <= FLT_MAX);
       low = fminf(low, x[i]);
       high = fmaxf(high, x[i]);
@@ -98,12 +113,7 @@ __global__ void __launch_bounds__(256) append_kv4_kernel(const T *__restrict__ q
       low = fminf(low, __shfl_xor_sync(0xffffffffu, low, off));
       high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, off));
     }
-    if (!live) continue;
-    if (head < heads) {
-      *reinterpret_cast<uint4 *>(q_out + (token * heads + head) * cache.dim + c0) = raw;
-      continue;
-    }
-    if (padding || slot >= cache.capacity) continue;
+    if (!live || head < heads || padding || slot >= cache.capacity) continue;
     const float range = __fsub_rn(high, low);
     const T scale16 = from_f<T>(range <= FLT_MAX ? __fdiv_rn(range, 15.f) : NAN);
     const float scale = to_f(scale16);
@@ -262,42 +272,69 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_kv4_select_kernel(floa
   // `want` of the entries whose key is `prefix` stay, the first ones.  With no place at all (want == 0) none does, nor can a key
   // be above it: the passes then end at the top digit of each.
   const bool none = keep == sinks + recent;
-  __shared__ int s_equal[32], s_keep[32];
+  // 4096 entries a step: counts of 32 entries each, in order, their sums by one warp, twice (those equal to the smallest, those that stay)
+  constexpr int kEach = 4;
+  __shared__ int counts[2][32 * kEach], totals[2];
+  const auto add_up = [&](int which) {  // counts -> the sums before them; every thread comes here
+    __syncthreads();
+    if (warp == 0) {
+      int c[kEach], sum = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) sum += c[i] = counts[which][kEach * lane + i];
+      int up_to = sum;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, up_to, off);
+        if (lane >= off) up_to += x;
+      }
+      if (lane == 31) totals[which] = up_to;
+      up_to -= sum;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        counts[which][kEach * lane + i] = up_to;
+        up_to += c[i];
+      }
+    }
+    __syncthreads();
+  };
   int equal_before = 0, keep_before = 0;
-  for (int base = 0; base < n; base += kEvictThreads) {
-    const int j = base + tid;
-    const float value = j < n ? w[j] : 0.f;
-    const bool fixed = j < n && (j < first || j >= last);
-    const bool rival = j < n && !fixed && !none;
-    const uint32_t key = weight_key(value);
-    const bool equal = rival && key == prefix;
-    const unsigned eq_mask = __ballot_sync(0xffffffffu, equal);
-    if (lane == 0) s_equal[warp] = __popc(eq_mask);
-    __syncthreads();
-    int eq_rank = equal_before + __popc(eq_mask & ((1u << lane) - 1));
-    int eq_total = 0;
-    for (int i = 0; i < 32; ++i) {
-      if (i < warp) eq_rank += s_equal[i];
-      eq_total += s_equal[i];
+  for (int base = 0; base < n; base += kEach * kEvictThreads) {
+    float value[kEach];
+    unsigned equal[kEach], stays[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int j = base + k * kEvictThreads + tid;
+      value[k] = j < n ? w[j] : 0.f;
     }
-    const bool stays = fixed || (rival && key > prefix) || (equal && eq_rank < want);
-    const unsigned mask = __ballot_sync(0xffffffffu, stays);
-    if (lane == 0) s_keep[warp] = __popc(mask);
-    __syncthreads();  // also: every weight of these 1024 has been read
-    int at = keep_before + __popc(mask & ((1u << lane) - 1));
-    int total = 0;
-    for (int i = 0; i < 32; ++i) {
-      if (i < warp) at += s_keep[i];
-      total += s_keep[i];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int j = base + k * kEvictThreads + tid;
+      equal[k] = __ballot_sync(0xffffffffu, j >= first && j < last && !none && weight_key(value[k]) == prefix);
+      if (lane == 0) counts[0][k * 32 + warp] = __popc(equal[k]);
     }
-    if (stays && at < keep) {
-      mine[at] = j;
-      w[at] = value;  // at <= j: behind what is still to be read
+    add_up(0);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int j = base + k * kEvictThreads + tid;
+      const bool rival = j >= first && j < last && !none;
+      const int rank = equal_before + counts[0][k * 32 + warp] + __popc(equal[k] & ((1u << lane) - 1));
+      const bool stay = (j < n && !(j >= first && j < last)) || (rival && weight_key(value[k]) > prefix) || (((equal[k] >> lane) & 1u) && rank < want);
+      stays[k] = __ballot_sync(0xffffffffu, stay);
+      if (lane == 0) counts[1][k * 32 + warp] = __popc(stays[k]);
     }
-    equal_before += eq_total;
-    keep_before += total;
-    __syncthreads();
+    add_up(1);  // also: every weight of this step has been read
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int j = base + k * kEvictThreads + tid, at = keep_before + counts[1][k * 32 + warp] + __popc(stays[k] & ((1u << lane) - 1));
+      if (((stays[k] >> lane) & 1u) && at < keep) {
+        mine[at] = j;
+        w[at] = value[k];  // at <= j: behind what is still to be read
+      }
+    }
+    equal_before += totals[0];
+    keep_before += totals[1];
   }
+  __syncthreads();
   for (int j = keep + tid; j < n; j += kEvictThreads) w[j] = 0.f;
 }
 
