@@ -104,11 +104,6 @@ __global__ void __launch_bounds__(kNormThreads) add_rmsnorm_vec_kernel(T *__rest
   }
 }
 
-// The rotation with its roundings spelled out: left to the compiler, the two kernels below contracted the same expression
-// differently, and a model whose layers amplify one flipped bit showed it.
-__device__ __forceinline__ float rotated_even(float a, float c, float cs, float sn) { return __fmaf_rn(a, cs, -__fmul_rn(c, sn)); }
-__device__ __forceinline__ float rotated_odd(float a, float c, float cs, float sn) { return __fmaf_rn(c, cs, __fmul_rn(a, sn)); }
-
 // qkv [B, S, (H + 2*KV) * d] -> q_out [B, H, S, d] rotated; k rotated and v written into the caches
 // [B, KV, max_seq, d] at positions[s].  cos/sin are [max_seq, d/2] fp32.  Pairs are (2i, 2i+1).
 template <typename T>

@@ -16,6 +16,11 @@ template <typename T> __device__ __forceinline__ T from_f(float v);
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// The rotation with its roundings spelled out: left to the compiler, the kernels that rotate contracted the same expression
+// differently, and a model whose layers amplify one flipped bit showed it.
+__device__ __forceinline__ float rotated_even(float a, float c, float cs, float sn) { return __fmaf_rn(a, cs, -__fmul_rn(c, sn)); }
+__device__ __forceinline__ float rotated_odd(float a, float c, float cs, float sn) { return __fmaf_rn(c, cs, __fmul_rn(a, sn)); }
+
 // Programmatic dependent launch: let the next kernel of the stream start its prologue now (the packed products
 // prefetch their weights there), then wait until the previous kernel's results are complete and visible.  Both
 // are no-ops for a kernel that was launched without the attribute and has no dependents.

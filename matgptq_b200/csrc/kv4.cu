@@ -2,6 +2,7 @@
 // is in kv4_attention.cu.  The reference keeps its cache in 16 bits and leaves it to vLLM / transformers.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cfloat>
 #include <initializer_list>
 
@@ -18,7 +19,8 @@ MG_DEFINE_STATUS_ACCESSOR(kv4_device_status)
 // ---- writing ----------------------------------------------------------------------------------------------------------
 //
 // One row (a token's head) per d/8 lanes, eight channels a lane.  q and k are turned by the angles of the token's position in
-// pairs (2i, 2i + 1) and rounded to fp32, then to the model's type; k (rounded) and v are then quantised:
+// pairs (2i, 2i + 1) and rounded to the model's type: q as rope_kv does it, k as exactly as can be (below).  k (rounded) and v are then
+// quantised:
 //   scale = T((max - min) / 15),  code = min(15, rint((x - min) / scale))
 // with fp32 differences and quotients, each rounded once.  A code is the nearest one for the scale as it is kept.
 // A row with an infinity, a NaN or a range beyond fp32 gets a NaN for its scale, so that what reads it comes out as NaN.
@@ -40,105 +42,143 @@ template <> __device__ __forceinline__ uint32_t two_bits<__nv_bfloat16>(float a,
   const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t *>(&r);
 }
-// the pair (x, y) turned by the angle of cosine c and sine s
-template <typename T> __device__ __forceinline__ uint32_t turned(float x, float y, float c, float s) {
+// the pair (x, y) turned by the angle of cosine c and sine s; `doubt` where 64 bits have to decide
+template <typename T> __device__ __forceinline__ uint32_t turned(float x, float y, float c, float s, bool &doubt) {
   const float p0 = __fmul_rn(y, -s), r0 = __fmaf_rn(x, c, p0), p1 = __fmul_rn(x, s), r1 = __fmaf_rn(y, c, p1);
   const float off0 = __fmaf_rn(0x1p-23f, fabsf(r0) + fabsf(p0), FLT_MIN), off1 = __fmaf_rn(0x1p-23f, fabsf(r1) + fabsf(p1), FLT_MIN);
-  const uint32_t low = two_bits<T>(r0 - off0, r1 - off1), high = two_bits<T>(r0 + off0, r1 + off1);
-  if (low == high) return low;
-  return two_bits<T>(turned_exactly(x, c, y, -s), turned_exactly(y, c, x, s));
+  const uint32_t low = two_bits<T>(r0 - off0, r1 - off1);
+  doubt |= low != two_bits<T>(r0 + off0, r1 + off1);
+  return low;
 }
 
-// rint(x / scale) for the fp32 quotient rounded once, 0 <= x / scale < 32: the approximate quotient is off by less than 2^-17, and only
+// rint(x / scale) for the fp32 quotient rounded once, 0 <= x / scale < 32: the approximate quotient is off by less than 2^-16, and only
 // a quotient that near a border is divided for.
-__device__ __forceinline__ float nearest_code(float x, float scale, float per) {
+__device__ __forceinline__ float nearest_code(float x, float per, bool &doubt) {
   const float q = x * per, code = rintf(q);
-  return fabsf(q - code) < 0.5f - 0x1p-16f ? code : rintf(__fdiv_rn(x, scale));
+  doubt |= !(fabsf(q - code) < 0.5f - 0x1p-16f);
+  return code;
 }
 
-// blockIdx.x over the 16-byte pieces of a token's row, blockIdx.y walks the tokens
+// What a thread does with eight channels of one row of a token, c0 the first of them.  `code` words and scales of K and V go to `entry`.
 template <typename T>
-__global__ void __launch_bounds__(256) append_kv4_kernel(const T *__restrict__ qkv, const long long *__restrict__ positions,
+__device__ __forceinline__ void quantise_row(const uint32_t (&pair)[4], bool writes, int lanes, const Kv4Cache &cache, size_t entry, int c0, bool is_v) {
+  float x[8], low = FLT_MAX, high = -FLT_MAX;
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = kv4_to_f<T>(static_cast<uint16_t>(pair[i >> 1] >> (16 * (i & 1))));
+    odd |= !(fabsf(x[i]) <= FLT_MAX);
+    low = fminf(low, x[i]);
+    high = fmaxf(high, x[i]);
+  }
+  if (odd) high = INFINITY;
+  for (int off = lanes >> 1; off >= 1; off >>= 1) {  // whole warps come here: rows of one warp differ, lanes of one row do not
+    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, off));
+    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, off));
+  }
+  if (!writes) return;
+  const float range = __fsub_rn(high, low);
+  const T scale16 = from_f<T>(range <= FLT_MAX ? __fdiv_rn(range, 15.f) : NAN);
+  const float scale = to_f(scale16);
+  float per;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(per) : "f"(scale));
+  float code[8];
+  bool doubt = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) code[i] = nearest_code(__fsub_rn(x[i], low), per, doubt);
+  if (doubt) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) code[i] = scale > 0.f ? rintf(__fdiv_rn(__fsub_rn(x[i], low), scale)) : 0.f;  // (and a scale of 0 or NaN)
+  }
+  uint32_t word = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) word |= static_cast<uint32_t>(fminf(15.f, code[i])) << (4 * i);
+  if (is_v) {
+    uint16_t *units = reinterpret_cast<uint16_t *>(cache.v + (entry >> 1) * cache.dim) + (entry & 1) + (c0 >> 1);
+    units[0] = static_cast<uint16_t>(word);
+    units[2] = static_cast<uint16_t>(word >> 16);
+  } else {
+    *reinterpret_cast<uint32_t *>(cache.k + entry * (cache.dim >> 1) + (c0 >> 1)) = word;
+  }
+  if (c0 == 0) {
+    const T low16 = from_f<T>(low);
+    const uint32_t both = static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(&scale16)) |
+                          static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(&low16)) << 16;
+    *reinterpret_cast<uint32_t *>(cache.params + entry * 4 + (is_v ? 2 : 0)) = both;
+  }
+}
+
+// blockIdx.x walks the tokens of sequence blockIdx.y; a block takes a token's rows side by side, N times as
+// many as it has threads for: a thread keeps the angles of its channels for all of them, and asks for all of them at once.
+template <typename T, int N>
+__global__ void __launch_bounds__(256, 4) append_kv4_kernel(const T *__restrict__ qkv, const long long *__restrict__ positions,
                                                          long long position_stride, const float *__restrict__ cos_t,
                                                          const float *__restrict__ sin_t, long long n_positions,
                                                          const int *__restrict__ lengths, T *__restrict__ q_out, Kv4Cache cache, int seq,
                                                          int heads) {
   pdl_prologue();
   const int lanes = cache.dim >> 3, shift = cache.dim == 128 ? 4 : 3;  // of a row: 8 or 16
-  const int all = heads + 2 * cache.kv_heads;
-  const int at = blockIdx.x * 256 + threadIdx.x, c0 = (at & (lanes - 1)) * 8;
-  const bool live = (at >> shift) < all;
-  const int head = live ? at >> shift : 0;
-  for (int row = blockIdx.y; row < cache.batch * seq; row += gridDim.y) {
-    const long long token = row;
-    const int b = row / seq, s = row - b * seq;
-    const long long slot = static_cast<long long>(lengths[b]) - seq + s;
+  const int all = heads + 2 * cache.kv_heads, at_once = 256 >> shift;
+  const int row0 = threadIdx.x >> shift, c0 = (threadIdx.x & (lanes - 1)) * 8;
+  const int b = blockIdx.y;
+  const int slot0 = max(min(lengths[b], cache.capacity + seq), 0) - seq;  // (a length near the ends of 32 bits stays outside)
+  long long next_pos = positions[b * position_stride + blockIdx.x];
+  for (int s = blockIdx.x; s < seq; s += gridDim.x) {
+    const size_t token = static_cast<size_t>(b) * seq + s;
+    const T *src = qkv + token * all * cache.dim + c0;
+    T *dst = q_out + token * heads * cache.dim + c0;
+    const int slot = slot0 + s;
     const bool padding = slot < 0;
-    bool outside = !padding && slot >= cache.capacity;
-
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    uint32_t *pair = reinterpret_cast<uint32_t *>(&raw);
-    if (live && !padding) raw = *reinterpret_cast<const uint4 *>(qkv + (token * all + head) * cache.dim + c0);
-    if (head < heads + cache.kv_heads && live && !padding) {
-      const long long pos = positions[b * position_stride + s];
-      if (pos < 0 || pos >= n_positions) {
-        outside = true;
+    const long long pos = next_pos;
+    if (s + static_cast<int>(gridDim.x) < seq) next_pos = positions[b * position_stride + s + gridDim.x];
+    const bool placed = pos >= 0 && pos < n_positions;
+    uint4 raw[N];
+    const auto ask = [&](int first) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pair[i] = two_bits<T>(NAN, NAN);
-      } else {
-        const float4 cs = *reinterpret_cast<const float4 *>(cos_t + pos * (cache.dim >> 1) + (c0 >> 1));
-        const float4 sn = *reinterpret_cast<const float4 *>(sin_t + pos * (cache.dim >> 1) + (c0 >> 1));
-        const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          pair[p] = turned<T>(kv4_to_f<T>(static_cast<uint16_t>(pair[p])), kv4_to_f<T>(static_cast<uint16_t>(pair[p] >> 16)), cv[p], sv[p]);
-        }
+      for (int n = 0; n < N; ++n) {
+        raw[n] = make_uint4(0, 0, 0, 0);
+        if (first + n * at_once < all && !padding) raw[n] = *reinterpret_cast<const uint4 *>(src + (first + n * at_once) * cache.dim);
       }
+    };
+    ask(row0);
+    float4 cs = make_float4(0.f, 0.f, 0.f, 0.f), sn = cs;
+    if (placed) {
+      cs = *reinterpret_cast<const float4 *>(cos_t + pos * (cache.dim >> 1) + (c0 >> 1));
+      sn = *reinterpret_cast<const float4 *>(sin_t + pos * (cache.dim >> 1) + (c0 >> 1));
     }
-    if (outside) report_status(kStatusCacheRange);
-
-    if (live && head < heads) *reinterpret_cast<uint4 *>(q_out + (token * heads + head) * cache.dim + c0) = raw;
-    if (__all_sync(0xffffffffu, !live || head < heads)) continue;  // nothing to quantise in this warp
-    float x[8], low = FLT_MAX, high = -FLT_MAX;
-    bool odd = false;
+    const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
+    if (!padding && (!placed || slot >= cache.capacity)) report_status(kStatusCacheRange);
+    for (int first = row0; first - row0 < all; first += N * at_once) {
+      if (first != row0) ask(first);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = kv4_to_f<T>(static_cast<uint16_t>(pair[i >> 1] >> (16 * (i & 1))));
-      odd |= !(fabsf(x[i]) <= FLT_MAX);
-      low = fminf(low, x[i]);
-      high = fmaxf(high, x[i]);
-    }
-    if (odd) high = INFINITY;
-    for (int off = lanes >> 1; off >= 1; off >>= 1) {  // whole warps come here: rows of one warp differ, lanes of one row do not
-      low = fminf(low, __shfl_xor_sync(0xffffffffu, low, off));
-      high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, off));
-    }
-    if (!live || head < heads || padding || slot >= cache.capacity) continue;
-    const float range = __fsub_rn(high, low);
-    const T scale16 = from_f<T>(range <= FLT_MAX ? __fdiv_rn(range, 15.f) : NAN);
-    const float scale = to_f(scale16);
-    float per;
-    asm("rcp.approx.f32 %0, %1;" : "=f"(per) : "f"(scale));
-    uint32_t word = 0;
+      for (int n = 0; n < N; ++n) {
+        const int row = first + n * at_once;
+        const uint32_t in[4] = {raw[n].x, raw[n].y, raw[n].z, raw[n].w};
+        const auto x = [&](int p) { return kv4_to_f<T>(static_cast<uint16_t>(in[p])); };
+        const auto y = [&](int p) { return kv4_to_f<T>(static_cast<uint16_t>(in[p] >> 16)); };
+        uint32_t pair[4] = {in[0], in[1], in[2], in[3]};
+        if (row < heads) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float c = scale > 0.f ? fminf(15.f, nearest_code(__fsub_rn(x[i], low), scale, per)) : 0.f;
-      word |= static_cast<uint32_t>(c) << (4 * i);
-    }
-    const bool is_v = head >= heads + cache.kv_heads;
-    const size_t entry = (static_cast<size_t>(b) * cache.kv_heads + (head - heads - (is_v ? cache.kv_heads : 0))) * cache.capacity + slot;
-    if (is_v) {
-      uint16_t *units = reinterpret_cast<uint16_t *>(cache.v + (entry >> 1) * cache.dim) + (entry & 1) + (c0 >> 1);
-      units[0] = static_cast<uint16_t>(word);
-      units[2] = static_cast<uint16_t>(word >> 16);
-    } else {
-      *reinterpret_cast<uint32_t *>(cache.k + entry * (cache.dim >> 1) + (c0 >> 1)) = word;
-    }
-    if (c0 == 0) {
-      const T low16 = from_f<T>(low);
-      const uint32_t both = static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(&scale16)) |
-                            static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(&low16)) << 16;
-      *reinterpret_cast<uint32_t *>(cache.params + entry * 4 + (is_v ? 2 : 0)) = both;
+          for (int p = 0; p < 4; ++p) pair[p] = two_bits<T>(rotated_even(x(p), y(p), cv[p], sv[p]), rotated_odd(x(p), y(p), cv[p], sv[p]));
+          if (!placed && !padding) pair[0] = pair[1] = pair[2] = pair[3] = two_bits<T>(NAN, NAN);
+          *reinterpret_cast<uint4 *>(dst + row * cache.dim) = make_uint4(pair[0], pair[1], pair[2], pair[3]);
+        }
+        if (__all_sync(0xffffffffu, row < heads || row >= all)) continue;  // nothing to quantise in this warp
+        const int kv = row - heads;
+        const bool is_v = kv >= cache.kv_heads;
+        if (kv >= 0 && !is_v) {
+          bool doubt = false;
+#pragma unroll
+          for (int p = 0; p < 4; ++p) pair[p] = turned<T>(x(p), y(p), cv[p], sv[p], doubt);
+          if (doubt) {
+#pragma unroll
+            for (int p = 0; p < 4; ++p) pair[p] = two_bits<T>(turned_exactly(x(p), cv[p], y(p), -sv[p]), turned_exactly(y(p), cv[p], x(p), sv[p]));
+          }
+          if (!placed) pair[0] = pair[1] = pair[2] = pair[3] = two_bits<T>(NAN, NAN);
+        }
+        const size_t entry = (static_cast<size_t>(b) * cache.kv_heads + (is_v ? kv - cache.kv_heads : max(kv, 0))) * cache.capacity + max(slot, 0);
+        quantise_row<T>(pair, kv >= 0 && row < all && !padding && slot < cache.capacity, lanes, cache, entry, c0, is_v);
+      }
     }
   }
 }
@@ -473,19 +513,24 @@ int matgptq_b200_append_kv4(const matgptq_b200_kv4_cache *cache, const void *qkv
   if (seq < 0 || seq > (1 << 30) || n_heads <= 0 || n_heads > (1 << 20) || n_positions <= 0 || position_stride < 0) return MG_ERR_BAD_ARG;
   if (misaligned({qkv, cos_table, sin_table, q_out})) return MG_ERR_ALIGNMENT;
   const Kv4Cache c = mg::kv4_cache(cache);
-  const long long tokens = cache->batch * seq;
-  if (tokens == 0) return MG_OK;
-  if (tokens > INT32_MAX) return MG_ERR_UNSUPPORTED;
-  const long long x = ((n_heads + 2 * cache->n_kv_heads) * (c.dim / 8) + 255) / 256, most = (148LL * 64 + x - 1) / x;
-  const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(tokens < most ? tokens : most));
-  const auto go = [&](auto tag) {
+  if (cache->batch == 0 || seq == 0) return MG_OK;
+  // a block for each token as long as the SMs of a B200 have fewer than sixteen, then blocks that walk
+  const long long x = std::min<long long>(seq, std::max(1LL, 148LL * 16 / cache->batch));
+  const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(cache->batch));
+  const bool wide = (n_heads + 2 * cache->n_kv_heads) * (c.dim / 8) > 256;  // more rows than a block takes at once
+  const auto go = [&](auto kernel, auto tag) {
     using T = decltype(tag);
-    return mg::launch_helper(mg::append_kv4_kernel<T>, grid, 256, static_cast<cudaStream_t>(stream),
-                             (flags & MATGPTQ_B200_FLAG_PDL) != 0, static_cast<const T *>(qkv), reinterpret_cast<const long long *>(positions),
-                             static_cast<long long>(position_stride), cos_table, sin_table, static_cast<long long>(n_positions),
-                             static_cast<const int *>(lengths), static_cast<T *>(q_out), c, static_cast<int>(seq), static_cast<int>(n_heads));
+    return mg::launch_helper(kernel, grid, 256, static_cast<cudaStream_t>(stream), (flags & MATGPTQ_B200_FLAG_PDL) != 0, static_cast<const T *>(qkv),
+                             reinterpret_cast<const long long *>(positions), static_cast<long long>(position_stride), cos_table, sin_table,
+                             static_cast<long long>(n_positions), static_cast<const int *>(lengths), static_cast<T *>(q_out), c,
+                             static_cast<int>(seq), static_cast<int>(n_heads));
   };
-  return (flags & MATGPTQ_B200_FLAG_BF16) ? go(__nv_bfloat16{}) : go(__half{});
+  if (flags & MATGPTQ_B200_FLAG_BF16) {
+    using T = __nv_bfloat16;
+    return wide ? go(mg::append_kv4_kernel<T, 3>, T{}) : go(mg::append_kv4_kernel<T, 1>, T{});
+  }
+  using T = __half;
+  return wide ? go(mg::append_kv4_kernel<T, 3>, T{}) : go(mg::append_kv4_kernel<T, 1>, T{});
 }
 
 int matgptq_b200_dequantize_kv4(const matgptq_b200_kv4_cache *cache, const int32_t *lengths, int64_t count, void *k_out, void *v_out,

@@ -139,9 +139,9 @@ def test_append_rotates(cuda, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 def test_append_rounds_the_rotation_once(cuda, dtype):
-    """q, codes and scales are to the bit those of the rotation in 64 bits, rounded to fp32 and to the type: no code goes by an error of
-    the rotation.  Zero coordinates, infinities and magnitudes near the type's limits among them."""
-    from matgptq_b200 import ops
+    """Codes and scales are to the bit those of the rotation in 64 bits, rounded to fp32 and to the type: no code goes by an error of the
+    rotation.  q has the bits that the 16-bit cache's operator gives it.  Zero coordinates, small and large values among them."""
+    from matgptq_b200 import _native, ops
     b, seq, heads, kv, d, capacity = 4, 500, 6, 2, 128, 512
     gen = torch.Generator(device=cuda).manual_seed(4)
     qkv = torch.randn(b, seq, heads + 2 * kv, d, generator=gen, device=cuda)
@@ -149,6 +149,7 @@ def test_append_rounds_the_rotation_once(cuda, dtype):
     qkv[1] *= 1e-4
     qkv[2, :, :, ::9] *= 500
     qkv = qkv.to(dtype)
+    qkv = qkv.contiguous()
     positions = torch.arange(capacity - seq, capacity, device=cuda)
     angle = torch.arange(capacity, device=cuda)[:, None] / 500000 ** (torch.arange(0, d, 2, device=cuda) / d)[None]
     cos, sin = angle.cos().float().contiguous(), angle.sin().float().contiguous()
@@ -161,7 +162,13 @@ def test_append_rounds_the_rotation_once(cuda, dtype):
     turned[..., 0::2] = x[..., 0::2] * c - x[..., 1::2] * s
     turned[..., 1::2] = x[..., 1::2] * c + x[..., 0::2] * s
     turned = turned.float().to(dtype)
-    assert torch.equal(q, turned[:, :, :heads])
+    q16 = torch.empty(b, heads, seq, d, dtype=dtype, device=cuda)
+    k16 = torch.zeros(b, kv, capacity, d, dtype=dtype, device=cuda)
+    v16 = torch.zeros_like(k16)
+    _native.check(_native.load().matgptq_b200_rope_kv(
+        qkv.data_ptr(), positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), q16.data_ptr(), k16.data_ptr(), v16.data_ptr(), b, seq, heads, kv, d,
+        capacity, flag_of(dtype), torch.cuda.current_stream().cuda_stream), "rope_kv")
+    assert torch.equal(q.transpose(1, 2), q16)
     k_codes, k_scale, k_min = oracle.quantise_rows(turned[:, :, heads:].transpose(1, 2))
     assert torch.equal(oracle.unpack_k(cache[0])[:, :, :seq], k_codes)
     assert torch.equal(cache[2][:, :, :seq, 0:2].double(), torch.cat([k_scale, k_min], -1))
