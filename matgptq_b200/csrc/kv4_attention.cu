@@ -754,7 +754,7 @@ int matgptq_b200_attention_kv4(const matgptq_b200_kv4_cache *cache, const void *
   if (st != MG_OK) return st;
   if (!q || !lengths || !out) return MG_ERR_BAD_ARG;
   if (seq < 0 || n_heads <= 0 || n_heads % cache->n_kv_heads != 0 || window < 0 || sinks < 0) return MG_ERR_BAD_ARG;
-  if (seq > (1 << 24) || n_heads > (1 << 16) || seq * (n_heads / cache->n_kv_heads) > (1 << 24)) return MG_ERR_UNSUPPORTED;
+  if (seq > (1 << 24) || n_heads > (1 << 16) || seq * (n_heads / cache->n_kv_heads) >= (1 << 24)) return MG_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) % 16 != 0) return MG_ERR_ALIGNMENT;
   if (cache->batch == 0 || seq == 0) return MG_OK;
   const int64_t need = matgptq_b200_attention_kv4_workspace_bytes(cache, seq, n_heads, window, sinks, weights != nullptr);

@@ -1,10 +1,10 @@
 // Attention over the 4-bit cache for many rows (the mathematics: kv4_attention.cu), on the tensor cores: a CTA takes 256 rows of one
 // key/value head and goes over tiles of 128 entries.
 //
-//   * four producer warps turn a tile's codes into operands in shared memory, once for both halves of the rows: K as fp16 subnormals
+//   * two producer warps turn a tile's codes into operands in shared memory, once for both halves of the rows: K as fp16 subnormals
 //     (one mask per two codes; the codes that sit 4 bits up meet a q that was divided by 16), V centred; and its scales and minima as fp32;
 //   * one warp issues the MMAs: S = Q K^T (M 128 rows, N 128 entries) into tensor memory, and O += P V with P read from there;
-//   * two times four warps, a thread per row, take S from tensor memory, scale, mask and exponentiate it and put P = p v_scale back as
+//   * two times four warps, a lane four rows' quarters, take S from tensor memory, scale, mask and exponentiate it and put P = p v_scale back as
 //     fp16 over it.  While one half does that, the MMAs of the other run.
 //
 // The accumulator stays in tensor memory.  It is only rescaled when a row's maximum has grown by more than a factor of 2^8 (P then has
@@ -28,15 +28,17 @@ namespace mg {
 MG_DEFINE_STATUS_ACCESSOR(kv4_prompt_device_status)
 
 constexpr int kPrRows = 256, kPrTile = 128;   // rows of a CTA, entries of a tile
-constexpr int kPrWarps = 13;                  // 8 of softmax, 4 producers, 1 that issues
+constexpr int kPrProducers = 2;
+constexpr int kPrWarps = 12;                  // 8 of softmax, the producers, 1 that issues (1 idle: registers are dealt out to four warps)
 // Shared memory: barriers, Q, two stages of K, V and params.
 constexpr int kPrBarKFull = 0, kPrBarVFull = 16, kPrBarEmpty = 32, kPrBarS = 48, kPrBarP = 64, kPrBarQ = 80, kPrBarEnd = 88, kPrTmemSlot = 96,
-              kPrUnit = 104 /* unit of P of each stage */, kPrMax = 112 /* four warps' maxima */;
+              kPrUnit = 104 /* unit of P of each stage */, kPrMax = 112 /* the producers' maxima */;
 template <int D> struct PromptPlan {
   static constexpr int q = 1024, q_bytes = 128 * D * 2;                    // per half
   static constexpr int stages = q + 2 * q_bytes, k_bytes = kPrTile * D * 2;  // K and V have the same size
   static constexpr int params = stages + 4 * k_bytes, param_bytes = 4 * kPrTile * 4;
-  static constexpr int end = params + 2 * param_bytes;
+  static constexpr int rows = params + 2 * param_bytes;  // three numbers for each row
+  static constexpr int end = rows + kPrRows * 12;
 };
 
 // 32 columns of this warp's 32 lanes of tensor memory, and back; the caller waits
@@ -50,12 +52,30 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *v) {
         "=r"(v[31])
       : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]),
-      "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
-      "r"(v[15]), "r"(taddr)
-      : "memory");
+// 32 columns of 16 lanes: a lane (g, t) has of row g the columns 8 i + 2 t and + 1 in v[4 i] and v[4 i + 1], of row g + 8 in v[4 i + 2]
+// and v[4 i + 3]; the caller waits
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t *v) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+                 "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_16x32(uint32_t taddr, const uint32_t *v) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
+               "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(taddr)
+               : "memory");
+}
+// 16 columns of 16 lanes: of row g column 4 i + t in v[2 i], of row g + 8 in v[2 i + 1]
+__device__ __forceinline__ void tmem_ld_16x16(uint32_t taddr, uint32_t *v) {
+  asm volatile("tcgen05.ld.sync.aligned.16x128b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_16x16(uint32_t taddr, const uint32_t *v) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+               "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(taddr)
+               : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -89,115 +109,193 @@ __device__ __forceinline__ void lds_2x64(uint32_t addr, uint64_t &a, uint64_t &b
 // the lowest n of 32 bits
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
-// What a thread keeps of its row
-struct PromptRow {
-  float unit, sum;   // log2 of a weight per score, score per minimum of K
-  float m;           // maximum so far, a whole number of log2
-  float v_unit;      // unit of P, and of the accumulator
-  uint64_t l2, fix2; // sums of the weights, and of the weights times the centres; two halves each
+// What a lane (g, t) keeps of its four rows, g, g + 8, g + 16 and g + 24 of the warp's 32, of which it has a quarter of the columns, 2 t
+// and 2 t + 1 of every eight.  (A lane with one row and all columns needs the scales and minima of all entries: at four numbers an
+// entry and lane, shared memory then takes 4096 cycles for a tile whose exponentials take 2048.)
+struct PromptRows {
+  uint64_t unit2[4], sum2[4];  // log2 of a weight per score, score per minimum of K; twice each
+  float m[4];                  // what the exponentials are taken against: about the maximum so far, a whole number of log2
+  uint64_t shift2[4];          // -m twice; 0 where nothing was seen
+  bool unset;                  // some row of the warp has not seen anything yet
+  uint64_t l2[4], fix2[4];     // this lane's part of the sums of the weights, and of the weights times the centres; two halves each
+  float v_unit;                // unit of P, and of the accumulator
 };
 
-// A thread's row over a tile of 128 entries: S from tensor memory, P back over it.  Entry c of the tile is seen when c <= hi and
-// (c > lo or c < sk); WHOLE: all are.  `started`: the accumulator at t_o holds something.
+// Scores of eight columns of the four rows, from what tensor memory holds of them
+__device__ __forceinline__ void prompt_scores(uint64_t (&score)[4], const uint32_t (&s)[2][16], int i, uint64_t ks, uint64_t kl, const PromptRows &r) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t *raw = s[k >> 1] + 4 * i + 2 * (k & 1);
+    score[k] = fma2(ks, pack2(__uint_as_float(raw[0]), __uint_as_float(raw[1])), mul2(kl, r.sum2[k]));
+  }
+}
+
+// Raises the rows' maxima to those of a tile's entries 32 c .. + 31, and brings what was summed up so far into the new units: the lane's
+// sums, the accumulator where it has been started, P of the tile's entries before these.
 template <bool WHOLE, int D>
-__device__ __forceinline__ void prompt_tile(PromptRow &r, uint32_t t_s, uint32_t t_o, uint32_t par, float unit_now, bool started, int hi, int lo,
-                                            int sk) {
-  const uint64_t sum2 = pack2(r.sum, r.sum), unit2 = pack2(r.unit, r.unit);
-#pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    union {
-      uint32_t u[32];
-      uint64_t d[16];
-    } s;
-    tmem_ld32(t_s + 32 * c, s.u);
-    uint32_t seen = 0xffffffffu;
-    if (!WHOLE) seen = bits_below(hi + 1 - 32 * c) & (~bits_below(lo + 1 - 32 * c) | bits_below(sk - 32 * c));
-    const uint32_t at = par + 32 * 4 * c;
+__device__ __forceinline__ void prompt_raise(PromptRows &r, const uint32_t (&seen)[4], uint32_t at, uint32_t t_s, uint32_t t_o, float unit_now,
+                                             bool started, int c) {
+  constexpr uint32_t kLanes16 = 16u << 16;
+  float f[4], top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  {
+    uint32_t s[2][16];
+    tmem_ld_16x32(t_s + 32 * c, s[0]);
+    tmem_ld_16x32(t_s + kLanes16 + 32 * c, s[1]);
     tmem_wait_ld();
-    float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-      uint64_t ks[2], kl[2];
-      lds_2x64(at + i * 8, ks[0], ks[1]);
-      lds_2x64(at + kPrTile * 4 + i * 8, kl[0], kl[1]);
+    for (int i = 0; i < 4; ++i) {
+      uint64_t ks, kl, score[4];
+      lds_2x64(at + i * 128, ks, kl);
+      prompt_scores(score, s, i, ks, kl, r);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        s.d[i + k] = fma2(ks[k], s.d[i + k], mul2(kl[k], sum2));
+      for (int k = 0; k < 4; ++k) {
         float x, y;
-        unpack2(s.d[i + k], x, y);
-        if (WHOLE || ((seen >> (2 * (i + k))) & 1u)) top = fmaxf(top, x);
-        if (WHOLE || ((seen >> (2 * (i + k) + 1)) & 1u)) top = fmaxf(top, y);
+        unpack2(score[k], x, y);
+        if (WHOLE || ((seen[k] >> (8 * i)) & 1u)) top[k] = fmaxf(top[k], x);
+        if (WHOLE || ((seen[k] >> (8 * i + 1)) & 1u)) top[k] = fmaxf(top[k], y);
       }
     }
-    top *= r.unit;
-    // The maximum may lag by 2^8; whole numbers keep the factors powers of two, which P in fp16 takes without another rounding.
-    if (__any_sync(0xffffffffu, top > r.m + 8.f || r.v_unit != unit_now)) {
-      const float m_new = fmaxf(r.m, ceilf(top));
-      const float f = r.m == -INFINITY ? 0.f : exp2_approx(r.m - m_new);
-      r.m = m_new;
-      const uint64_t f2 = pack2(f, f);
-      r.l2 = mul2(r.l2, f2);
-      r.fix2 = mul2(r.fix2, f2);
-      const float g = f * (r.v_unit / unit_now);
-      if (started) {
-        // the accumulator is at rest: S of this tile was asked for after P V of the last one
-#pragma unroll 1
-        for (int col = 0; col < D; col += 16) {
-          uint32_t o[16];
-          tmem_ld16(t_o + col, o);
+  }
+  bool unset = false;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * g);
-          tmem_st16(t_o + col, o);
-        }
-      }
-      // the first 32 c entries' P, if any: its unit is this tile's already
-      tmem_wait_st();
-      const __half2 f16 = __float2half2_rn(f);
+  for (int k = 0; k < 4; ++k) {
+    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
+    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
+    float unit, same;
+    unpack2(r.unit2[k], unit, same);
+    const float m_new = fmaxf(r.m[k], ceilf(top[k] * unit));
+    f[k] = r.m[k] == -INFINITY ? 0.f : exp2_approx(r.m[k] - m_new);
+    r.m[k] = m_new;
+    unset |= m_new == -INFINITY;
+    const float shift = m_new == -INFINITY ? 0.f : -m_new;
+    r.shift2[k] = pack2(shift, shift);
+    const uint64_t f2 = pack2(f[k], f[k]);
+    r.l2[k] = mul2(r.l2[k], f2);
+    r.fix2[k] = mul2(r.fix2[k], f2);
+  }
+  r.unset = __any_sync(0xffffffffu, unset);
+  tmem_wait_st();
+  if (started) {
+    // the accumulator is at rest: S of this tile was asked for after P V of the last one
+    const float unit_change = r.v_unit / unit_now;  // powers of two
 #pragma unroll 1
-      for (int col = 0; col < 16 * c; col += 16) {
+    for (int half = 0; half < 2; ++half)
+#pragma unroll 1
+      for (int col = 0; col < D; col += 32) {
         uint32_t o[16];
-        tmem_ld16(t_s + col, o);
+        tmem_ld_16x32(t_o + half * kLanes16 + col, o);
+        tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const __half2 x = __hmul2(*reinterpret_cast<const __half2 *>(&o[i]), f16);
-          o[i] = *reinterpret_cast<const uint32_t *>(&x);
-        }
-        tmem_st16(t_s + col, o);
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * ((i & 2) ? (half ? f[3] : f[1]) : (half ? f[2] : f[0])) * unit_change);
+        tmem_st_16x32(t_o + half * kLanes16 + col, o);
       }
-      r.v_unit = unit_now;
+  }
+  // P of this tile: its unit is the tile's already
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    const __half2 f_low = __float2half2_rn(half ? f[2] : f[0]), f_high = __float2half2_rn(half ? f[3] : f[1]);
+#pragma unroll 1
+    for (int col = 0; col < 16 * c; col += 16) {
+      uint32_t o[8];
+      tmem_ld_16x16(t_s + half * kLanes16 + col, o);
+      tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const __half2 x = __hmul2(*reinterpret_cast<const __half2 *>(&o[i]), (i & 1) ? f_high : f_low);
+        o[i] = *reinterpret_cast<const uint32_t *>(&x);
+      }
+      tmem_st_16x16(t_s + half * kLanes16 + col, o);
     }
-    const float shift = r.m == -INFINITY ? 0.f : -r.m;
-    const uint64_t shift2 = pack2(shift, shift);
-    uint32_t pv[16];
+  }
+  r.v_unit = unit_now;
+}
+
+// The warp's rows over a tile of 128 entries: S from tensor memory, P back over it.  Entry c of the tile is seen by row r when
+// c <= hi[r] and (c > lo[r] or c < sk); WHOLE: all are.  `started`: the accumulator at t_o holds something.
+template <bool WHOLE, int D>
+__device__ __forceinline__ void prompt_tile(PromptRows &r, uint32_t t_s, uint32_t t_o, uint32_t par, float unit_now, bool started, const int (&hi)[4],
+                                            int window, int sk) {
+  const int t = threadIdx.x & 3;
+  constexpr uint32_t kLanes16 = 16u << 16;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {  // 32 entries
+    const uint32_t at = par + (16 * c + t) * 32;
+    uint32_t seen[4];
+    if (!WHOLE) {
 #pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-      uint64_t vs[2], mid[2];
-      lds_2x64(at + 2 * kPrTile * 4 + i * 8, vs[0], vs[1]);
-      lds_2x64(at + 3 * kPrTile * 4 + i * 8, mid[0], mid[1]);
+      for (int k = 0; k < 4; ++k) {
+        const int lo = window > 0 ? hi[k] - window : -1;
+        seen[k] = (bits_below(hi[k] + 1 - 32 * c) & (~bits_below(lo + 1 - 32 * c) | bits_below(sk - 32 * c))) >> (2 * t);
+      }
+    }
+    // The exponentials are taken against a maximum that may lag: it is looked for when a row sees its first entries, and when eight
+    // weights of a row add up to more than 2^8 of what the maximum stands for.  (Looking for it every time took 1300 cycles of 4500:
+    // no exponential could begin before the last score.)  Whole numbers keep the factors powers of two, which P in fp16 takes without
+    // another rounding.
+    if (r.unset || r.v_unit != unit_now) prompt_raise<WHOLE, D>(r, seen, at, t_s, t_o, unit_now, started, c);
+    uint32_t pv[2][8];
+    uint64_t l_here[4], fix_here[4];
+    for (int pass = 0;; ++pass) {
+      uint32_t s[2][16];
+      tmem_ld_16x32(t_s + 32 * c, s[0]);
+      tmem_ld_16x32(t_s + kLanes16 + 32 * c, s[1]);
+      tmem_wait_ld();
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int i = 0; i < 4; ++i) {
+        uint64_t ks, kl, vs, mid, w[4];
+        float x[4], y[4];
+        lds_2x64(at + i * 128, ks, kl);
+        lds_2x64(at + i * 128 + 16, vs, mid);
+        prompt_scores(w, s, i, ks, kl, r);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = fma2(w[k], r.unit2[k], r.shift2[k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          unpack2(w[k], x[k], y[k]);
+          x[k] = exp2_approx(x[k]);
+          y[k] = exp2_approx(y[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint64_t v = vs, centre = mid;
+          if (!WHOLE) {  // hidden entries may hold a NaN: nothing of theirs is multiplied
+            float m0, m1, v0, v1;
+            unpack2(centre, m0, m1);
+            unpack2(v, v0, v1);
+            if (!((seen[k] >> (8 * i)) & 1u)) x[k] = 0.f, m0 = 0.f, v0 = 0.f;
+            if (!((seen[k] >> (8 * i + 1)) & 1u)) y[k] = 0.f, m1 = 0.f, v1 = 0.f;
+            centre = pack2(m0, m1);
+            v = pack2(v0, v1);
+          }
+          w[k] = pack2(x[k], y[k]);
+          l_here[k] = i == 0 ? w[k] : add2(l_here[k], w[k]);
+          fix_here[k] = i == 0 ? mul2(w[k], centre) : fma2(w[k], centre, fix_here[k]);
+          w[k] = mul2(w[k], v);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          unpack2(w[k], x[k], y[k]);
+          const __half2 h = __floats2half2_rn(x[k], y[k]);
+          pv[k >> 1][2 * i + (k & 1)] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+      }
+      bool raise = false;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
         float x, y;
-        unpack2(fma2(s.d[i + k], unit2, shift2), x, y);
-        x = exp2_approx(x);
-        y = exp2_approx(y);
-        if (!WHOLE) {  // hidden entries may hold a NaN: nothing of theirs is multiplied
-          float m0, m1, v0, v1;
-          unpack2(mid[k], m0, m1);
-          unpack2(vs[k], v0, v1);
-          if (!((seen >> (2 * (i + k))) & 1u)) x = 0.f, m0 = 0.f, v0 = 0.f;
-          if (!((seen >> (2 * (i + k) + 1)) & 1u)) y = 0.f, m1 = 0.f, v1 = 0.f;
-          mid[k] = pack2(m0, m1);
-          vs[k] = pack2(v0, v1);
-        }
-        const uint64_t p2 = pack2(x, y);
-        r.l2 = add2(r.l2, p2);
-        r.fix2 = fma2(p2, mid[k], r.fix2);
-        unpack2(mul2(p2, vs[k]), x, y);
-        const __half2 h = __floats2half2_rn(x, y);
-        pv[i + k] = *reinterpret_cast<const uint32_t *>(&h);
+        unpack2(l_here[k], x, y);
+        raise |= x + y > 256.f;
       }
+      if (pass > 0 || !__any_sync(0xffffffffu, raise)) break;
+      prompt_raise<WHOLE, D>(r, seen, at, t_s, t_o, unit_now, started, c);
     }
-    tmem_st16(t_s + 16 * c, pv);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      r.l2[k] = add2(r.l2[k], l_here[k]);
+      r.fix2[k] = add2(r.fix2[k], fix_here[k]);
+    }
+    tmem_st_16x16(t_s + 16 * c, pv[0]);
+    tmem_st_16x16(t_s + kLanes16 + 16 * c, pv[1]);
   }
 }
 
@@ -207,11 +305,11 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
   extern __shared__ __align__(1024) unsigned char prompt_smem[];
   const uint32_t base = smem_u32(prompt_smem);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  constexpr int kProducer = 8, kMma = 12;
+  constexpr int kProducer = 8, kMma = kProducer + kPrProducers;
   if (warp == kMma) {
     if (lane < 2) {
-      mbar_init(base + kPrBarKFull + 8 * lane, 4);
-      mbar_init(base + kPrBarVFull + 8 * lane, 4);
+      mbar_init(base + kPrBarKFull + 8 * lane, kPrProducers);
+      mbar_init(base + kPrBarVFull + 8 * lane, kPrProducers);
       mbar_init(base + kPrBarEmpty + 8 * lane, 1);
       mbar_init(base + kPrBarS + 8 * lane, 1);
       mbar_init(base + kPrBarP + 8 * lane, 4);
@@ -231,11 +329,11 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(prompt_smem + kPrTmemSlot);
   pdl_prologue();
 
-  const int b = blockIdx.y / p.cache.kv_heads, h = blockIdx.y - b * p.cache.kv_heads;
+  const int bh = blockIdx.x, b = bh / p.cache.kv_heads, h = bh - b * p.cache.kv_heads;
   const int total = p.seq * p.group;
-  const int r0 = (gridDim.x - 1 - blockIdx.x) * kPrRows;  // the tiles with the most entries first
+  const int r0 = (gridDim.y - 1 - blockIdx.y) * kPrRows;  // the tiles with the most entries first, of all heads
   const int length = kv4_length(p.lengths, b, p.cache.capacity);
-  const size_t first = static_cast<size_t>(blockIdx.y) * p.cache.capacity;
+  const size_t first = static_cast<size_t>(bh) * p.cache.capacity;
   const int pos_lo = length - p.seq + r0 / p.group, pos_hi = length - p.seq + (min(r0 + kPrRows, total) - 1) / p.group;
   // the tiles that the rows see: those of first entries, then those of the window
   const Kv4Range range = kv4_range<kPrTile>(pos_lo, pos_hi, p.window, p.sinks, p.cache.capacity);
@@ -249,37 +347,38 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
     const int row = r0 + threadIdx.x;  // of the key/value head
     const bool live = row < total;
     const int query = live ? row / p.group : 0;
-    const int pos = live ? length - p.seq + query : -1;
     const int wg_lo = length - p.seq + (r0 + half * 128) / p.group;                                  // of this half's rows
     const int wg_hi = length - p.seq + (min(r0 + half * 128 + 128, total) - 1) / p.group;
     const size_t out_at = ((static_cast<size_t>(b) * p.seq + query) * p.heads + static_cast<size_t>(h) * p.group + (live ? row - query * p.group : 0)) * D;
     // this row's tile for the pass that adds up the weights, where there is one
     uint8_t *tile_out = nullptr;
     if (p.row_tiles != nullptr && r0 + half * 128 < total)
-      tile_out = p.row_tiles + (static_cast<size_t>(blockIdx.y) * ((total + 127) / 128) + (r0 >> 7) + half) * kv4_row_tile_bytes(D);
+      tile_out = p.row_tiles + (static_cast<size_t>(bh) * ((total + 127) / 128) + (r0 >> 7) + half) * kv4_row_tile_bytes(D);
     // Q: scaled so that the largest value lies in [2^8, 2^9), which leaves the values divided by 16 their bits
     float unit, sum = 0.f;
     {
-      const uint16_t *src = p.q + out_at;
+      uint4 raw[D / 8];
       float top = 0.f;
-#pragma unroll 4
+#pragma unroll
       for (int c = 0; c < D / 8; ++c) {
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (live) raw = *reinterpret_cast<const uint4 *>(src + 8 * c);
-        const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+        raw[c] = make_uint4(0, 0, 0, 0);
+        if (live) raw[c] = *reinterpret_cast<const uint4 *>(p.q + out_at + 8 * c);
+      }
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           top = fmaxf(top, fmaxf(fabsf(kv4_to_f<T>(static_cast<uint16_t>(u[i]))), fabsf(kv4_to_f<T>(static_cast<uint16_t>(u[i] >> 16)))));
       }
       const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 16), 253);
       const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * (p.scale_log2 < 0.f ? -256.f : 256.f);
-      unit = __uint_as_float(static_cast<uint32_t>(e) << 23) * (fabsf(p.scale_log2) * 65536.f);  // 2^24 / 2^8
+      // 2^24 / 2^8; never 0
+      unit = fmaxf(__uint_as_float(static_cast<uint32_t>(e) << 23) * (fabsf(p.scale_log2) * 65536.f), FLT_MIN);
       const uint32_t dst = base + Plan::q + half * Plan::q_bytes + (quad * 32 + lane) * 16;
-#pragma unroll 4
+#pragma unroll
       for (int c = 0; c < D / 8; ++c) {
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (live) raw = *reinterpret_cast<const uint4 *>(src + 8 * c);
-        const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+        const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
         uint32_t x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -300,7 +399,26 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
 
     const uint32_t t_s = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * 128;
     const uint32_t t_o = tmem + (static_cast<uint32_t>(quad * 32) << 16) + 256 + half * D;
-    PromptRow r = {unit, sum, -INFINITY, 0.f, 0, 0};
+    // from here on a lane has four rows: their numbers go through shared memory
+    const uint32_t warp_rows = base + Plan::rows + warp * 32 * 12, my_row = warp_rows + lane * 12;
+    sts_f32(my_row, unit);
+    sts_f32(my_row + 4, sum);
+    __syncwarp();
+    PromptRows r;
+    int row_pos[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int row_of = (lane >> 2) + 8 * k;
+      const float row_unit = lds_f32(warp_rows + row_of * 12), row_sum = lds_f32(warp_rows + row_of * 12 + 4);
+      r.unit2[k] = pack2(row_unit, row_unit);
+      r.sum2[k] = pack2(row_sum, row_sum);
+      r.shift2[k] = r.l2[k] = r.fix2[k] = 0;
+      const int of = r0 + warp * 32 + row_of;
+      row_pos[k] = of < total ? length - p.seq + of / p.group : -1;
+      r.m[k] = row_pos[k] < 0 ? 0.f : -INFINITY;  // rows that never see anything are not waited for
+    }
+    r.unset = true;
+    r.v_unit = 0.f;
     for (int t = 0; t < tiles; ++t) {
       const int stage = t & 1;
       if (!mbar_wait_chain(base + kPrBarS + 8 * half, t & 1) || !mbar_wait_chain(base + kPrBarVFull + 8 * stage, (t >> 1) & 1)) {
@@ -312,25 +430,45 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
       const float unit_now = lds_f32(base + kPrUnit + 4 * stage);
       const int j0 = range.block(t) * kPrTile;
       const bool whole = j0 + kPrTile - 1 <= wg_lo && (p.window == 0 || j0 > wg_hi - p.window || j0 + kPrTile <= p.sinks);
-      const int hi = pos - j0, lo = p.window > 0 ? hi - p.window : -1, sk = p.sinks - j0;
+      int hi[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) hi[k] = row_pos[k] - j0;
       if (whole)
-        prompt_tile<true, D>(r, t_s, t_o, par, unit_now, t > 0, hi, lo, sk);
+        prompt_tile<true, D>(r, t_s, t_o, par, unit_now, t > 0, hi, p.window, p.sinks - j0);
       else
-        prompt_tile<false, D>(r, t_s, t_o, par, unit_now, t > 0, hi, lo, sk);
+        prompt_tile<false, D>(r, t_s, t_o, par, unit_now, t > 0, hi, p.window, p.sinks - j0);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(base + kPrBarP + 8 * half);
     }
+    // and back to a thread per row
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float l0, l1, f0, f1;
+      unpack2(r.l2[k], l0, l1);
+      unpack2(r.fix2[k], f0, f1);
+      float l = l0 + l1, f = f0 + f1;
+#pragma unroll
+      for (int off = 1; off <= 2; off <<= 1) {
+        l += __shfl_xor_sync(0xffffffffu, l, off);
+        f += __shfl_xor_sync(0xffffffffu, f, off);
+      }
+      if ((lane & 3) == 0) {
+        const uint32_t at = warp_rows + ((lane >> 2) + 8 * k) * 12;
+        sts_f32(at, l);
+        sts_f32(at + 4, f);
+        sts_f32(at + 8, r.m[k]);
+      }
+    }
+    __syncwarp();
     if (!failed && tiles > 0 && !mbar_wait_chain(base + kPrBarEnd, 0)) failed = true;
     if (failed) {
       report_status(kStatusMmaTimeout);
     } else {
       tc_fence_after();
-      float l0, l1, f0, f1;
-      unpack2(r.l2, l0, l1);
-      unpack2(r.fix2, f0, f1);
-      const float l = l0 + l1, fix = f0 + f1, inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
+      const float l = lds_f32(my_row), fix = lds_f32(my_row + 4), inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
       // column i D/4 + u of the accumulator is channel 4 u + i
       constexpr int U = D / 4;
 #pragma unroll
@@ -360,37 +498,42 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
         float *numbers = reinterpret_cast<float *>(tile_out + 128 * D * 2) + quad * 32 + lane;
         numbers[0] = unit;
         numbers[128] = sum * unit;
-        numbers[256] = !live || l == 0.f ? INFINITY : r.m + log2f(l);
+        numbers[256] = !live || l == 0.f ? INFINITY : lds_f32(my_row + 8) + log2f(l);
       }
     }
   } else if (warp < kMma) {
     // ------------------------------------------------------------------ producers
     const int pw = warp - kProducer, tid = threadIdx.x - kProducer * 32;
-    constexpr int KW = D / 8;            // words of a K row, one per thread
+    constexpr int kThreads = kPrProducers * 32, E = kPrTile / kThreads;  // entries of a thread: tid, tid + kThreads, ..
+    constexpr int KW = D / 8;            // words of a K row
     constexpr int U = D / 4;             // units of a V pair
     constexpr int G = 32 / U;            // groups of 8 entries that a warp takes at once
-    constexpr int VP = 16 / (4 * G);     // passes over the 16 groups of a tile
-    uint32_t kw[KW], vw[VP][4];
-    uint2 par = make_uint2(0, 0);
+    constexpr int VP = 16 / (kPrProducers * G);  // passes over the 16 groups of a tile
+    uint32_t kw[E][KW], vw[VP][4];
+    uint2 par[E];
     const int unit_lane = lane & (U - 1), group0 = G * pw + (G == 2 ? lane >> 4 : 0);
     auto load = [&](int t) {
       const int j0 = range.block(t) * kPrTile;
-      const bool there = j0 + tid < p.cache.capacity;
-      const uint8_t *kr = p.cache.k + (first + j0 + (there ? tid : 0)) * (D / 2);
 #pragma unroll
-      for (int i = 0; i < KW; i += 4) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (there) x = *reinterpret_cast<const uint4 *>(kr + 4 * i);
-        kw[i] = x.x, kw[i + 1] = x.y, kw[i + 2] = x.z, kw[i + 3] = x.w;
+      for (int n = 0; n < E; ++n) {
+        const int j = j0 + tid + n * kThreads;
+        const bool there = j < p.cache.capacity;
+        const uint8_t *kr = p.cache.k + (first + (there ? j : j0)) * (D / 2);
+#pragma unroll
+        for (int i = 0; i < KW; i += 4) {
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (there) x = *reinterpret_cast<const uint4 *>(kr + 4 * i);
+          kw[n][i] = x.x, kw[n][i + 1] = x.y, kw[n][i + 2] = x.z, kw[n][i + 3] = x.w;
+        }
+        // entries that no row sees may hold anything: their scales and minima are taken as zero
+        par[n] = make_uint2(0, 0);
+        if (j <= min(pos_hi, p.cache.capacity - 1)) par[n] = *reinterpret_cast<const uint2 *>(p.cache.params + (first + j) * 4);
       }
-      // entries that no row sees may hold anything: their scales and minima are taken as zero
-      par = make_uint2(0, 0);
-      if (j0 + tid <= min(pos_hi, p.cache.capacity - 1)) par = *reinterpret_cast<const uint2 *>(p.cache.params + (first + j0 + tid) * 4);
 #pragma unroll
       for (int v = 0; v < VP; ++v)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int pair = (j0 >> 1) + 4 * (group0 + 4 * G * v) + i;
+          const int pair = (j0 >> 1) + 4 * (group0 + kPrProducers * G * v) + i;
           vw[v][i] = 0;
           if (2 * pair < p.cache.capacity) vw[v][i] = *reinterpret_cast<const uint32_t *>(p.cache.v + ((first >> 1) + pair) * D + 4 * unit_lane);
         }
@@ -403,35 +546,45 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
       // a warp that gives up goes on through the named barriers, which the others wait at, but hands nothing on
       if (!failed && !mbar_wait_chain(base + kPrBarEmpty + 8 * stage, ((t >> 1) & 1) ^ 1)) failed = true;
       const uint32_t k_at = base + Plan::stages + stage * 2 * Plan::k_bytes, v_at = k_at + Plan::k_bytes;
+      float mine = 0.f;
 #pragma unroll
-      for (int i = 0; i < KW; ++i) {
-        const uint32_t x = kw[i], y = x >> 8;
-        sts_v4(k_at + i * kChunkQ + tid * 16, x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u);
+      for (int n = 0; n < E; ++n) {
+#pragma unroll
+        for (int i = 0; i < KW; ++i) {
+          const uint32_t x = kw[n][i], y = x >> 8;
+          sts_v4(k_at + i * kChunkQ + (tid + n * kThreads) * 16, x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u);
+        }
+        const float vs = fabsf(kv4_to_f<T>(static_cast<uint16_t>(par[n].y)));
+        if (vs <= FLT_MAX) mine = fmaxf(mine, vs);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0 && !failed) mbar_arrive(base + kPrBarKFull + 8 * stage);
       // the unit of P: a power of two within a factor of 16 of the tile's largest v_scale, or larger
-      const float ks = kv4_to_f<T>(static_cast<uint16_t>(par.x)), kl = kv4_to_f<T>(static_cast<uint16_t>(par.x >> 16));
-      const float vs = kv4_to_f<T>(static_cast<uint16_t>(par.y)), vl = kv4_to_f<T>(static_cast<uint16_t>(par.y >> 16));
-      const float mine = fabsf(vs) <= FLT_MAX ? fabsf(vs) : 0.f;
       const uint32_t top_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(mine));
       if (lane == 0) sts_f32(base + kPrMax + 4 * pw, __uint_as_float(top_bits));
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
       float top = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, lds_f32(base + kPrMax + 4 * i));
+      for (int i = 0; i < kPrProducers; ++i) top = fmaxf(top, lds_f32(base + kPrMax + 4 * i));
       if (top > 16.f * v_unit) v_unit = __uint_as_float(static_cast<uint32_t>(min(max(static_cast<int>(__float_as_uint(top) >> 23), 27), 250)) << 23);
       const float v_per = __uint_as_float(static_cast<uint32_t>(254 - (__float_as_uint(v_unit) >> 23)) << 23);
-      const uint32_t at = base + Plan::params + stage * Plan::param_bytes + tid * 4;
-      sts_f32(at, ks);
-      sts_f32(at + kPrTile * 4, kl);
-      sts_f32(at + 2 * kPrTile * 4, vs * v_per);
-      sts_f32(at + 3 * kPrTile * 4, fmaf(8.f, vs, vl));
+#pragma unroll
+      for (int n = 0; n < E; ++n) {
+        const float ks = kv4_to_f<T>(static_cast<uint16_t>(par[n].x)), kl = kv4_to_f<T>(static_cast<uint16_t>(par[n].x >> 16));
+        const float vs = kv4_to_f<T>(static_cast<uint16_t>(par[n].y)), vl = kv4_to_f<T>(static_cast<uint16_t>(par[n].y >> 16));
+        // of two neighbours side by side: scales, minima, scales of V in this unit, centres of V
+        const int j = tid + n * kThreads;
+        const uint32_t at = base + Plan::params + stage * Plan::param_bytes + (j >> 1) * 32 + (j & 1) * 4;
+        sts_f32(at, ks);
+        sts_f32(at + 8, kl);
+        sts_f32(at + 16, vs * v_per);
+        sts_f32(at + 24, fmaf(8.f, vs, vl));
+      }
       if (tid == 0) sts_f32(base + kPrUnit + 4 * stage, v_unit);
 #pragma unroll
       for (int v = 0; v < VP; ++v) {
-        const uint32_t dst = v_at + (group0 + 4 * G * v) * kChunkV + unit_lane * 16;
+        const uint32_t dst = v_at + (group0 + kPrProducers * G * v) * kChunkV + unit_lane * 16;
         const uint32_t *w = vw[v];
         sts_v4(dst, centre.lower(w[0]), centre.lower(w[1]), centre.lower(w[2]), centre.lower(w[3]));
         sts_v4(dst + U * 16, centre.upper(w[0]), centre.upper(w[1]), centre.upper(w[2]), centre.upper(w[3]));
@@ -442,7 +595,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
       __syncwarp();
       if (lane == 0 && !failed) mbar_arrive(base + kPrBarVFull + 8 * stage);
       if (t + 1 < tiles) load(t + 1);
-      asm volatile("bar.sync 1, 128;" ::: "memory");  // the maxima have been read
+      asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");  // the maxima have been read
     }
     if (failed) report_status(kStatusWeightCopyTimeout);
   } else {
@@ -709,7 +862,7 @@ template <typename T, int D> int launch_prompt(const Kv4AttentionParams &p, bool
   const int st = opt_in.ensure(kv4_prompt_kernel<T, D>, smem);
   if (st != MG_OK) return st;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.seq * p.group + kPrRows - 1) / kPrRows, p.cache.batch * p.cache.kv_heads);
+  cfg.gridDim = dim3(p.cache.batch * p.cache.kv_heads, (p.seq * p.group + kPrRows - 1) / kPrRows);
   cfg.blockDim = dim3(kPrWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
