@@ -27,12 +27,12 @@ namespace mg {
 
 MG_DEFINE_STATUS_ACCESSOR(kv4_prompt_device_status)
 
-constexpr int kPrRows = 256, kPrTile = 128;   // rows of a CTA, entries of a tile
+constexpr int kPrRows = 256, kPrTile = 128, kPrStep = 64;  // rows of a CTA, entries of a tile and of a step of softmax
 constexpr int kPrProducers = 2;
 constexpr int kPrWarps = 12;                  // 8 of softmax, the producers, 1 that issues (1 idle: registers are dealt out to four warps)
 // Shared memory: barriers, Q, two stages of K, V and params.
-constexpr int kPrBarKFull = 0, kPrBarVFull = 16, kPrBarEmpty = 32, kPrBarS = 48, kPrBarP = 64, kPrBarQ = 80, kPrBarEnd = 88, kPrTmemSlot = 96,
-              kPrUnit = 104 /* unit of P of each stage */, kPrMax = 112 /* the producers' maxima */;
+constexpr int kPrBarKFull = 0, kPrBarVFull = 16, kPrBarEmpty = 32, kPrBarS = 48, kPrBarP = 80, kPrBarO = 112, kPrBarQ = 128, kPrBarEnd = 136,
+              kPrTmemSlot = 144, kPrUnit = 152 /* unit of P of each stage */, kPrMax = 160 /* the producers' maxima */;
 template <int D> struct PromptPlan {
   static constexpr int q = 1024, q_bytes = 128 * D * 2;                    // per half
   static constexpr int stages = q + 2 * q_bytes, k_bytes = kPrTile * D * 2;  // K and V have the same size
@@ -130,11 +130,11 @@ __device__ __forceinline__ void prompt_scores(uint64_t (&score)[4], const uint32
   }
 }
 
-// Raises the rows' maxima to those of a tile's entries 32 c .. + 31, and brings what was summed up so far into the new units: the lane's
-// sums, the accumulator where it has been started, P of the tile's entries before these.
+// Raises the rows' maxima to those of a step's entries 32 c .. + 31, and brings what was summed up so far into the new units: the lane's
+// sums, the accumulator, P of the step's entries before these.  False where the accumulator's last product did not end in time.
 template <bool WHOLE, int D>
-__device__ __forceinline__ void prompt_raise(PromptRows &r, const uint32_t (&seen)[4], uint32_t at, uint32_t t_s, uint32_t t_o, float unit_now,
-                                             bool started, int c) {
+__device__ __forceinline__ bool prompt_raise(PromptRows &r, const uint32_t (&seen)[4], uint32_t at, uint32_t t_s, uint32_t t_o, float unit_now,
+                                             uint32_t bar_o, int step, int c) {
   constexpr uint32_t kLanes16 = 16u << 16;
   float f[4], top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
   {
@@ -175,8 +175,9 @@ __device__ __forceinline__ void prompt_raise(PromptRows &r, const uint32_t (&see
   }
   r.unset = __any_sync(0xffffffffu, unset);
   tmem_wait_st();
-  if (started) {
-    // the accumulator is at rest: S of this tile was asked for after P V of the last one
+  if (step > 0) {
+    if (!mbar_wait_chain(bar_o, (step - 1) & 1)) return false;  // P V of the last step
+    tc_fence_after();
     const float unit_change = r.v_unit / unit_now;  // powers of two
 #pragma unroll 1
     for (int half = 0; half < 2; ++half)
@@ -190,7 +191,7 @@ __device__ __forceinline__ void prompt_raise(PromptRows &r, const uint32_t (&see
         tmem_st_16x32(t_o + half * kLanes16 + col, o);
       }
   }
-  // P of this tile: its unit is the tile's already
+  // P of this step: its unit is the tile's already
 #pragma unroll 1
   for (int half = 0; half < 2; ++half) {
     const __half2 f_low = __float2half2_rn(half ? f[2] : f[0]), f_high = __float2half2_rn(half ? f[3] : f[1]);
@@ -208,17 +209,18 @@ __device__ __forceinline__ void prompt_raise(PromptRows &r, const uint32_t (&see
     }
   }
   r.v_unit = unit_now;
+  return true;
 }
 
-// The warp's rows over a tile of 128 entries: S from tensor memory, P back over it.  Entry c of the tile is seen by row r when
-// c <= hi[r] and (c > lo[r] or c < sk); WHOLE: all are.  `started`: the accumulator at t_o holds something.
+// The warp's rows over a step's 64 entries: S from tensor memory, P back over it.  Entry c of these is seen by row r when
+// c <= hi[r] and (c > lo[r] or c < sk); WHOLE: all are.  False where a wait ran out.
 template <bool WHOLE, int D>
-__device__ __forceinline__ void prompt_tile(PromptRows &r, uint32_t t_s, uint32_t t_o, uint32_t par, float unit_now, bool started, const int (&hi)[4],
-                                            int window, int sk) {
+__device__ __forceinline__ bool prompt_step(PromptRows &r, uint32_t t_s, uint32_t t_o, uint32_t par, float unit_now, uint32_t bar_o, int step,
+                                            const int (&hi)[4], int window, int sk) {
   const int t = threadIdx.x & 3;
   constexpr uint32_t kLanes16 = 16u << 16;
 #pragma unroll 1
-  for (int c = 0; c < 4; ++c) {  // 32 entries
+  for (int c = 0; c < kPrStep / 32; ++c) {  // 32 entries
     const uint32_t at = par + (16 * c + t) * 32;
     uint32_t seen[4];
     if (!WHOLE) {
@@ -232,7 +234,7 @@ __device__ __forceinline__ void prompt_tile(PromptRows &r, uint32_t t_s, uint32_
     // weights of a row add up to more than 2^8 of what the maximum stands for.  (Looking for it every time took 1300 cycles of 4500:
     // no exponential could begin before the last score.)  Whole numbers keep the factors powers of two, which P in fp16 takes without
     // another rounding.
-    if (r.unset || r.v_unit != unit_now) prompt_raise<WHOLE, D>(r, seen, at, t_s, t_o, unit_now, started, c);
+    if ((r.unset || r.v_unit != unit_now) && !prompt_raise<WHOLE, D>(r, seen, at, t_s, t_o, unit_now, bar_o, step, c)) return false;
     uint32_t pv[2][8];
     uint64_t l_here[4], fix_here[4];
     for (int pass = 0;; ++pass) {
@@ -287,7 +289,7 @@ __device__ __forceinline__ void prompt_tile(PromptRows &r, uint32_t t_s, uint32_
         raise |= x + y > 256.f;
       }
       if (pass > 0 || !__any_sync(0xffffffffu, raise)) break;
-      prompt_raise<WHOLE, D>(r, seen, at, t_s, t_o, unit_now, started, c);
+      if (!prompt_raise<WHOLE, D>(r, seen, at, t_s, t_o, unit_now, bar_o, step, c)) return false;
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -297,6 +299,7 @@ __device__ __forceinline__ void prompt_tile(PromptRows &r, uint32_t t_s, uint32_
     tmem_st_16x16(t_s + 16 * c, pv[0]);
     tmem_st_16x16(t_s + kLanes16 + 16 * c, pv[1]);
   }
+  return true;
 }
 
 template <typename T, int D>
@@ -311,6 +314,9 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
       mbar_init(base + kPrBarKFull + 8 * lane, kPrProducers);
       mbar_init(base + kPrBarVFull + 8 * lane, kPrProducers);
       mbar_init(base + kPrBarEmpty + 8 * lane, 1);
+      mbar_init(base + kPrBarO + 8 * lane, 1);
+    }
+    if (lane < 4) {  // a half's even and odd steps: a warp may be a step ahead of the others
       mbar_init(base + kPrBarS + 8 * lane, 1);
       mbar_init(base + kPrBarP + 8 * lane, 4);
     }
@@ -338,7 +344,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
   // the tiles that the rows see: those of first entries, then those of the window
   const Kv4Range range = kv4_range<kPrTile>(pos_lo, pos_hi, p.window, p.sinks, p.cache.capacity);
   const int tiles = range.blocks;
-  constexpr uint32_t kIdescS = 128, kChunkQ = 128 * 16, kChunkV = D * 16;
+  constexpr uint32_t kChunkQ = 128 * 16, kChunkV = D * 16;
   bool failed = false;
 
   if (warp < kProducer) {
@@ -397,7 +403,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
     __syncwarp();
     if (lane == 0) mbar_arrive(base + kPrBarQ);
 
-    const uint32_t t_s = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * 128;
+    const uint32_t t_s0 = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * 128;
     const uint32_t t_o = tmem + (static_cast<uint32_t>(quad * 32) << 16) + 256 + half * D;
     // from here on a lane has four rows: their numbers go through shared memory
     const uint32_t warp_rows = base + Plan::rows + warp * 32 * 12, my_row = warp_rows + lane * 12;
@@ -419,28 +425,30 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
     }
     r.unset = true;
     r.v_unit = 0.f;
-    for (int t = 0; t < tiles; ++t) {
-      const int stage = t & 1;
-      if (!mbar_wait_chain(base + kPrBarS + 8 * half, t & 1) || !mbar_wait_chain(base + kPrBarVFull + 8 * stage, (t >> 1) & 1)) {
+    for (int u = 0; u < 2 * tiles; ++u) {  // 64 entries
+      const int t = u >> 1, stage = t & 1, buf = u & 1;
+      if (!mbar_wait_chain(base + kPrBarS + 16 * half + 8 * buf, (u >> 1) & 1) || (buf == 0 && !mbar_wait_chain(base + kPrBarVFull + 8 * stage, (t >> 1) & 1))) {
         failed = true;
         break;
       }
       tc_fence_after();
-      const uint32_t par = base + Plan::params + stage * Plan::param_bytes;
+      const uint32_t par = base + Plan::params + stage * Plan::param_bytes + buf * (kPrStep * 16);
       const float unit_now = lds_f32(base + kPrUnit + 4 * stage);
-      const int j0 = range.block(t) * kPrTile;
-      const bool whole = j0 + kPrTile - 1 <= wg_lo && (p.window == 0 || j0 > wg_hi - p.window || j0 + kPrTile <= p.sinks);
+      const int j0 = range.block(t) * kPrTile + buf * kPrStep;
+      const bool whole = j0 + kPrStep - 1 <= wg_lo && (p.window == 0 || j0 > wg_hi - p.window || j0 + kPrStep <= p.sinks);
       int hi[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) hi[k] = row_pos[k] - j0;
-      if (whole)
-        prompt_tile<true, D>(r, t_s, t_o, par, unit_now, t > 0, hi, p.window, p.sinks - j0);
-      else
-        prompt_tile<false, D>(r, t_s, t_o, par, unit_now, t > 0, hi, p.window, p.sinks - j0);
+      const uint32_t t_s = t_s0 + buf * kPrStep, bar_o = base + kPrBarO + 8 * half;
+      if (!(whole ? prompt_step<true, D>(r, t_s, t_o, par, unit_now, bar_o, u, hi, p.window, p.sinks - j0)
+                  : prompt_step<false, D>(r, t_s, t_o, par, unit_now, bar_o, u, hi, p.window, p.sinks - j0))) {
+        failed = true;
+        break;
+      }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(base + kPrBarP + 8 * half);
+      if (lane == 0) mbar_arrive(base + kPrBarP + 16 * half + 8 * buf);
     }
     // and back to a thread per row
     __syncwarp();
@@ -601,16 +609,18 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
   } else {
     if (warp == kMma) {
       // ---------------------------------------------------------------- MMAs
-      const uint32_t idesc_s = umma_instr_desc(0, kIdescS), idesc_o = umma_instr_desc(0, D);
+      const uint32_t idesc_s = umma_instr_desc(0, kPrStep), idesc_o = umma_instr_desc(0, D);
       const uint64_t dq = umma_smem_desc(base + Plan::q, kChunkQ, 128, 0);
       const uint64_t dk = umma_smem_desc(base + Plan::stages, kChunkQ, 128, 0);
       const uint64_t dv = umma_smem_desc(base + Plan::stages + Plan::k_bytes, kChunkV, 128, 0);
-      auto scores = [&](int half, int stage) {  // by one lane
+      // S of a step: two of them per half of the rows, so that the next one's is there when softmax is done with this one's
+      auto scores = [&](int half, int u) {  // by one lane
+        const int buf = u & 1, stage = (u >> 1) & 1;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          umma_f16(tmem + half * 128, dq + half * (Plan::q_bytes >> 4) + k * (2 * kChunkQ >> 4),
-                   dk + stage * (2 * Plan::k_bytes >> 4) + k * (2 * kChunkQ >> 4), idesc_s, k > 0);
-        umma_commit(base + kPrBarS + 8 * half);
+          umma_f16(tmem + half * 128 + buf * kPrStep, dq + half * (Plan::q_bytes >> 4) + k * (2 * kChunkQ >> 4),
+                   dk + stage * (2 * Plan::k_bytes >> 4) + buf * kPrStep + k * (2 * kChunkQ >> 4), idesc_s, k > 0);
+        umma_commit(base + kPrBarS + 16 * half + 8 * buf);
       };
       if (tiles > 0) {
         if (!mbar_wait_chain(base + kPrBarQ, 0) || !mbar_wait_chain(base + kPrBarKFull, 0)) failed = true;
@@ -618,29 +628,33 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
         if (!failed && elect_one()) {
           scores(0, 0);
           scores(1, 0);
+          scores(0, 1);
+          scores(1, 1);
         }
         __syncwarp();
       }
-      for (int t = 0; t < tiles && !failed; ++t) {
-        const int stage = t & 1, next = stage ^ 1;
-        if (!mbar_wait_chain(base + kPrBarVFull + 8 * stage, (t >> 1) & 1)) {
+      for (int u = 0; u < 2 * tiles && !failed; ++u) {
+        const int t = u >> 1, stage = t & 1, buf = u & 1;
+        const bool more = u + 2 < 2 * tiles;
+        if (buf == 0 && (!mbar_wait_chain(base + kPrBarVFull + 8 * stage, (t >> 1) & 1) ||
+                         (more && !mbar_wait_chain(base + kPrBarKFull + 8 * (stage ^ 1), ((t + 1) >> 1) & 1)))) {
           failed = true;
           break;
         }
         for (int half = 0; half < 2; ++half) {
-          if (!mbar_wait_chain(base + kPrBarP + 8 * half, t & 1) ||
-              (half == 0 && t + 1 < tiles && !mbar_wait_chain(base + kPrBarKFull + 8 * next, ((t + 1) >> 1) & 1))) {
+          if (!mbar_wait_chain(base + kPrBarP + 16 * half + 8 * buf, (u >> 1) & 1)) {
             failed = true;
             break;
           }
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < kPrTile / 16; ++k)
-              mma_ts(tmem + 256 + half * D, tmem + half * 128 + k * 8, dv + stage * (2 * Plan::k_bytes >> 4) + k * (2 * kChunkV >> 4), idesc_o,
-                     (t > 0 || k > 0) ? 1u : 0u);
-            if (half == 1) umma_commit(base + kPrBarEmpty + 8 * stage);
-            if (t + 1 < tiles) scores(half, next);
+            for (int k = 0; k < kPrStep / 16; ++k)
+              mma_ts(tmem + 256 + half * D, tmem + half * 128 + buf * kPrStep + k * 8,
+                     dv + stage * (2 * Plan::k_bytes >> 4) + (buf * (kPrStep / 16) + k) * (2 * kChunkV >> 4), idesc_o, (u > 0 || k > 0) ? 1u : 0u);
+            umma_commit(base + kPrBarO + 8 * half);
+            if (half == 1 && buf == 1) umma_commit(base + kPrBarEmpty + 8 * stage);
+            if (more) scores(half, u + 2);
           }
           __syncwarp();
         }
