@@ -406,7 +406,8 @@ std::tuple<Tensor, Tensor> dequantize_kv4(const Tensor &k_codes, const Tensor &v
   TORCH_CHECK(count >= 0, "dequantize_kv4: count must not be negative");
   const c10::Device dev = k_codes.device();
   const c10::cuda::CUDAGuard on_device(dev);
-  Tensor k = empty_on({cache.batch, cache.n_kv_heads, count, cache.head_dim}, type_of(flags), dev), v = at::empty_like(k);
+  Tensor k = empty_on({cache.batch, cache.n_kv_heads, count, cache.head_dim}, type_of(flags), dev),
+         v = empty_on({cache.batch, cache.n_kv_heads, count, cache.head_dim}, type_of(flags), dev);
   if (k.numel() == 0) return {k, v};
   check_status(lib.dequantize_kv4(&cache, lengths.const_data_ptr<int32_t>(), count, k.data_ptr(), v.data_ptr(), static_cast<uint32_t>(flags),
                                   stream_of(dev)),
@@ -662,6 +663,101 @@ PyObject *py_matmul_raw(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the 4-bit cache without the dispatcher -----------------------------------------------------------------------
+// append_kv4(...), attention_kv4(...), evict_kv4(...), dequantize_kv4(...) with the operators' arguments: None when the call has to go
+// through the dispatcher, which is so as well where a derivative is asked for.
+bool plain_tensors(PyObject *const *args, std::initializer_list<int> which) {
+  for (const int i : which) {
+    if (!plain_cuda(args[i])) return false;
+    const Tensor &t = THPVariable_Unpack(args[i]);
+    if ((at::GradMode::is_enabled() && t.requires_grad()) || torch::autograd::isFwGradDefined(t)) return false;
+  }
+  return dispatcher_not_needed();
+}
+
+void count_writes(PyObject *const *args, std::initializer_list<int> which) {
+  for (const int i : which) {
+    const Tensor &t = THPVariable_Unpack(args[i]);
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  }
+}
+
+PyObject *two(Tensor a, Tensor b) {
+  PyObject *pa = THPVariable_Wrap(std::move(a)), *pb = THPVariable_Wrap(std::move(b));
+  PyObject *both = pa && pb ? PyTuple_Pack(2, pa, pb) : nullptr;
+  Py_XDECREF(pa);
+  Py_XDECREF(pb);
+  return both;
+}
+
+PyObject *py_append_kv4(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  int64_t v[2];  // n_heads, flags
+  if (nargs != 10 || !plain_tensors(args, {0, 1, 2, 3, 4, 5, 6, 7}) || !as_ints(args + 8, 2, v)) Py_RETURN_NONE;
+  RECORD_FUNCTION("matgptq_cuda::append_kv4", std::vector<c10::IValue>());
+  Tensor q;
+  {
+    const WithoutGil released;
+    const at::AutoDispatchBelowADInplaceOrView below;
+    q = append_kv4(THPVariable_Unpack(args[0]), THPVariable_Unpack(args[1]), THPVariable_Unpack(args[2]), THPVariable_Unpack(args[3]),
+                   THPVariable_Unpack(args[4]), THPVariable_Unpack(args[5]), THPVariable_Unpack(args[6]), THPVariable_Unpack(args[7]), v[0], v[1]);
+  }
+  count_writes(args, {5, 6, 7});
+  return THPVariable_Wrap(std::move(q));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject *py_attention_kv4(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  int64_t v[2], flags;  // window, sinks
+  if (nargs != 10 || !plain_tensors(args, {0, 1, 2, 3, 4}) || !as_ints(args + 5, 2, v) || !PyFloat_Check(args[7]) || !as_ints(args + 8, 1, &flags) ||
+      (args[9] != Py_None && !plain_tensors(args, {9})))
+    Py_RETURN_NONE;
+  RECORD_FUNCTION("matgptq_cuda::attention_kv4", std::vector<c10::IValue>());
+  const double scale = PyFloat_AS_DOUBLE(args[7]);
+  const std::optional<Tensor> weights = args[9] == Py_None ? std::nullopt : std::optional<Tensor>(THPVariable_Unpack(args[9]));
+  Tensor out;
+  {
+    const WithoutGil released;
+    const at::AutoDispatchBelowADInplaceOrView below;
+    out = attention_kv4(THPVariable_Unpack(args[0]), THPVariable_Unpack(args[1]), THPVariable_Unpack(args[2]), THPVariable_Unpack(args[3]),
+                        THPVariable_Unpack(args[4]), v[0], v[1], scale, flags, weights);
+  }
+  if (weights) count_writes(args, {9});
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject *py_evict_kv4(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  int64_t v[5];  // keep, slack, sinks, recent, flags
+  if (nargs != 10 || !plain_tensors(args, {0, 1, 2, 3, 4}) || !as_ints(args + 5, 5, v)) Py_RETURN_NONE;
+  RECORD_FUNCTION("matgptq_cuda::evict_kv4", std::vector<c10::IValue>());
+  std::tuple<Tensor, Tensor> both;
+  {
+    const WithoutGil released;
+    both = evict_kv4(THPVariable_Unpack(args[0]), THPVariable_Unpack(args[1]), THPVariable_Unpack(args[2]), THPVariable_Unpack(args[3]),
+                     THPVariable_Unpack(args[4]), v[0], v[1], v[2], v[3], v[4]);
+  }
+  count_writes(args, {0, 1, 2, 3});
+  return two(std::move(std::get<0>(both)), std::move(std::get<1>(both)));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject *py_dequantize_kv4(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  int64_t v[2];  // count, flags
+  if (nargs != 6 || !plain_tensors(args, {0, 1, 2, 3}) || !as_ints(args + 4, 2, v)) Py_RETURN_NONE;
+  RECORD_FUNCTION("matgptq_cuda::dequantize_kv4", std::vector<c10::IValue>());
+  std::tuple<Tensor, Tensor> both;
+  {
+    const WithoutGil released;
+    both = dequantize_kv4(THPVariable_Unpack(args[0]), THPVariable_Unpack(args[1]), THPVariable_Unpack(args[2]), THPVariable_Unpack(args[3]), v[0], v[1]);
+  }
+  return two(std::move(std::get<0>(both)), std::move(std::get<1>(both)));
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(path): the C-ABI library that the operators call (already loaded by the caller; its handle is kept)
 PyObject *py_bind(PyObject *, PyObject *path) {
   HANDLE_TH_ERRORS
@@ -695,6 +791,10 @@ PyMethodDef methods[] = {
     {"linear_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_forward)), METH_FASTCALL, nullptr},
     {"grouped_raw", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_grouped_raw)), METH_FASTCALL, nullptr},
     {"matmul_raw", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_matmul_raw)), METH_FASTCALL, nullptr},
+    {"append_kv4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_append_kv4)), METH_FASTCALL, nullptr},
+    {"attention_kv4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_attention_kv4)), METH_FASTCALL, nullptr},
+    {"evict_kv4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_evict_kv4)), METH_FASTCALL, nullptr},
+    {"dequantize_kv4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_dequantize_kv4)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

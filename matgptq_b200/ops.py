@@ -177,6 +177,10 @@ def append_kv4(qkv: torch.Tensor, positions: torch.Tensor, cos_table: torch.Tens
     cache (layout: ``include/matgptq_b200.h``); ``lengths`` int32 ``[B]`` counts the entries of each sequence with the new ones: token
     ``i`` becomes entry ``lengths[b] - S + i``, and is padding where that is negative.  ``positions`` int64 ``[S]`` or ``[B, S]`` select the
     rows of the fp32 tables ``[positions, d/2]``; pairs of channels are ``(2i, 2i + 1)``."""
+    if not torch.compiler.is_compiling():  # straight to the kernel, where nothing wants to see the operator (as MatGPTQLinear.forward)
+        done = _ext.append_kv4(qkv, positions, cos_table, sin_table, lengths, k_codes, v_codes, params, n_heads, feature_flag)
+        if done is not None:
+            return done
     return _ops.append_kv4(qkv, positions, cos_table, sin_table, lengths, k_codes, v_codes, params, n_heads, feature_flag)
 
 
@@ -191,6 +195,10 @@ def attention_kv4(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
     ``S`` entries.  Query ``i`` is entry ``p = lengths[b] - S + i`` and sees entry ``j`` when ``j <= p`` and (``window == 0``, or
     ``j > p - window``, or ``j < sinks``); one that sees nothing gives zeros.  ``weights`` fp32 ``[B, KV, capacity]``: the softmax weights of
     each entry, summed over the queries and heads that share it, are added to it."""
+    if not torch.compiler.is_compiling():  # straight to the kernel, where nothing wants to see the operator (as MatGPTQLinear.forward)
+        done = _ext.attention_kv4(q, k_codes, v_codes, params, lengths, window, sinks, scale, feature_flag, weights)
+        if done is not None:
+            return done
     return _ops.attention_kv4(q, k_codes, v_codes, params, lengths, window, sinks, scale, feature_flag, weights)
 
 
@@ -204,6 +212,10 @@ def evict_kv4(k_codes: torch.Tensor, v_codes: torch.Tensor, params: torch.Tensor
     """Addition: cuts every sequence of more than ``keep + slack`` entries back to ``keep``, in place: the first ``sinks``, the last
     ``recent``, and of the others, head by head, those with the largest ``weights`` (ties: the lowest entry).  Returns the new lengths
     int32 ``[B]`` and the old indices of the entries that stayed, int32 ``[B, KV, keep]`` (-1 where a sequence was not cut)."""
+    if not torch.compiler.is_compiling():  # straight to the kernel, where nothing wants to see the operator (as MatGPTQLinear.forward)
+        done = _ext.evict_kv4(k_codes, v_codes, params, weights, lengths, keep, slack, sinks, recent, feature_flag)
+        if done is not None:
+            return done
     return _ops.evict_kv4(k_codes, v_codes, params, weights, lengths, keep, slack, sinks, recent, feature_flag)
 
 
@@ -216,6 +228,10 @@ def dequantize_kv4(k_codes: torch.Tensor, v_codes: torch.Tensor, params: torch.T
                    feature_flag: int) -> tuple[torch.Tensor, torch.Tensor]:
     """Addition: the last ``count`` entries of every sequence as dense K and V ``[B, KV, count, d]``, zeros in front where a sequence
     has fewer."""
+    if not torch.compiler.is_compiling():  # straight to the kernel, where nothing wants to see the operator (as MatGPTQLinear.forward)
+        done = _ext.dequantize_kv4(k_codes, v_codes, params, lengths, count, feature_flag)
+        if done is not None:
+            return done
     return _ops.dequantize_kv4(k_codes, v_codes, params, lengths, count, feature_flag)
 
 
