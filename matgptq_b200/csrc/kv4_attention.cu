@@ -198,7 +198,7 @@ template <int R> __device__ __forceinline__ bool step_find(StepPiece &s, const K
     return true;
   }
   // The smallest share (about) that leaves no more pieces than run at once; with more segments than that, the mean work of a CTA.  (A
-  // few pieces more are a second round for all: 64 heads of 4096 entries in 5 pieces each, 24.0 us, in 4 17.6.)
+  // few pieces more are a second round for all: 64 heads of 4096 entries in 5 pieces each, 24.0 us, in 4 19.5.)
   const auto sum = [&](auto of) {
     int x = 0;
     for (int b0 = 0; b0 < batch; b0 += 32) {
@@ -376,14 +376,15 @@ __device__ __forceinline__ void step_block(StepSums<D, NT> &a, const Kv4Rows<D> 
 // One warp per 32 entries at a time: the warps of a CTA share out its part of a segment, each keeps a running maximum of its own.  A
 // warp's next blocks are on their way into its ring of stages while it works on one; a block is 32 x (D + 8) bytes in three places.
 // (With a bulk copy for each of the three a SM took in no more than 11 bytes a cycle, one copy in 130 cycles; cp.async has no such limit.)
-template <typename T, int D, int NT>
+// WEIGHS: a CTA has a segment as a whole and adds its entries' weights up as well.
+template <typename T, int D, int NT, bool WEIGHS>
 __global__ void __launch_bounds__(kStepWarps * 32, NT == 1 ? 2 : 1) kv4_step_kernel(const Kv4StepParams sp) {
   pdl_prologue();
   const Kv4AttentionParams &p = sp.a;
   constexpr int R = 8 * NT, W = D / 32;
   using Stage = StepStage<D>;
   extern __shared__ __align__(128) unsigned char step_smem[];
-  __shared__ float part_m[kStepWarps][R], part_l[kStepWarps][R];
+  __shared__ float part_m[kStepWarps][R], part_l[kStepWarps][R], part_lse[R];
   float *part = reinterpret_cast<float *>(step_smem);  // [warps][R][D], over the stages once these are done with
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -501,7 +502,8 @@ __global__ void __launch_bounds__(kStepWarps * 32, NT == 1 ? 2 : 1) kv4_step_ker
       sum.z = fmaf(x.z, f, sum.z);
       sum.w = fmaf(x.w, f, sum.w);
     }
-    if ((!complete || p.weights != nullptr) && i % (D / 4) == 0) {
+    if (WEIGHS && i % (D / 4) == 0) part_lse[r] = norm == 0.f ? INFINITY : top + log2f(norm);
+    if ((!complete || (!WEIGHS && p.weights != nullptr)) && i % (D / 4) == 0) {
       sp.ml[(static_cast<size_t>(slot) * 2) * R + r] = top;
       sp.ml[(static_cast<size_t>(slot) * 2 + 1) * R + r] = norm;
     }
@@ -517,20 +519,71 @@ __global__ void __launch_bounds__(kStepWarps * 32, NT == 1 ? 2 : 1) kv4_step_ker
       *reinterpret_cast<uint2 *>(p.out + at) = w;
     }
   }
+  if constexpr (WEIGHS) {
+    // The rows' sums are known: once more over the scores, from K's codes and params (out of L2), for each entry's share of them.
+    __syncthreads();
+    float lse[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) lse[n][k] = r0 + 8 * n + 2 * t + k < total ? part_lse[8 * n + 2 * t + k] : INFINITY;
+    constexpr int kAhead = 2;
+    for (int i0 = from; i0 < to; i0 += kAhead) {
+      uint32_t k0[kAhead][2][W], k1[kAhead][2][W], kp[kAhead][2][2];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        if (i0 + a >= to) continue;
+        const size_t e = first + static_cast<size_t>(range.block(i0 + a)) * kStepBlock;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          kv4_load_words(k0[a][u], p.cache.k + (e + 16 * u + g) * (D / 2) + t * (D / 8));
+          kv4_load_words(k1[a][u], p.cache.k + (e + 16 * u + 8 + g) * (D / 2) + t * (D / 8));
+          kp[a][u][0] = *reinterpret_cast<const uint32_t *>(p.cache.params + (e + 16 * u + g) * 4);
+          kp[a][u][1] = *reinterpret_cast<const uint32_t *>(p.cache.params + (e + 16 * u + 8 + g) * 4);
+        }
+      }
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        if (i0 + a >= to) continue;
+        const int j0 = range.block(i0 + a) * kStepBlock;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float sum[2] = {0.f, 0.f};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float s[4];
+            kv4_scores<T, D>(s, k0[a][u], k1[a][u], kp[a][u], rows[n]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (kv4_sees(rows[n].pos[e & 1], j0 + 16 * u + g + 8 * (e >> 1), p.window, p.sinks))
+                sum[e >> 1] += exp2_approx(fmaf(s[e], rows[n].unit[e & 1], -lse[n][e & 1]));
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
+            sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
+            const int j = j0 + 16 * u + g + 8 * e;
+            if (t == 0 && j < length) p.weights[first + j] += sum[e];
+          }
+        }
+      }
+    }
+  }
 }
 
 // What is left once every piece has been seen: joins the partial results of segments that were cut, and adds up the weights.
-// blockIdx.y: sequence and head; blockIdx.x: a part of a tile's results (256 numbers), and kFinishEntries entries whose weights are due.
+// blockIdx.y: sequence and head; blockIdx.x: a part of a tile's results (1024 / LANES numbers), and kFinishEntries
+// entries whose weights are due.
 // Every step is a round trip to memory, so what does not hang on another is asked for at once.
 constexpr int kFinishEach = 4, kFinishEntries = kStepWarps * 16 * kFinishEach;
 
-template <typename T, int D, int NT> __global__ void __launch_bounds__(kStepWarps * 32) kv4_finish_kernel(const Kv4StepParams sp) {
+template <typename T, int D, int NT, int LANES> __global__ void __launch_bounds__(kStepWarps * 32) kv4_finish_kernel(const Kv4StepParams sp) {
   pdl_prologue();
   const Kv4AttentionParams &p = sp.a;
-  constexpr int R = 8 * NT, kParts = R * D / 256;
+  constexpr int R = 8 * NT, kFours = kStepWarps * 32 / LANES, kParts = R * D / 4 / kFours;
   __shared__ float row_lse[kKv4FewRows];
-  __shared__ float4 quarter[3][64];
-  __shared__ float quarter_m[3][64], quarter_l[3][64];
+  __shared__ float4 other[LANES - 1][kFours];
+  __shared__ float other_m[LANES - 1][kFours], other_l[LANES - 1][kFours];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kv = p.cache.kv_heads, total = p.seq * p.group, b = blockIdx.y / kv, h = blockIdx.y - b * kv;
   const int part = blockIdx.x, tile = part / kParts;
@@ -557,8 +610,8 @@ template <typename T, int D, int NT> __global__ void __launch_bounds__(kStepWarp
     // a sequence without entries has no piece: its rows have not been written
     if (step_range<R>(p, length, tile).blocks == 0) pieces.y = 0;
     if (pieces.y != 1) {
-      // 64 times four numbers, four threads for each: every fourth partial result
-      const int i = (part - tile * kParts) * 64 + (threadIdx.x & 63), fourth = threadIdx.x >> 6, r = i / (D / 4), row = tile * R + r;
+      // four numbers a thread, LANES threads for each four: every LANES-th partial result
+      const int four = threadIdx.x % kFours, from = threadIdx.x / kFours, i = (part - tile * kParts) * kFours + four, r = i / (D / 4), row = tile * R + r;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
       float m = -INFINITY, l = 0.f;
       const auto add = [&](float m1, float l1, float4 x) {
@@ -572,14 +625,14 @@ template <typename T, int D, int NT> __global__ void __launch_bounds__(kStepWarp
         sum.w = fmaf(sum.w, f, x.w * f1);
       };
       constexpr int kAhead = 5;
-      for (int k = fourth; k < pieces.y; k += 4 * kAhead) {
+      for (int k = from; k < pieces.y; k += LANES * kAhead) {
         float4 x[kAhead];
         float m1[kAhead], l1[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-          const size_t slot = pieces.x + k + 4 * u;
+          const size_t slot = pieces.x + k + LANES * u;
           l1[u] = 0.f;
-          if (k + 4 * u < pieces.y) {
+          if (k + LANES * u < pieces.y) {
             m1[u] = sp.ml[slot * 2 * R + r];
             l1[u] = sp.ml[(slot * 2 + 1) * R + r];
             x[u] = *reinterpret_cast<const float4 *>(sp.partial + slot * R * D + 4 * i);
@@ -588,15 +641,15 @@ template <typename T, int D, int NT> __global__ void __launch_bounds__(kStepWarp
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) add(m1[u], l1[u], x[u]);
       }
-      if (fourth > 0) {
-        quarter[fourth - 1][threadIdx.x & 63] = sum;
-        quarter_m[fourth - 1][threadIdx.x & 63] = m;
-        quarter_l[fourth - 1][threadIdx.x & 63] = l;
+      if (from > 0) {
+        other[from - 1][four] = sum;
+        other_m[from - 1][four] = m;
+        other_l[from - 1][four] = l;
       }
       __syncthreads();
-      if (fourth == 0 && row < total) {
+      if (from == 0 && row < total) {
 #pragma unroll
-        for (int k = 0; k < 3; ++k) add(quarter_m[k][threadIdx.x], quarter_l[k][threadIdx.x], quarter[k][threadIdx.x]);
+        for (int k = 0; k < LANES - 1; ++k) add(other_m[k][four], other_l[k][four], other[k][four]);
         const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
         const int q = row / p.group;
         const size_t at = ((static_cast<size_t>(b) * p.seq + q) * p.heads + static_cast<size_t>(h) * p.group + (row - q * p.group)) * D + (i % (D / 4)) * 4;
@@ -666,7 +719,7 @@ namespace {
 
 struct StepPlan {
   int rows, tiles, segments;  // rows of a tile
-  bool whole;
+  bool whole, weighs;
   int64_t slots, pieces_bytes, ml_bytes, partial_bytes;
 };
 
@@ -682,7 +735,8 @@ StepPlan step_plan(const Kv4Cache &c, int seq, int group, int window, int sinks,
   // pieces of all segments: blocks / share and one for what is left over, each; shares are at least all blocks / kStepCtas
   s.slots = s.whole ? s.segments : s.segments + kStepCtas;
   s.pieces_bytes = s.whole ? 0 : (s.segments * 8 + 15) / 16 * 16;
-  s.ml_bytes = s.whole && !weights ? 0 : s.slots * 2 * s.rows * 4;
+  s.weighs = s.whole && s.tiles == 1;  // one CTA sees all rows and all entries
+  s.ml_bytes = s.whole && (!weights || s.weighs) ? 0 : s.slots * 2 * s.rows * 4;
   s.partial_bytes = s.whole ? 0 : s.slots * s.rows * c.dim * 4;
   return s;
 }
@@ -704,14 +758,20 @@ int launch_step(Kernel kernel, dim3 grid, int smem, cudaStream_t stream, bool pd
 
 template <typename T, int D, int NT> int kv4_step(const Kv4StepParams &p, const StepPlan &plan, cudaStream_t stream, bool pdl) {
   constexpr int ring = kStepWarps * kStepStages * StepStage<D>::bytes, part = kStepWarps * 8 * NT * D * 4, smem = ring > part ? ring : part;
-  static SharedMemoryOptIn opt_in;
-  int st = opt_in.ensure(kv4_step_kernel<T, D, NT>, smem);
+  const bool weighs = p.a.weights != nullptr && plan.weighs;
+  static SharedMemoryOptIn opt_in, opt_in_weighs;
+  int st = weighs ? opt_in_weighs.ensure(kv4_step_kernel<T, D, NT, true>, smem) : opt_in.ensure(kv4_step_kernel<T, D, NT, false>, smem);
   if (st != MG_OK) return st;
-  st = launch_step(kv4_step_kernel<T, D, NT>, dim3(static_cast<unsigned>(plan.slots)), smem, stream, pdl, p);
-  if (st != MG_OK || (plan.whole && p.a.weights == nullptr)) return st;
-  const int parts = plan.whole ? 1 : 8 * NT * D / 256 * plan.tiles;
+  const dim3 grid(static_cast<unsigned>(plan.slots));
+  st = weighs ? launch_step(kv4_step_kernel<T, D, NT, true>, grid, smem, stream, pdl, p) : launch_step(kv4_step_kernel<T, D, NT, false>, grid, smem, stream, pdl, p);
+  if (st != MG_OK || (plan.whole && (p.a.weights == nullptr || weighs))) return st;
   const int entries = p.a.weights != nullptr ? (p.a.cache.capacity + kFinishEntries - 1) / kFinishEntries : 1;
-  return launch_step(kv4_finish_kernel<T, D, NT>, dim3(std::max(parts, entries), p.a.cache.batch * p.a.cache.kv_heads), 0, stream, true, p);
+  const auto finish = [&](auto kernel, int lanes) {
+    const int parts = plan.whole ? 1 : 8 * NT * D * lanes / 1024 * plan.tiles;
+    return launch_step(kernel, dim3(std::max(parts, entries), p.a.cache.batch * p.a.cache.kv_heads), 0, stream, true, p);
+  };
+  // few segments have many pieces each: more threads for each number then
+  return plan.segments <= 4 ? finish(kv4_finish_kernel<T, D, NT, 16>, 16) : finish(kv4_finish_kernel<T, D, NT, 4>, 4);
 }
 
 template <typename T, int D> int kv4_step_rows(const Kv4StepParams &p, const StepPlan &plan, cudaStream_t stream, bool pdl) {
