@@ -132,6 +132,12 @@ __device__ __forceinline__ void kv4_scores(float (&s)[4], const uint32_t (&k0)[D
   }
 }
 
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -145,7 +151,8 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
 // ---- the work and who does it ---------------------------------------------------------------------------------------
 //
 // A segment is a tile of R = 8 or 16 rows of one key/value head of one sequence, its work the blocks of 32 entries that these rows
-// see.  Segments of few blocks get a CTA each.  Otherwise a segment is cut into pieces of equal size, none larger than a share that
+// see.  Segments of few blocks get a CTA each, or a cluster of CTAs as long as there are SMs for it, whose results are joined through
+// distributed shared memory.  Otherwise a segment is cut into pieces of equal size, none larger than a share that
 // makes at most `kStepCtas` pieces of all the work, where there are not more segments already; each piece is a CTA, leaves a partial result, and kv4_finish_kernel joins them in
 // their order.  Lengths are known on the device only: every CTA works out by itself which piece is its own, and the grid is as large as
 // the pieces can become.  (A CTA that goes on into the next segment, for shares that are all equal, has the latencies of a second
@@ -155,7 +162,7 @@ constexpr int kStepBlock = 32;       // entries of a block
 constexpr int kStepStages = 3;       // blocks in flight per warp
 constexpr int kStepCtas = 296;       // two on each SM of a B200
 constexpr int kStepLeast = kStepWarps;  // blocks of a share at least: one for each warp
-constexpr int kStepWhole = 64;          // blocks of a segment up to which it is not cut
+constexpr int kStepWhole = 64;          // blocks of a CTA up to which segments are not cut
 
 struct Kv4StepParams {
   Kv4AttentionParams a;
@@ -163,7 +170,7 @@ struct Kv4StepParams {
   float *ml;       // [slots][2][R]: maximum and sum of the partial result in a slot
   float *partial;  // [slots][R][D]
   int tiles;       // of rows
-  int whole;       // a CTA per segment
+  int cluster;     // CTAs of a segment that is not cut (1: no cluster); 0: segments are cut into pieces
 };
 
 template <int D> struct StepStage {
@@ -188,12 +195,13 @@ struct StepPiece {
 };
 template <int R> __device__ __forceinline__ bool step_find(StepPiece &s, const Kv4StepParams &p, int cta) {
   const int kv = p.a.cache.kv_heads, batch = p.a.cache.batch, lane = threadIdx.x & 31;
-  if (p.whole) {
-    s.b = cta / (p.tiles * kv);
-    s.tile = (cta - s.b * p.tiles * kv) / kv;
-    s.h = cta - (s.b * p.tiles + s.tile) * kv;
-    s.index = 0;
-    s.pieces = 1;
+  if (p.cluster > 0) {
+    const int segment = cta / p.cluster;
+    s.b = segment / (p.tiles * kv);
+    s.tile = (segment - s.b * p.tiles * kv) / kv;
+    s.h = segment - (s.b * p.tiles + s.tile) * kv;
+    s.index = cta - segment * p.cluster;
+    s.pieces = p.cluster;
     s.length = kv4_length(p.a.lengths, s.b, p.a.cache.capacity);
     return true;
   }
@@ -384,7 +392,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, NT == 1 ? 2 : 1) kv4_step_ker
   constexpr int R = 8 * NT, W = D / 32;
   using Stage = StepStage<D>;
   extern __shared__ __align__(128) unsigned char step_smem[];
-  __shared__ float part_m[kStepWarps][R], part_l[kStepWarps][R], part_lse[R];
+  __shared__ float part_m[kStepWarps][R], part_l[kStepWarps][R], part_lse[R], cta_m[R], cta_l[R];
   float *part = reinterpret_cast<float *>(step_smem);  // [warps][R][D], over the stages once these are done with
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -393,16 +401,17 @@ __global__ void __launch_bounds__(kStepWarps * 32, NT == 1 ? 2 : 1) kv4_step_ker
   const int kv = p.cache.kv_heads, total = p.seq * p.group;
   StepPiece piece;
   if (!step_find<R>(piece, sp, blockIdx.x)) return;
-  const int b = piece.b, tile = piece.tile, h = piece.h, length = piece.length, slot = blockIdx.x;
+  const int b = piece.b, tile = piece.tile, h = piece.h, length = piece.length, slot = sp.cluster > 0 ? blockIdx.x / sp.cluster : blockIdx.x;
   const Kv4Range range = step_range<R>(p, length, tile);
-  const bool complete = piece.pieces == 1;
+  const int ctas = sp.cluster > 0 ? sp.cluster : 1;  // whose results this one's are joined with here
+  const bool complete = piece.pieces == ctas;
   const int r0 = tile * R;
   const int pos_lo = length - p.seq + r0 / p.group, pos_hi = length - p.seq + (min(r0 + R, total) - 1) / p.group;
   const size_t first = (static_cast<size_t>(b) * kv + h) * p.cache.capacity;
   const int lo = static_cast<int>(static_cast<long long>(range.blocks) * piece.index / piece.pieces);
   const int count = static_cast<int>(static_cast<long long>(range.blocks) * (piece.index + 1) / piece.pieces) - lo;
   const int from = lo + count * warp / kStepWarps, to = lo + count * (warp + 1) / kStepWarps;
-  if (!sp.whole && piece.index == 0 && threadIdx.x == 0) sp.pieces[(b * sp.tiles + tile) * kv + h] = make_int2(slot, piece.pieces);
+  if (sp.cluster == 0 && piece.index == 0 && threadIdx.x == 0) sp.pieces[(b * sp.tiles + tile) * kv + h] = make_int2(slot, piece.pieces);
 
   // a block into a stage, 16 bytes a lane at a time; every call is a group of its own, with nothing in it behind the last block
   const auto request = [&](int i, uint32_t stage) {
@@ -485,24 +494,9 @@ __global__ void __launch_bounds__(kStepWarps * 32, NT == 1 ? 2 : 1) kv4_step_ker
       }
     }
   __syncthreads();
-  for (int i = threadIdx.x; i < R * D / 4; i += kStepWarps * 32) {
+  // the CTA's sums, and out with them where they are all
+  const auto write = [&](int i, float top, float norm, const float4 &sum) {
     const int r = i / (D / 4), row = r0 + r;
-    float top = -INFINITY, norm = 0.f;
-#pragma unroll
-    for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, part_m[w][r]);
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < kStepWarps; ++w) {
-      if (part_l[w][r] == 0.f) continue;  // nothing seen
-      const float f = exp2_approx(part_m[w][r] - top);
-      norm = fmaf(part_l[w][r], f, norm);
-      const float4 x = *reinterpret_cast<const float4 *>(part + (w * R) * D + 4 * i);
-      sum.x = fmaf(x.x, f, sum.x);
-      sum.y = fmaf(x.y, f, sum.y);
-      sum.z = fmaf(x.z, f, sum.z);
-      sum.w = fmaf(x.w, f, sum.w);
-    }
-    if (WEIGHS && i % (D / 4) == 0) part_lse[r] = norm == 0.f ? INFINITY : top + log2f(norm);
     if ((!complete || (!WEIGHS && p.weights != nullptr)) && i % (D / 4) == 0) {
       sp.ml[(static_cast<size_t>(slot) * 2) * R + r] = top;
       sp.ml[(static_cast<size_t>(slot) * 2 + 1) * R + r] = norm;
@@ -518,6 +512,73 @@ __global__ void __launch_bounds__(kStepWarps * 32, NT == 1 ? 2 : 1) kv4_step_ker
       w.y = kv4_bits<T>(sum.z * inv) | static_cast<uint32_t>(kv4_bits<T>(sum.w * inv)) << 16;
       *reinterpret_cast<uint2 *>(p.out + at) = w;
     }
+  };
+  for (int i = threadIdx.x; i < R * D / 4; i += kStepWarps * 32) {
+    const int r = i / (D / 4);
+    float top = -INFINITY, norm = 0.f;
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, part_m[w][r]);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w) {
+      if (part_l[w][r] == 0.f) continue;  // nothing seen
+      const float f = exp2_approx(part_m[w][r] - top);
+      norm = fmaf(part_l[w][r], f, norm);
+      const float4 x = *reinterpret_cast<const float4 *>(part + (w * R) * D + 4 * i);
+      sum.x = fmaf(x.x, f, sum.x);
+      sum.y = fmaf(x.y, f, sum.y);
+      sum.z = fmaf(x.z, f, sum.z);
+      sum.w = fmaf(x.w, f, sum.w);
+    }
+    if (ctas == 1) {
+      if (WEIGHS && i % (D / 4) == 0) part_lse[r] = norm == 0.f ? INFINITY : top + log2f(norm);
+      write(i, top, norm, sum);
+    } else {  // for the others of the cluster, where this thread alone has read
+      *reinterpret_cast<float4 *>(part + 4 * i) = sum;
+      if (i % (D / 4) == 0) cta_m[r] = top, cta_l[r] = norm;
+    }
+  }
+  if (ctas > 1) {
+    cluster_sync_all();
+    const uint32_t sums = smem_u32(part), tops = smem_u32(cta_m), norms = smem_u32(cta_l);
+    const auto join = [&](int i, float &top, float &norm, float4 &sum, bool whole) {  // in the order of the pieces
+      const int r = i / (D / 4);
+      float m[8], l[8];
+      float4 x[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        if (c >= ctas) continue;
+        m[c] = ld_cluster_f32(map_to_cta(tops + 4 * r, c));
+        l[c] = ld_cluster_f32(map_to_cta(norms + 4 * r, c));
+        if (whole) x[c] = ld_cluster_f32x4(map_to_cta(sums + 16 * i, c));
+      }
+      top = -INFINITY, norm = 0.f, sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < ctas) top = fmaxf(top, m[c]);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        if (c >= ctas || l[c] == 0.f) continue;
+        const float f = exp2_approx(m[c] - top);
+        norm = fmaf(l[c], f, norm);
+        if (!whole) continue;
+        sum.x = fmaf(x[c].x, f, sum.x);
+        sum.y = fmaf(x[c].y, f, sum.y);
+        sum.z = fmaf(x[c].z, f, sum.z);
+        sum.w = fmaf(x[c].w, f, sum.w);
+      }
+    };
+    float top, norm;
+    float4 sum;
+    for (int i = piece.index * (kStepWarps * 32) + threadIdx.x; i < R * D / 4; i += ctas * (kStepWarps * 32)) {
+      join(i, top, norm, sum, true);
+      write(i, top, norm, sum);
+    }
+    if (WEIGHS && threadIdx.x < R) {
+      join(threadIdx.x * (D / 4), top, norm, sum, false);
+      part_lse[threadIdx.x] = norm == 0.f ? INFINITY : top + log2f(norm);
+    }
+    cluster_sync_all();  // no CTA leaves while another reads its shared memory
   }
   if constexpr (WEIGHS) {
     // The rows' sums are known: once more over the scores, from K's codes and params (out of L2), for each entry's share of them.
@@ -587,7 +648,7 @@ template <typename T, int D, int NT, int LANES> __global__ void __launch_bounds_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kv = p.cache.kv_heads, total = p.seq * p.group, b = blockIdx.y / kv, h = blockIdx.y - b * kv;
   const int part = blockIdx.x, tile = part / kParts;
-  const bool joins = !sp.whole && tile < sp.tiles;
+  const bool joins = sp.cluster == 0 && tile < sp.tiles;
   int2 pieces = make_int2(0, 1);
   if (joins) pieces = sp.pieces[(b * sp.tiles + tile) * kv + h];
   const int length = kv4_length(p.lengths, b, p.cache.capacity);
@@ -665,7 +726,7 @@ template <typename T, int D, int NT, int LANES> __global__ void __launch_bounds_
   for (int row = warp; row < total; row += kStepWarps) {
     const int segment = (b * sp.tiles + row / R) * kv + h, r = row % R;
     int2 of = make_int2(segment, 1);
-    if (!sp.whole) of = sp.pieces[segment];
+    if (sp.cluster == 0) of = sp.pieces[segment];
     if (step_range<R>(p, length, row / R).blocks == 0) of.y = 0;
     float m = -INFINITY, l = 0.f;
     for (int i = lane; i < of.y; i += 32) {
@@ -719,7 +780,8 @@ namespace {
 
 struct StepPlan {
   int rows, tiles, segments;  // rows of a tile
-  bool whole, weighs;
+  int cluster;  // as in Kv4StepParams
+  bool weighs;
   int64_t slots, pieces_bytes, ml_bytes, partial_bytes;
 };
 
@@ -731,28 +793,40 @@ StepPlan step_plan(const Kv4Cache &c, int seq, int group, int window, int sinks,
   const int all = (c.capacity + kStepBlock - 1) / kStepBlock;
   // a window of w entries and the s rows' own lie in at most (w + s - 2) / 32 + 2 blocks
   const int blocks = window > 0 ? std::min(all, (window + seq - 2) / kStepBlock + 2 + (sinks + kStepBlock - 1) / kStepBlock) : all;
-  s.whole = blocks <= kStepWhole || s.segments >= 4 * kStepCtas;
+  // CTAs for a segment while they all run at once and each warp of them has a block
+  int cluster = 1;
+  while (cluster < 8 && s.segments * cluster * 2 <= kStepCtas && cluster * 2 * kStepWarps <= blocks) cluster *= 2;
+  s.cluster = (blocks + cluster - 1) / cluster <= kStepWhole || s.segments >= 4 * kStepCtas ? cluster : 0;
   // pieces of all segments: blocks / share and one for what is left over, each; shares are at least all blocks / kStepCtas
-  s.slots = s.whole ? s.segments : s.segments + kStepCtas;
-  s.pieces_bytes = s.whole ? 0 : (s.segments * 8 + 15) / 16 * 16;
-  s.weighs = s.whole && s.tiles == 1;  // one CTA sees all rows and all entries
-  s.ml_bytes = s.whole && (!weights || s.weighs) ? 0 : s.slots * 2 * s.rows * 4;
-  s.partial_bytes = s.whole ? 0 : s.slots * s.rows * c.dim * 4;
+  s.slots = s.cluster > 0 ? s.segments : s.segments + kStepCtas;
+  s.pieces_bytes = s.cluster > 0 ? 0 : (s.segments * 8 + 15) / 16 * 16;
+  s.weighs = s.cluster > 0 && s.tiles == 1;  // the CTAs of a segment see all rows and all entries
+  s.ml_bytes = s.cluster > 0 && (!weights || s.weighs) ? 0 : s.slots * 2 * s.rows * 4;
+  s.partial_bytes = s.cluster > 0 ? 0 : s.slots * s.rows * c.dim * 4;
   return s;
 }
 
 template <typename Kernel, typename... Args>
-int launch_step(Kernel kernel, dim3 grid, int smem, cudaStream_t stream, bool pdl, Args... args) {
+int launch_step(Kernel kernel, dim3 grid, int cluster, int smem, cudaStream_t stream, bool pdl, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(kStepWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
+  cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? MG_OK : MG_ERR_CUDA;
 }
 
@@ -762,13 +836,15 @@ template <typename T, int D, int NT> int kv4_step(const Kv4StepParams &p, const 
   static SharedMemoryOptIn opt_in, opt_in_weighs;
   int st = weighs ? opt_in_weighs.ensure(kv4_step_kernel<T, D, NT, true>, smem) : opt_in.ensure(kv4_step_kernel<T, D, NT, false>, smem);
   if (st != MG_OK) return st;
-  const dim3 grid(static_cast<unsigned>(plan.slots));
-  st = weighs ? launch_step(kv4_step_kernel<T, D, NT, true>, grid, smem, stream, pdl, p) : launch_step(kv4_step_kernel<T, D, NT, false>, grid, smem, stream, pdl, p);
-  if (st != MG_OK || (plan.whole && (p.a.weights == nullptr || weighs))) return st;
+  const int cluster = std::max(plan.cluster, 1);
+  const dim3 grid(static_cast<unsigned>(plan.slots * cluster));
+  st = weighs ? launch_step(kv4_step_kernel<T, D, NT, true>, grid, cluster, smem, stream, pdl, p)
+              : launch_step(kv4_step_kernel<T, D, NT, false>, grid, cluster, smem, stream, pdl, p);
+  if (st != MG_OK || (plan.cluster > 0 && (p.a.weights == nullptr || weighs))) return st;
   const int entries = p.a.weights != nullptr ? (p.a.cache.capacity + kFinishEntries - 1) / kFinishEntries : 1;
   const auto finish = [&](auto kernel, int lanes) {
-    const int parts = plan.whole ? 1 : 8 * NT * D * lanes / 1024 * plan.tiles;
-    return launch_step(kernel, dim3(std::max(parts, entries), p.a.cache.batch * p.a.cache.kv_heads), 0, stream, true, p);
+    const int parts = plan.cluster > 0 ? 1 : 8 * NT * D * lanes / 1024 * plan.tiles;
+    return launch_step(kernel, dim3(std::max(parts, entries), p.a.cache.batch * p.a.cache.kv_heads), 1, 0, stream, true, p);
   };
   // few segments have many pieces each: more threads for each number then
   return plan.segments <= 4 ? finish(kv4_finish_kernel<T, D, NT, 16>, 16) : finish(kv4_finish_kernel<T, D, NT, 4>, 4);
@@ -786,7 +862,7 @@ int kv4_few_rows(const Kv4AttentionParams &a, void *workspace, bool bf16, bool p
   p.ml = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + plan.pieces_bytes);
   p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + plan.pieces_bytes + plan.ml_bytes);
   p.tiles = plan.tiles;
-  p.whole = plan.whole;
+  p.cluster = plan.cluster;
   if (a.cache.dim == 64) return bf16 ? kv4_step_rows<__nv_bfloat16, 64>(p, plan, stream, pdl) : kv4_step_rows<__half, 64>(p, plan, stream, pdl);
   return bf16 ? kv4_step_rows<__nv_bfloat16, 128>(p, plan, stream, pdl) : kv4_step_rows<__half, 128>(p, plan, stream, pdl);
 }

@@ -80,7 +80,7 @@ def test_c_abi_refuses_bad_arguments(lib):
     attend = lambda **k: lib.matgptq_b200_attention_kv4(c, *{**dict(q=p, seq=1, heads=H, len=p, window=0, sinks=0, scale=1.0, weights=None, out=p,  # noqa: E731
                                                                   ws=None, ws_bytes=0, flags=0, stream=None), **k}.values())
     for bad in (dict(q=None), dict(len=None), dict(out=None), dict(seq=-1), dict(heads=0), dict(heads=3), dict(window=-1), dict(sinks=-1),
-                dict(weights=p), dict(weights=p, ws=p, ws_bytes=0)):
+                dict(seq=12, weights=p), dict(seq=12, weights=p, ws=p, ws_bytes=0)):
         assert attend(**bad) == 1, bad
     assert attend(q=odd) == 4 and attend(out=odd) == 4
     assert attend(seq=1 << 25) == 3
@@ -97,7 +97,7 @@ def test_c_abi_refuses_bad_arguments(lib):
     assert lib.matgptq_b200_dequantize_kv4(c, p, 0, None, None, 0, None) == 0
     assert lib.matgptq_b200_attention_kv4_workspace_bytes(c, 5, H, 0, 0, 0) == 0
     assert lib.matgptq_b200_attention_kv4_workspace_bytes(None, 5, H, 0, 0, 1) == 0
-    for seq in (1, 5, 16, 17, 500):
+    for seq in (12, 17, 500):  # more rows than one CTA has: what it leaves for the weights goes through the workspace
         need = lib.matgptq_b200_attention_kv4_workspace_bytes(c, seq, H, 0, 0, 1)
         assert need >= B * seq * H * 4
         assert lib.matgptq_b200_attention_kv4_workspace_bytes(c, seq, H, 9, 1, 1) >= B * seq * H * 4
