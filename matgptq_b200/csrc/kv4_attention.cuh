@@ -91,9 +91,9 @@ struct Centring {
 
 constexpr int kKv4FewRows = 32;  // of a key/value head, for kv4_attention.cu; more go to kv4_prompt.cu
 
-// What the second pass over many rows, for the weights, reads of 128 rows: q as the operand it is in shared memory, then three
-// numbers for each row: log2 of a weight per score, per minimum of K, and the log2 of the row's sum.
-__host__ __device__ constexpr int kv4_row_tile_bytes(int dim) { return 128 * dim * 2 + 3 * 128 * 4; }
+// What the second pass over many rows, for the weights, reads of 128 rows: q as the operand it is in shared memory, then of each two
+// rows side by side log2 of a weight per score, per minimum of K, less the log2 of the row's sum, and two unused.
+__host__ __device__ constexpr int kv4_row_tile_bytes(int dim) { return 128 * dim * 2 + 128 * 16; }
 
 // kv4_prompt.cu
 int kv4_prompt_launch(const Kv4AttentionParams &p, bool bf16, bool pdl, cudaStream_t stream);

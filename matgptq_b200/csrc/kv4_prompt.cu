@@ -503,10 +503,11 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
         }
       }
       if (tile_out != nullptr) {
-        float *numbers = reinterpret_cast<float *>(tile_out + 128 * D * 2) + quad * 32 + lane;
+        const int of = quad * 32 + lane;
+        float *numbers = reinterpret_cast<float *>(tile_out + 128 * D * 2) + (of >> 1) * 8 + (of & 1);
         numbers[0] = unit;
-        numbers[128] = sum * unit;
-        numbers[256] = !live || l == 0.f ? INFINITY : lds_f32(my_row + 8) + log2f(l);
+        numbers[2] = sum * unit;
+        numbers[4] = !live || l == 0.f ? -INFINITY : -(lds_f32(my_row + 8) + log2f(l));
       }
     }
   } else if (warp < kMma) {
@@ -673,16 +674,16 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
 
 // weights[j] += sum over the rows that see entry j of exp2(score - log2 of the row's sum).  A CTA takes 128 entries and goes over the
 // tiles of 128 rows that kv4_prompt_kernel left: S^T = K Q^T puts an entry in each lane of tensor memory and the rows in its
-// columns, so that a thread adds up one entry's weights, in the order of the rows, with no other to wait for.  Four warps do that; the
-// fifth requests the tiles (one copy each, they are operands already) and issues the MMAs, two accumulators in turn.  What bounds it
-// are the exponentials (16 a cycle and SM) and what goes with them.
-constexpr int kPwWarps = 5, kPwMma = 4;
-constexpr int kPwBarK = 0, kPwBarQFull = 8, kPwBarQEmpty = 24, kPwBarSFull = 40, kPwBarSEmpty = 56, kPwBarEnd = 72, kPwTmemSlot = 80;
+// columns.  Two times four warps add up, each half of the columns; a lane has four entries and a quarter of the columns (as in
+// kv4_prompt_kernel), and all its sums have one order.  The last warp requests the tiles (one copy each, they are operands already) and
+// issues the MMAs, two accumulators in turn.  What bounds it are the exponentials (16 a cycle and SM) and what goes with them.
+constexpr int kPwWarps = 9, kPwMma = 8;
+constexpr int kPwBarK = 0, kPwBarQFull = 8, kPwBarQEmpty = 24, kPwBarSFull = 40, kPwBarSEmpty = 56, kPwBarEnd = 72, kPwTmemSlot = 80, kPwSums = 512;
 template <int D> struct WeightsPlan {
   static constexpr int k = 1024, k_bytes = 128 * D * 2, q = k + k_bytes, q_bytes = kv4_row_tile_bytes(D), end = q + 2 * q_bytes;
 };
 
-template <typename T, int D> __global__ void __launch_bounds__(kPwWarps * 32) kv4_prompt_weights_kernel(const Kv4AttentionParams p) {
+template <typename T, int D> __global__ void __launch_bounds__(kPwWarps * 32, 2) kv4_prompt_weights_kernel(const Kv4AttentionParams p) {
   using Plan = WeightsPlan<D>;
   extern __shared__ __align__(1024) unsigned char weights_smem[];
   const uint32_t base = smem_u32(weights_smem);
@@ -694,9 +695,9 @@ template <typename T, int D> __global__ void __launch_bounds__(kPwWarps * 32) kv
     }
     if (lane < 2) {
       mbar_init(base + kPwBarQFull + 8 * lane, 1);
-      mbar_init(base + kPwBarQEmpty + 8 * lane, 5);  // the MMAs and four warps
+      mbar_init(base + kPwBarQEmpty + 8 * lane, 9);  // the MMAs and eight warps
       mbar_init(base + kPwBarSFull + 8 * lane, 1);
-      mbar_init(base + kPwBarSEmpty + 8 * lane, 4);
+      mbar_init(base + kPwBarSEmpty + 8 * lane, 8);
     }
     mbar_init_fence();
     __syncwarp();
@@ -709,10 +710,10 @@ template <typename T, int D> __global__ void __launch_bounds__(kPwWarps * 32) kv
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(weights_smem + kPwTmemSlot);
   pdl_prologue();
 
-  const int b = blockIdx.y / p.cache.kv_heads;
+  const int heads = p.cache.batch * p.cache.kv_heads, bh = blockIdx.x % heads, b = bh / p.cache.kv_heads;
   const int total = p.seq * p.group, length = kv4_length(p.lengths, b, p.cache.capacity), behind = length - p.seq;
-  const size_t first = static_cast<size_t>(blockIdx.y) * p.cache.capacity;
-  const int j0 = blockIdx.x * 128;
+  const size_t first = static_cast<size_t>(bh) * p.cache.capacity;
+  const int j0 = blockIdx.x / heads * 128;
   // rows that see entry j: [from(j), to(j)); both grow with j, but for the first entries, which every later row sees
   const auto from = [&](int j) { return min(max(j - behind, 0), p.seq) * p.group; };
   const auto to = [&](int j) { return p.window > 0 && j >= p.sinks ? min(max(j + p.window - behind, 0), p.seq) * p.group : total; };
@@ -721,11 +722,9 @@ template <typename T, int D> __global__ void __launch_bounds__(kPwWarps * 32) kv
   const int tile_lo = row_lo >> 7, tiles = row_hi > row_lo ? ((row_hi + 127) >> 7) - tile_lo : 0;
   bool failed = false;
   if (tiles > 0 && warp < kPwMma) {
-    const int tid = threadIdx.x, j = j0 + tid;
-    uint2 par = make_uint2(0, 0);  // entries behind the last one may hold anything: no row sees them
-    {
-      const bool there = j < p.cache.capacity;
-      const uint8_t *kr = p.cache.k + (first + (there ? j : j0)) * (D / 2);
+    if (warp < 4) {  // K, an entry a thread
+      const int tid = threadIdx.x;
+      const uint8_t *kr = p.cache.k + (first + (j0 + tid < p.cache.capacity ? j0 + tid : j0)) * (D / 2);
 #pragma unroll
       for (int i = 0; i < D / 8; i += 4) {
         const uint4 v = *reinterpret_cast<const uint4 *>(kr + 4 * i);
@@ -736,15 +735,26 @@ template <typename T, int D> __global__ void __launch_bounds__(kPwWarps * 32) kv
           sts_v4(base + Plan::k + (i + k) * 2048 + tid * 16, x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u);
         }
       }
-      if (j < length) par = *reinterpret_cast<const uint2 *>(p.cache.params + (first + j) * 4);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(base + kPwBarK);
     }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncwarp();
-    if (lane == 0) mbar_arrive(base + kPwBarK);
-    const float ks = kv4_to_f<T>(static_cast<uint16_t>(par.x)), kl = kv4_to_f<T>(static_cast<uint16_t>(par.x >> 16));
-    const uint64_t ks2 = pack2(ks, ks), kl2 = pack2(kl, kl);
-    const int mine_lo = from(j), mine_hi = j < length ? to(j) : 0;
-    uint64_t sum2 = 0;
+    const int quad = warp & 3, side = warp >> 2, t4 = lane & 3;
+    constexpr uint32_t kLanes16 = 16u << 16;
+    uint64_t ks2[4], kl2[4], sum2[4];
+    int mine_lo[4], mine_hi[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int j = j0 + quad * 32 + (lane >> 2) + 8 * k;
+      uint32_t par = 0;  // entries behind the last one may hold anything: no row sees them
+      if (j < length) par = *reinterpret_cast<const uint32_t *>(p.cache.params + (first + j) * 4);
+      const float ks = kv4_to_f<T>(static_cast<uint16_t>(par)), kl = kv4_to_f<T>(static_cast<uint16_t>(par >> 16));
+      ks2[k] = pack2(ks, ks);
+      kl2[k] = pack2(kl, kl);
+      sum2[k] = 0;
+      mine_lo[k] = from(j);
+      mine_hi[k] = j < length ? to(j) : 0;
+    }
     for (int t = 0; t < tiles; ++t) {
       const int stage = t & 1, parity = (t >> 1) & 1;
       if (!mbar_wait_chain(base + kPwBarQFull + 8 * stage, parity) || !mbar_wait_chain(base + kPwBarSFull + 8 * stage, parity)) {
@@ -752,39 +762,51 @@ template <typename T, int D> __global__ void __launch_bounds__(kPwWarps * 32) kv
         break;
       }
       tc_fence_after();
-      const uint32_t t_s = tmem + (static_cast<uint32_t>(warp * 32) << 16) + stage * 128;
-      const uint32_t numbers = base + Plan::q + stage * Plan::q_bytes + 128 * D * 2;
-      const int row0 = (tile_lo + t) * 128;
-      const bool whole = __all_sync(0xffffffffu, mine_lo <= row0 && mine_hi >= row0 + 128);
-      uint64_t tile2 = 0;
+      const uint32_t t_s = tmem + (static_cast<uint32_t>(quad * 32) << 16) + stage * 128 + side * 64;
+      const uint32_t numbers = base + Plan::q + stage * Plan::q_bytes + 128 * D * 2 + (side * 32 + t4) * 32;
+      const int row0 = (tile_lo + t) * 128 + side * 64;
+      bool whole = true;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) whole &= mine_lo[k] <= row0 && mine_hi[k] >= row0 + 64;
+      whole = __all_sync(0xffffffffu, whole);
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        uint32_t s[32];
-        tmem_ld32(t_s + 32 * c, s);
-        const uint32_t seen = whole ? 0xffffffffu : bits_below(mine_hi - row0 - 32 * c) & ~bits_below(mine_lo - row0 - 32 * c);
+      for (int c = 0; c < 2; ++c) {  // 32 rows
+        uint32_t s[2][16], seen[4];
+        tmem_ld_16x32(t_s + 32 * c, s[0]);
+        tmem_ld_16x32(t_s + kLanes16 + 32 * c, s[1]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          seen[k] = whole ? 0xffffffffu
+                          : (bits_below(mine_hi[k] - row0 - 32 * c) & ~bits_below(mine_lo[k] - row0 - 32 * c)) >> (2 * t4);
         tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          uint64_t unit[2], low[2], lse[2];
-          const uint32_t at = numbers + (32 * c + i) * 4;
-          lds_2x64(at, unit[0], unit[1]);
-          lds_2x64(at + 512, low[0], low[1]);
-          lds_2x64(at + 1024, lse[0], lse[1]);
+        for (int i = 0; i < 4; ++i) {
+          uint64_t unit, low, lse, unused, w[4];
+          float x[4], y[4];
+          lds_2x64(numbers + (16 * c + 4 * i) * 32, unit, low);
+          lds_2x64(numbers + (16 * c + 4 * i) * 32 + 16, lse, unused);
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float x, y, lx, ly;
-            const uint64_t raw = mul2(ks2, pack2(__uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1])));
-            unpack2(lse[k], lx, ly);
-            unpack2(fma2(raw, unit[k], fma2(kl2, low[k], pack2(-lx, -ly))), x, y);
-            x = exp2_approx(x);
-            y = exp2_approx(y);
-            if (!((seen >> (i + 2 * k)) & 1u)) x = 0.f;
-            if (!((seen >> (i + 2 * k + 1)) & 1u)) y = 0.f;
-            tile2 = add2(tile2, pack2(x, y));
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t *raw = s[k >> 1] + 4 * i + 2 * (k & 1);
+            w[k] = fma2(mul2(ks2[k], pack2(__uint_as_float(raw[0]), __uint_as_float(raw[1]))), unit, fma2(kl2[k], low, lse));
           }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            unpack2(w[k], x[k], y[k]);
+            x[k] = exp2_approx(x[k]);
+            y[k] = exp2_approx(y[k]);
+          }
+          if (!whole) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (!((seen[k] >> (8 * i)) & 1u)) x[k] = 0.f;
+              if (!((seen[k] >> (8 * i + 1)) & 1u)) y[k] = 0.f;
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) sum2[k] = add2(sum2[k], pack2(x[k], y[k]));
         }
       }
-      sum2 = add2(sum2, tile2);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -792,14 +814,29 @@ template <typename T, int D> __global__ void __launch_bounds__(kPwWarps * 32) kv
         mbar_arrive(base + kPwBarQEmpty + 8 * stage);
       }
     }
-    float x, y;
-    unpack2(sum2, x, y);
-    if (j < length && !failed) p.weights[first + j] += x + y;
+    float sum[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float x, y;
+      unpack2(sum2[k], x, y);
+      sum[k] = x + y;
+      sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
+      sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
+      if (side == 1 && t4 == 0) sts_f32(base + kPwSums + (quad * 32 + (lane >> 2) + 8 * k) * 4, sum[k]);
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");  // the other side's sums are there; every warp comes here
+    if (side == 0 && t4 == 0 && !failed) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int of = quad * 32 + (lane >> 2) + 8 * k;
+        if (j0 + of < length) p.weights[first + j0 + of] += sum[k] + lds_f32(base + kPwSums + of * 4);
+      }
+    }
     if (failed) report_status(kStatusMmaTimeout);
   } else if (tiles > 0) {
     const uint32_t idesc = umma_instr_desc(0, 128);
     const uint64_t dk = umma_smem_desc(base + Plan::k, 2048, 128, 0), dq = umma_smem_desc(base + Plan::q, 2048, 128, 0);
-    const uint8_t *src = p.row_tiles + (static_cast<size_t>(blockIdx.y) * ((total + 127) / 128) + tile_lo) * Plan::q_bytes;
+    const uint8_t *src = p.row_tiles + (static_cast<size_t>(bh) * ((total + 127) / 128) + tile_lo) * Plan::q_bytes;
     const auto request = [&](int t) {  // by one lane
       const uint32_t bar = base + kPwBarQFull + 8 * (t & 1);
       mbar_arrive_expect_tx(bar, Plan::q_bytes);
@@ -858,7 +895,9 @@ template <typename T, int D> int launch_prompt_weights(const Kv4AttentionParams 
   const int st = opt_in.ensure(kv4_prompt_weights_kernel<T, D>, smem);
   if (st != MG_OK) return st;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.cache.capacity + 127) / 128, p.cache.batch * p.cache.kv_heads);
+  const long long ctas = static_cast<long long>(p.cache.batch) * p.cache.kv_heads * ((p.cache.capacity + 127) / 128);
+  if (ctas > INT32_MAX) return MG_ERR_UNSUPPORTED;
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(kPwWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
