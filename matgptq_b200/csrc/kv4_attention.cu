@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 #include "../../include/matgptq_b200.h"
 #include "async.cuh"
@@ -182,14 +183,14 @@ template <int R> __device__ __forceinline__ Kv4Range step_range(const Kv4Attenti
   return kv4_range<kStepBlock>(length - p.seq + r0 / p.group, length - p.seq + (min(r0 + R, total) - 1) / p.group, p.window, p.sinks, p.cache.capacity);
 }
 
-__device__ __forceinline__ int warp_sum(int x) {
+__device__ __forceinline__ uint32_t warp_sum(uint32_t x) {
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
   return x;
 }
 
 // The piece of CTA `cta`: its segment (b, tile, h), which of its segment's pieces it is, and how many these are; false where there are
-// fewer pieces than CTAs.  Pieces are numbered by sequence, tile and head; a warp looks at 32 sequences at a time.
+// fewer pieces than CTAs.  Pieces are numbered by sequence, tile and head; a warp looks at 32 tiles at a time.
 struct StepPiece {
   int b, tile, h, index, pieces, length;
 };
@@ -207,29 +208,30 @@ template <int R> __device__ __forceinline__ bool step_find(StepPiece &s, const K
   }
   // The smallest share (about) that leaves no more pieces than run at once; with more segments than that, the mean work of a CTA.  (A
   // few pieces more are a second round for all: 64 heads of 4096 entries in 5 pieces each, 24.0 us, in 4 19.5.)
+  const int tiles = batch * p.tiles;
+  const auto blocks_of = [&](int i, int &length) {  // of tile i of all sequences' tiles
+    const int b = i / p.tiles;
+    length = kv4_length(p.a.lengths, b, p.a.cache.capacity);
+    return step_range<R>(p.a, length, i - b * p.tiles).blocks;
+  };
   const auto sum = [&](auto of) {
-    int x = 0;
-    for (int b0 = 0; b0 < batch; b0 += 32) {
-      if (b0 + lane < batch) {
-        const int length = kv4_length(p.a.lengths, b0 + lane, p.a.cache.capacity);
-        for (int tile = 0; tile < p.tiles; ++tile) x += of(step_range<R>(p.a, length, tile).blocks);
-      }
-    }
+    uint32_t x = 0;  // (296 tiles of 2^28 entries pass 31 bits)
+    int length;
+    for (int i = lane; i < tiles; i += 32) x += of(blocks_of(i, length));
     return warp_sum(x) * kv;
   };
-  const int all = sum([](int blocks) { return blocks; }), segments = batch * p.tiles * kv;
+  const uint32_t all = sum([](int blocks) { return blocks; });
+  const int segments = tiles * kv;
   const int room = segments < kStepCtas ? kStepCtas - segments / 2 : kStepCtas;
-  int share = max((all + room - 1) / room, kStepLeast);
+  int share = max(static_cast<int>((all + room - 1) / room), kStepLeast);
   const auto cut = [&](int blocks) { return (blocks + share - 1) / share; };
   if (segments < kStepCtas)
     for (int i = 0; i < 16 && sum(cut) > kStepCtas; ++i) share += max(share >> 4, 1);
   int before = 0;
-  for (int b0 = 0; b0 < batch; b0 += 32) {
-    int length = 0, mine = 0;
-    if (b0 + lane < batch) {
-      length = kv4_length(p.a.lengths, b0 + lane, p.a.cache.capacity);
-      for (int tile = 0; tile < p.tiles; ++tile) mine += cut(step_range<R>(p.a, length, tile).blocks) * kv;
-    }
+  for (int i0 = 0; i0 < tiles; i0 += 32) {
+    int length = 0, pieces = 0;
+    if (i0 + lane < tiles) pieces = cut(blocks_of(i0 + lane, length));
+    const int mine = pieces * kv;
     int up_to = mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -238,15 +240,12 @@ template <int R> __device__ __forceinline__ bool step_find(StepPiece &s, const K
     }
     const unsigned past = __ballot_sync(0xffffffffu, before + up_to > cta);
     if (past != 0) {
-      const int l = __ffs(past) - 1;  // the sequence that the piece is in
-      s.b = b0 + l;
+      const int l = __ffs(past) - 1;  // the tile that the piece is of
+      s.b = (i0 + l) / p.tiles;
+      s.tile = i0 + l - s.b * p.tiles;
       s.length = __shfl_sync(0xffffffffu, length, l);
-      int at = cta - before - __shfl_sync(0xffffffffu, up_to - mine, l);
-      for (s.tile = 0; s.tile < p.tiles; ++s.tile) {
-        s.pieces = cut(step_range<R>(p.a, s.length, s.tile).blocks);
-        if (at < s.pieces * kv) break;
-        at -= s.pieces * kv;
-      }
+      s.pieces = __shfl_sync(0xffffffffu, pieces, l);
+      const int at = cta - before - __shfl_sync(0xffffffffu, up_to - mine, l);
       s.h = at / s.pieces;
       s.index = at - s.h * s.pieces;
       return true;
@@ -632,7 +631,8 @@ __global__ void __launch_bounds__(kStepWarps * 32, NT == 1 ? 2 : 1) kv4_step_ker
   }
 }
 
-// What is left once every piece has been seen: joins the partial results of segments that were cut, and adds up the weights.
+// What is left once every piece of segments that were cut has been seen: joins the partial results, and adds up the weights where all
+// rows are one tile.
 // blockIdx.y: sequence and head; blockIdx.x: a part of a tile's results (1024 / LANES numbers), and kFinishEntries
 // entries whose weights are due.
 // Every step is a round trip to memory, so what does not hang on another is asked for at once.
@@ -642,13 +642,13 @@ template <typename T, int D, int NT, int LANES> __global__ void __launch_bounds_
   pdl_prologue();
   const Kv4AttentionParams &p = sp.a;
   constexpr int R = 8 * NT, kFours = kStepWarps * 32 / LANES, kParts = R * D / 4 / kFours;
-  __shared__ float row_lse[kKv4FewRows];
+  __shared__ float row_lse[R];
   __shared__ float4 other[LANES - 1][kFours];
   __shared__ float other_m[LANES - 1][kFours], other_l[LANES - 1][kFours];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kv = p.cache.kv_heads, total = p.seq * p.group, b = blockIdx.y / kv, h = blockIdx.y - b * kv;
   const int part = blockIdx.x, tile = part / kParts;
-  const bool joins = sp.cluster == 0 && tile < sp.tiles;
+  const bool joins = tile < sp.tiles;
   int2 pieces = make_int2(0, 1);
   if (joins) pieces = sp.pieces[(b * sp.tiles + tile) * kv + h];
   const int length = kv4_length(p.lengths, b, p.cache.capacity);
@@ -724,13 +724,11 @@ template <typename T, int D, int NT, int LANES> __global__ void __launch_bounds_
   if (!weighs) return;
   // the rows' sums: a warp per row
   for (int row = warp; row < total; row += kStepWarps) {
-    const int segment = (b * sp.tiles + row / R) * kv + h, r = row % R;
-    int2 of = make_int2(segment, 1);
-    if (sp.cluster == 0) of = sp.pieces[segment];
-    if (step_range<R>(p, length, row / R).blocks == 0) of.y = 0;
+    int2 of = sp.pieces[blockIdx.y];  // all rows are one tile
+    if (step_range<R>(p, length, 0).blocks == 0) of.y = 0;
     float m = -INFINITY, l = 0.f;
     for (int i = lane; i < of.y; i += 32) {
-      const float m1 = sp.ml[static_cast<size_t>(of.x + i) * 2 * R + r], l1 = sp.ml[(static_cast<size_t>(of.x + i) * 2 + 1) * R + r];
+      const float m1 = sp.ml[static_cast<size_t>(of.x + i) * 2 * R + row], l1 = sp.ml[(static_cast<size_t>(of.x + i) * 2 + 1) * R + row];
       if (l1 == 0.f) continue;
       const float top = fmaxf(m, m1);
       l = (l == 0.f ? 0.f : l * exp2_approx(m - top)) + l1 * exp2_approx(m1 - top);
@@ -776,23 +774,73 @@ template <typename T, int D, int NT, int LANES> __global__ void __launch_bounds_
     }
 }
 
+// Rows of several tiles: what the pass for their weights needs of 128 rows, a thread each: q as an operand, and the row's sum from the
+// sums of the pieces.  (The finish kernel, which took a head's rows 8 at a time, needed 159 us for 32 rows of 64 heads of 8192 entries
+// and 54 for 2048; this pass 144 and 49.  It costs a launch more, and with one tile of rows most of its products would be for nothing.)
+template <typename T, int D> __global__ void __launch_bounds__(128) kv4_row_tiles_kernel(const Kv4StepParams sp) {
+  constexpr int R = 16;
+  pdl_prologue();
+  const Kv4AttentionParams &p = sp.a;
+  const int kv = p.cache.kv_heads, total = p.seq * p.group, b = blockIdx.y / kv, h = blockIdx.y - b * kv;
+  const int row = blockIdx.x * 128 + threadIdx.x, query = row / p.group;
+  const bool live = row < total;
+  uint8_t *tile = p.row_tiles + (static_cast<size_t>(blockIdx.y) * gridDim.x + blockIdx.x) * kv4_row_tile_bytes(D);
+  float unit, sum, l = 0.f, m = -INFINITY;
+  const size_t at = ((static_cast<size_t>(b) * p.seq + query) * p.heads + static_cast<size_t>(h) * p.group + (row - query * p.group)) * D;
+  kv4_operand_row<T, D>(p.q + at, live, p.scale_log2, unit, sum, [&](int c, const uint4 &chunk) {
+    *reinterpret_cast<uint4 *>(tile + c * (128 * 16) + threadIdx.x * 16) = chunk;
+  });
+  if (live) {
+    const int segment = (b * sp.tiles + row / R) * kv + h, r = row % R;
+    int2 of = make_int2(segment, 1);
+    if (sp.cluster == 0) of = sp.pieces[segment];
+    if (step_range<R>(p, kv4_length(p.lengths, b, p.cache.capacity), row / R).blocks == 0) of.y = 0;
+    for (int i = 0; i < of.y; ++i) {
+      const float m1 = sp.ml[static_cast<size_t>(of.x + i) * 2 * R + r], l1 = sp.ml[(static_cast<size_t>(of.x + i) * 2 + 1) * R + r];
+      if (l1 == 0.f) continue;
+      const float top = fmaxf(m, m1);
+      l = (l == 0.f ? 0.f : l * exp2_approx(m - top)) + l1 * exp2_approx(m1 - top);
+      m = top;
+    }
+  }
+  kv4_row_numbers(tile + 128 * D * 2, threadIdx.x, unit, sum, l, m);
+}
+
 namespace {
 
 struct StepPlan {
   int rows, tiles, segments;  // rows of a tile
   int cluster;  // as in Kv4StepParams
-  bool weighs;
-  int64_t slots, pieces_bytes, ml_bytes, partial_bytes;
+  bool weighs;   // kv4_step_kernel adds up the weights
+  int64_t slots, pieces_bytes, ml_bytes, partial_bytes, row_tiles_bytes;
+  int64_t bytes() const { return pieces_bytes + ml_bytes + partial_bytes + row_tiles_bytes; }
 };
+
+int64_t row_tiles_bytes(const Kv4Cache &c, int64_t rows) {
+  return static_cast<int64_t>(c.batch) * c.kv_heads * ((rows + 127) / 128) * kv4_row_tile_bytes(c.dim);
+}
+
+// The blocks that `seq` tokens see at most: a window of w entries and the tokens' own lie in at most (w + seq - 2) / 32 + 2
+int step_blocks(const Kv4Cache &c, int seq, int window, int sinks) {
+  const int all = (c.capacity + kStepBlock - 1) / kStepBlock;
+  return window > 0 ? std::min(all, (window + seq - 2) / kStepBlock + 2 + (sinks + kStepBlock - 1) / kStepBlock) : all;
+}
+
+// Whether the kernels of this file take the rows.  A head's rows are 16 in a tile here, each of which goes over the entries anew, and
+// 256 in kv4_prompt.cu, one CTA with all their entries: with few tiles the one keeps more SMs busy, with many the other does less work.
+// 8 heads of 4096 entries, here and there: 128 rows 27 and 92 us, 512 rows 64 and 97, 1024 rows 123 and 97; 16 sequences of these 8
+// heads, 36 rows each, 96 and 93.  Up to 32 rows, whatever the number of heads, this side was ahead: 768 heads of 2048 entries, 32
+// rows 182 and 292.
+bool few_rows(const Kv4Cache &c, int64_t rows) {
+  return rows <= kKv4FewRows || static_cast<int64_t>(c.batch) * c.kv_heads * ((rows + 15) / 16) <= kStepCtas;
+}
 
 StepPlan step_plan(const Kv4Cache &c, int seq, int group, int window, int sinks, bool weights) {
   StepPlan s;
   s.rows = seq * group <= 8 ? 8 : 16;
   s.tiles = (seq * group + s.rows - 1) / s.rows;
   s.segments = c.batch * c.kv_heads * s.tiles;
-  const int all = (c.capacity + kStepBlock - 1) / kStepBlock;
-  // a window of w entries and the s rows' own lie in at most (w + s - 2) / 32 + 2 blocks
-  const int blocks = window > 0 ? std::min(all, (window + seq - 2) / kStepBlock + 2 + (sinks + kStepBlock - 1) / kStepBlock) : all;
+  const int blocks = step_blocks(c, seq, window, sinks);
   // CTAs for a segment while they all run at once and each warp of them has a block
   int cluster = 1;
   while (cluster < 8 && s.segments * cluster * 2 <= kStepCtas && cluster * 2 * kStepWarps <= blocks) cluster *= 2;
@@ -803,6 +851,7 @@ StepPlan step_plan(const Kv4Cache &c, int seq, int group, int window, int sinks,
   s.weighs = s.cluster > 0 && s.tiles == 1;  // the CTAs of a segment see all rows and all entries
   s.ml_bytes = s.cluster > 0 && (!weights || s.weighs) ? 0 : s.slots * 2 * s.rows * 4;
   s.partial_bytes = s.cluster > 0 ? 0 : s.slots * s.rows * c.dim * 4;
+  s.row_tiles_bytes = weights && s.tiles > 1 ? row_tiles_bytes(c, seq * group) : 0;
   return s;
 }
 
@@ -841,13 +890,31 @@ template <typename T, int D, int NT> int kv4_step(const Kv4StepParams &p, const 
   st = weighs ? launch_step(kv4_step_kernel<T, D, NT, true>, grid, cluster, smem, stream, pdl, p)
               : launch_step(kv4_step_kernel<T, D, NT, false>, grid, cluster, smem, stream, pdl, p);
   if (st != MG_OK || (plan.cluster > 0 && (p.a.weights == nullptr || weighs))) return st;
-  const int entries = p.a.weights != nullptr ? (p.a.cache.capacity + kFinishEntries - 1) / kFinishEntries : 1;
-  const auto finish = [&](auto kernel, int lanes) {
-    const int parts = plan.cluster > 0 ? 1 : 8 * NT * D * lanes / 1024 * plan.tiles;
-    return launch_step(kernel, dim3(std::max(parts, entries), p.a.cache.batch * p.a.cache.kv_heads), 1, 0, stream, true, p);
-  };
-  // few segments have many pieces each: more threads for each number then
-  return plan.segments <= 4 ? finish(kv4_finish_kernel<T, D, NT, 16>, 16) : finish(kv4_finish_kernel<T, D, NT, 4>, 4);
+  const int heads = p.a.cache.batch * p.a.cache.kv_heads;
+  const bool apart = plan.row_tiles_bytes > 0;  // the weights have a pass of their own
+  if (plan.cluster == 0) {
+    Kv4StepParams f = p;
+    if (apart) f.a.weights = nullptr;
+    const int entries = f.a.weights != nullptr ? (p.a.cache.capacity + kFinishEntries - 1) / kFinishEntries : 1;
+    const auto finish = [&](auto kernel, int lanes) {
+      const int parts = 8 * NT * D * lanes / 1024 * plan.tiles;
+      return launch_step(kernel, dim3(std::max(parts, entries), heads), 1, 0, stream, true, f);
+    };
+    // few segments have many pieces each: more threads for each number then
+    st = plan.segments <= 4 ? finish(kv4_finish_kernel<T, D, NT, 16>, 16) : finish(kv4_finish_kernel<T, D, NT, 4>, 4);
+  }
+  if (!apart || st != MG_OK) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((p.a.seq * p.a.group + 127) / 128, heads);
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kv4_row_tiles_kernel<T, D>, p) != cudaSuccess) return MG_ERR_CUDA;
+  return kv4_prompt_weights_launch(p.a, std::is_same<T, __nv_bfloat16>::value, stream);
 }
 
 template <typename T, int D> int kv4_step_rows(const Kv4StepParams &p, const StepPlan &plan, cudaStream_t stream, bool pdl) {
@@ -861,6 +928,7 @@ int kv4_few_rows(const Kv4AttentionParams &a, void *workspace, bool bf16, bool p
   p.pieces = static_cast<int2 *>(workspace);
   p.ml = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + plan.pieces_bytes);
   p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + plan.pieces_bytes + plan.ml_bytes);
+  p.a.row_tiles = static_cast<uint8_t *>(workspace) + plan.pieces_bytes + plan.ml_bytes + plan.partial_bytes;
   p.tiles = plan.tiles;
   p.cluster = plan.cluster;
   if (a.cache.dim == 64) return bf16 ? kv4_step_rows<__nv_bfloat16, 64>(p, plan, stream, pdl) : kv4_step_rows<__half, 64>(p, plan, stream, pdl);
@@ -882,13 +950,10 @@ int64_t matgptq_b200_attention_kv4_workspace_bytes(const matgptq_b200_kv4_cache 
   if (mg::kv4_check_cache(cache) != MG_OK || cache->batch == 0 || seq <= 0 || n_heads <= 0 || n_heads % cache->n_kv_heads != 0 || window < 0 ||
       sinks < 0 || seq > (1 << 24) || n_heads > (1 << 16))
     return 0;
-  const int64_t rows = seq * (n_heads / cache->n_kv_heads);
-  if (rows > mg::kKv4FewRows)
-    return with_weights ? cache->batch * cache->n_kv_heads * ((rows + 127) / 128) * mg::kv4_row_tile_bytes(static_cast<int>(cache->head_dim)) : 0;
   const mg::Kv4Cache c = mg::kv4_cache(cache);
-  const mg::StepPlan plan = mg::step_plan(c, static_cast<int>(seq), static_cast<int>(rows / seq), mg::kv4_window(c, window), mg::kv4_sinks(c, sinks),
-                                          with_weights != 0);
-  return plan.pieces_bytes + plan.ml_bytes + plan.partial_bytes;
+  const int64_t group = n_heads / cache->n_kv_heads;
+  if (!mg::few_rows(c, seq * group)) return with_weights ? mg::row_tiles_bytes(c, seq * group) : 0;
+  return mg::step_plan(c, static_cast<int>(seq), static_cast<int>(group), mg::kv4_window(c, window), mg::kv4_sinks(c, sinks), with_weights != 0).bytes();
 }
 
 int matgptq_b200_attention_kv4(const matgptq_b200_kv4_cache *cache, const void *q, int64_t seq, int64_t n_heads, const int32_t *lengths,
@@ -898,7 +963,7 @@ int matgptq_b200_attention_kv4(const matgptq_b200_kv4_cache *cache, const void *
   if (st != MG_OK) return st;
   if (!q || !lengths || !out) return MG_ERR_BAD_ARG;
   if (seq < 0 || n_heads <= 0 || n_heads % cache->n_kv_heads != 0 || window < 0 || sinks < 0) return MG_ERR_BAD_ARG;
-  if (seq > (1 << 24) || n_heads > (1 << 16) || seq * (n_heads / cache->n_kv_heads) >= (1 << 24)) return MG_ERR_UNSUPPORTED;
+  if (seq > (1 << 24) || n_heads > (1 << 16) || seq * (n_heads / cache->n_kv_heads) > 65535LL * 256) return MG_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) % 16 != 0) return MG_ERR_ALIGNMENT;
   if (cache->batch == 0 || seq == 0) return MG_OK;
   const int64_t need = matgptq_b200_attention_kv4_workspace_bytes(cache, seq, n_heads, window, sinks, weights != nullptr);
@@ -917,7 +982,7 @@ int matgptq_b200_attention_kv4(const matgptq_b200_kv4_cache *cache, const void *
   p.scale_log2 = scale * 1.44269504088896340736f;
   const bool bf16 = (flags & MATGPTQ_B200_FLAG_BF16) != 0, pdl = (flags & MATGPTQ_B200_FLAG_PDL) != 0;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  if (p.seq * p.group <= mg::kKv4FewRows) return mg::kv4_few_rows(p, workspace, bf16, pdl, cs);
+  if (mg::few_rows(p.cache, static_cast<int64_t>(p.seq) * p.group)) return mg::kv4_few_rows(p, workspace, bf16, pdl, cs);
   p.row_tiles = weights ? static_cast<uint8_t *>(workspace) : nullptr;
   return mg::kv4_prompt_launch(p, bf16, pdl, cs);
 }

@@ -1,5 +1,7 @@
 // What the attention kernels over the 4-bit cache share (kv4_attention.cu: few rows; kv4_prompt.cu: many).
 #pragma once
+#include <cfloat>
+
 #include "kv4.cuh"
 
 namespace mg {
@@ -89,13 +91,62 @@ struct Centring {
   }
 };
 
-constexpr int kKv4FewRows = 32;  // of a key/value head, for kv4_attention.cu; more go to kv4_prompt.cu
+constexpr int kKv4FewRows = 32;  // of a key/value head: up to these, all go to kv4_attention.cu
 
-// What the second pass over many rows, for the weights, reads of 128 rows: q as the operand it is in shared memory, then of each two
+// What the pass for the weights of many rows reads of 128 rows: q as the operand it is in shared memory, then of each two
 // rows side by side log2 of a weight per score, per minimum of K, less the log2 of the row's sum, and two unused.
 __host__ __device__ constexpr int kv4_row_tile_bytes(int dim) { return 128 * dim * 2 + 128 * 16; }
 
+// A row of q as the tensor cores of these passes take it, given to store(c, 16 bytes) eight channels at a time: scaled so that the
+// largest value lies in [2^8, 2^9), which leaves the odd channels their bits when they are divided by 16.  `unit` is then log2 of a
+// weight per score, `sum` the sum of the scaled values in units of a code.
+template <typename T, int D, typename Store>
+__device__ __forceinline__ void kv4_operand_row(const uint16_t *q, bool live, float scale_log2, float &unit, float &sum, Store store) {
+  uint4 raw[D / 8];
+  float top = 0.f;
+#pragma unroll
+  for (int c = 0; c < D / 8; ++c) {
+    raw[c] = make_uint4(0, 0, 0, 0);
+    if (live) raw[c] = *reinterpret_cast<const uint4 *>(q + 8 * c);
+  }
+#pragma unroll
+  for (int c = 0; c < D / 8; ++c) {
+    const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      top = fmaxf(top, fmaxf(fabsf(kv4_to_f<T>(static_cast<uint16_t>(u[i]))), fabsf(kv4_to_f<T>(static_cast<uint16_t>(u[i] >> 16)))));
+  }
+  const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 16), 253);
+  const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * (scale_log2 < 0.f ? -256.f : 256.f);
+  // 2^24 / 2^8; never 0
+  unit = fmaxf(__uint_as_float(static_cast<uint32_t>(e) << 23) * (fabsf(scale_log2) * 65536.f), FLT_MIN);
+  sum = 0.f;
+#pragma unroll
+  for (int c = 0; c < D / 8; ++c) {
+    const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+    uint32_t x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float v = kv4_to_f<T>(static_cast<uint16_t>(u[i >> 1] >> (16 * (i & 1)))) * down;
+      const __half q16 = __float2half_rn(v);
+      sum += __half2float(q16);
+      x[i] = __half_as_ushort(i & 1 ? __float2half_rn(__half2float(q16) * 0.0625f) : q16);
+    }
+    store(c, make_uint4(x[0] | x[4] << 16, x[1] | x[5] << 16, x[2] | x[6] << 16, x[3] | x[7] << 16));
+  }
+  sum *= 0x1p-24f;
+}
+
+// The numbers of row `of` of a tile (kv4_row_tile_bytes); l: the sum of its weights, against the maximum m; 0: it sees nothing
+__device__ __forceinline__ void kv4_row_numbers(uint8_t *all, int of, float unit, float sum, float l, float m) {
+  float *numbers = reinterpret_cast<float *>(all) + (of >> 1) * 8 + (of & 1);
+  numbers[0] = unit;
+  numbers[2] = sum * unit;
+  numbers[4] = l == 0.f ? -INFINITY : -(m + log2f(l));
+}
+
 // kv4_prompt.cu
+int kv4_prompt_weights_launch(const Kv4AttentionParams &p, bool bf16, cudaStream_t stream);  // from row_tiles
 int kv4_prompt_launch(const Kv4AttentionParams &p, bool bf16, bool pdl, cudaStream_t stream);
 
 }  // namespace mg

@@ -360,45 +360,12 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
     uint8_t *tile_out = nullptr;
     if (p.row_tiles != nullptr && r0 + half * 128 < total)
       tile_out = p.row_tiles + (static_cast<size_t>(bh) * ((total + 127) / 128) + (r0 >> 7) + half) * kv4_row_tile_bytes(D);
-    // Q: scaled so that the largest value lies in [2^8, 2^9), which leaves the values divided by 16 their bits
-    float unit, sum = 0.f;
-    {
-      uint4 raw[D / 8];
-      float top = 0.f;
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        raw[c] = make_uint4(0, 0, 0, 0);
-        if (live) raw[c] = *reinterpret_cast<const uint4 *>(p.q + out_at + 8 * c);
-      }
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          top = fmaxf(top, fmaxf(fabsf(kv4_to_f<T>(static_cast<uint16_t>(u[i]))), fabsf(kv4_to_f<T>(static_cast<uint16_t>(u[i] >> 16)))));
-      }
-      const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 16), 253);
-      const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * (p.scale_log2 < 0.f ? -256.f : 256.f);
-      // 2^24 / 2^8; never 0
-      unit = fmaxf(__uint_as_float(static_cast<uint32_t>(e) << 23) * (fabsf(p.scale_log2) * 65536.f), FLT_MIN);
-      const uint32_t dst = base + Plan::q + half * Plan::q_bytes + (quad * 32 + lane) * 16;
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
-        uint32_t x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float v = kv4_to_f<T>(static_cast<uint16_t>(u[i >> 1] >> (16 * (i & 1)))) * down;
-          const __half q16 = __float2half_rn(v);
-          sum += __half2float(q16);
-          x[i] = __half_as_ushort(i & 1 ? __float2half_rn(__half2float(q16) * 0.0625f) : q16);
-        }
-        const uint4 chunk = make_uint4(x[0] | x[4] << 16, x[1] | x[5] << 16, x[2] | x[6] << 16, x[3] | x[7] << 16);
-        sts_v4(dst + c * kChunkQ, chunk.x, chunk.y, chunk.z, chunk.w);
-        if (tile_out != nullptr) *reinterpret_cast<uint4 *>(tile_out + c * kChunkQ + (quad * 32 + lane) * 16) = chunk;
-      }
-      sum *= 0x1p-24f;
-    }
+    float unit, sum;
+    const uint32_t q_at = (quad * 32 + lane) * 16, dst = base + Plan::q + half * Plan::q_bytes + q_at;
+    kv4_operand_row<T, D>(p.q + out_at, live, p.scale_log2, unit, sum, [&](int c, const uint4 &chunk) {
+      sts_v4(dst + c * kChunkQ, chunk.x, chunk.y, chunk.z, chunk.w);
+      if (tile_out != nullptr) *reinterpret_cast<uint4 *>(tile_out + c * kChunkQ + q_at) = chunk;
+    });
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     if (lane == 0) mbar_arrive(base + kPrBarQ);
@@ -502,13 +469,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
           }
         }
       }
-      if (tile_out != nullptr) {
-        const int of = quad * 32 + lane;
-        float *numbers = reinterpret_cast<float *>(tile_out + 128 * D * 2) + (of >> 1) * 8 + (of & 1);
-        numbers[0] = unit;
-        numbers[2] = sum * unit;
-        numbers[4] = !live || l == 0.f ? -INFINITY : -(lds_f32(my_row + 8) + log2f(l));
-      }
+      if (tile_out != nullptr) kv4_row_numbers(tile_out + 128 * D * 2, quad * 32 + lane, unit, sum, live ? l : 0.f, lds_f32(my_row + 8));
     }
   } else if (warp < kMma) {
     // ------------------------------------------------------------------ producers
@@ -889,7 +850,7 @@ template <typename T, int D> __global__ void __launch_bounds__(kPwWarps * 32, 2)
 
 namespace {
 
-template <typename T, int D> int launch_prompt_weights(const Kv4AttentionParams &p, cudaStream_t stream) {
+template <typename T, int D> int launch_weights(const Kv4AttentionParams &p, cudaStream_t stream) {
   constexpr int smem = WeightsPlan<D>::end;
   static SharedMemoryOptIn opt_in;
   const int st = opt_in.ensure(kv4_prompt_weights_kernel<T, D>, smem);
@@ -925,7 +886,7 @@ template <typename T, int D> int launch_prompt(const Kv4AttentionParams &p, bool
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
   if (cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, p) != cudaSuccess) return MG_ERR_CUDA;
-  return p.weights != nullptr ? launch_prompt_weights<T, D>(p, stream) : MG_OK;
+  return p.weights != nullptr ? launch_weights<T, D>(p, stream) : MG_OK;
 }
 
 }  // namespace
@@ -933,6 +894,11 @@ template <typename T, int D> int launch_prompt(const Kv4AttentionParams &p, bool
 int kv4_prompt_launch(const Kv4AttentionParams &p, bool bf16, bool pdl, cudaStream_t stream) {
   if (p.cache.dim == 64) return bf16 ? launch_prompt<__nv_bfloat16, 64>(p, pdl, stream) : launch_prompt<__half, 64>(p, pdl, stream);
   return bf16 ? launch_prompt<__nv_bfloat16, 128>(p, pdl, stream) : launch_prompt<__half, 128>(p, pdl, stream);
+}
+
+int kv4_prompt_weights_launch(const Kv4AttentionParams &p, bool bf16, cudaStream_t stream) {
+  if (p.cache.dim == 64) return bf16 ? launch_weights<__nv_bfloat16, 64>(p, stream) : launch_weights<__half, 64>(p, stream);
+  return bf16 ? launch_weights<__nv_bfloat16, 128>(p, stream) : launch_weights<__half, 128>(p, stream);
 }
 
 }  // namespace mg

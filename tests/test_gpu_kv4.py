@@ -365,6 +365,236 @@ def test_strides_streams_and_empty_batches(cuda):
     assert ops.dequantize_kv4(*cache, lengths, 0, 1)[0].shape == (2, 2, 0, 128)
 
 
+# ---- many rows: enough of them, over all heads, that 256 rows share an entry's operands -----------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b, seq, kv, group", [(20, 33, 5, 1), (5, 130, 3, 4), (3, 257, 4, 3), (10, 70, 2, 8), (1, 1200, 4, 1)])
+def test_attention_of_many_rows(cuda, dtype, d, b, seq, kv, group):
+    """Prompts of which some are padded on the left (rows that see nothing), later pieces, sequences of one entry and of none."""
+    lengths = ([seq, seq + 61, max(1, seq // 2), 0, 1, 129, seq + 200] * 3)[:b]
+    check_attention(cuda, dtype, d, b, seq, kv, group, lengths, seed=seq)
+
+
+@pytest.mark.parametrize("window, sinks", [(1, 0), (1, 3), (17, 1), (64, 0), (65, 64), (128, 129), (200, 4), (1000, 5), (0, 7)])
+def test_attention_of_many_rows_with_a_window(cuda, window, sinks):
+    check_attention(cuda, torch.float16, 128, 4, 150, 8, 2, [450, 331, 150, 149], window, sinks, capacity=512, seed=window)
+    check_attention(cuda, torch.bfloat16, 64, 4, 150, 8, 2, [450, 331, 20, 0], window, sinks, capacity=512, seed=window + 1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("q_size, v_size", [(30.0, 1.0), (1e-3, 1.0), (1.5, 1e-4), (1.5, 200.0), (0.0, 1.0)])
+def test_attention_of_large_and_small_values_in_many_rows(cuda, dtype, q_size, v_size):
+    check_attention(cuda, dtype, 128, 2, 160, 8, 2, [300, 160], q_size=q_size, v_size=v_size, seed=6)
+
+
+def test_attention_of_many_rows_over_scales_that_vary_widely(cuda):
+    """As test_attention_of_scales_that_vary_widely; the unit of a tile's weights rises and what was added up follows it."""
+    from matgptq_b200 import ops
+    dtype, d, n, kv = torch.bfloat16, 128, 400, 8
+    gen = torch.Generator(device=cuda).manual_seed(8)
+    cache = filled_cache(1, kv, 448, d, dtype, [n], cuda, gen)
+    power = 2.0 ** torch.randint(-40, 41, (kv, n, 1), generator=gen, device=cuda)
+    cache[2][0, :, :n, 2:] = (cache[2][0, :, :n, 2:].float() * power).to(dtype)
+    q = torch.randn(1, 160, kv * 4, d, generator=gen, device=cuda).to(dtype)
+    out = ops.attention_kv4(q, *cache, lengths_tensor([n], cuda), 0, 0, 0.1, 3)
+    want, _, near, _ = oracle.attention(q, *cache, [n], 0, 0, 0.1)
+    assert ((out.double() - want).abs() <= near * 1.01 + want.abs() * half_step(dtype) * 1.01).all()
+
+
+def test_nan_reaches_the_rows_that_see_it_among_many(cuda):
+    """As test_nan_reaches_the_rows_that_see_it_and_no_others.  Beside a NaN the other rows keep their bits.  An infinite score makes its
+    warp take all its rows' weights against new maxima: by whole powers of two, so with the same error bound, but the exponents
+    score - maximum are rounded elsewhere, by half a step of fp32 of the larger of the two: these rows are held to the bound, not the bits."""
+    from matgptq_b200 import ops
+    dtype, d, kv, group, capacity, seq, b = torch.float16, 64, 1, 2, 192, 40, 64
+    n = [150] * b
+    for column in range(4):
+        gen = torch.Generator(device=cuda).manual_seed(column)
+        cache = filled_cache(b, kv, capacity, d, dtype, n, cuda, gen)
+        q = torch.randn(b, seq, group, d, generator=gen, device=cuda).to(dtype)
+        clean = ops.attention_kv4(q, *cache, lengths_tensor(n, cuda), 20, 2, 0.1, 1)
+        want, _, near, _ = oracle.attention(q, *cache, n, 20, 2, 0.1)
+        bound = near + want.abs() * half_step(dtype) * (1 + half_step(dtype)) + near * half_step(dtype) + torch.finfo(dtype).smallest_normal * half_step(dtype) * 2
+        bad = [(150 - 1, 150 - seq, 150 - seq - 5, 60, 1, 128)[i % 6] for i in range(b)]
+        for i, j in enumerate(bad):
+            cache[2][i, 0, j, column] = math.nan if i % 2 else math.inf
+        out = ops.attention_kv4(q, *cache, lengths_tensor(n, cuda), 20, 2, 0.1, 1)
+        for i, j in enumerate(bad):
+            seen = oracle.visible(150, seq, 20, 2)[:, j]
+            assert ((out[i].double() - want[i]).abs() <= bound[i])[~seen].all(), (column, i)
+            if i % 2:
+                assert torch.equal(out[i, ~seen], clean[i, ~seen]), (column, i)
+                assert out[i].isnan().all(-1).all(-1).cpu().tolist() == seen.tolist(), (column, i)
+
+
+def test_attention_of_many_rows_has_one_order(cuda):
+    from matgptq_b200 import ops
+    gen = torch.Generator(device=cuda).manual_seed(9)
+    n = [2048, 1000, 377]
+    cache = filled_cache(3, 4, 2048, 128, torch.float16, n, cuda, gen)
+    q = torch.randn(3, 300, 16, 128, generator=gen, device=cuda).half()
+    runs = []
+    for _ in range(4):
+        w = torch.zeros(3, 4, 2048, device=cuda)
+        runs.append((ops.attention_kv4(q, *cache, lengths_tensor(n, cuda), 0, 0, 0.1, 1, w), w))
+    for out, w in runs[1:]:
+        assert torch.equal(out, runs[0][0]) and torch.equal(w, runs[0][1])
+
+
+# ---- long caches: segments that are cut into pieces --------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("seq, group", [(1, 1), (1, 8), (1, 12), (2, 10), (9, 11)])
+def test_attention_over_a_long_cache(cuda, dtype, seq, group):
+    """One tile of rows and several, a sequence without entries and a short one beside the long one, everything and a window."""
+    check_attention(cuda, dtype, 64, 1, seq, 1, group, [20001], seed=seq)
+    check_attention(cuda, dtype, 64, 3, seq, 1, group, [33, 18000, 0], seed=seq + 1)
+    check_attention(cuda, dtype, 128, 1, seq, 1, group, [20480], 17000, 70, seed=seq + 2)
+
+
+@pytest.mark.parametrize("seq, group", [(1, 4), (4, 5)])
+def test_attention_over_the_caches_of_many_sequences(cuda, seq, group):
+    """More sequences than a warp has lanes, more segments than CTAs run at once, lengths from none to all."""
+    b = 45
+    lengths = [(i * 397) % 2241 for i in range(b)]
+    check_attention(cuda, torch.bfloat16, 64, b, seq, 8, group, lengths, capacity=2240, seed=seq)
+    check_attention(cuda, torch.float16, 64, b, seq, 1, group, lengths[:44] + [17000], capacity=17024, seed=seq + 1, weighted=seq > 1)
+
+
+def test_entries_past_four_gigabytes(cuda):
+    """Offsets that pass 32 bits: the last entries of the second head of a cache of 2**26 entries do what they do in a small one."""
+    from matgptq_b200 import ops
+    d, kv, group, capacity, small = 128, 2, 2, 2 ** 26, 512
+    if torch.cuda.mem_get_info()[0] < 24e9:
+        pytest.skip("needs 24 GB")
+    dtype, gen = torch.float16, torch.Generator(device=cuda).manual_seed(3)
+    part = filled_cache(1, kv, small, d, dtype, [small - 3], cuda, gen)
+    cache = [torch.empty(1, kv, capacity // r, t.shape[-1], dtype=t.dtype, device=cuda) for r, t in zip((1, 2, 1), part)]
+    for t, s in zip(cache, part):
+        t[:, :, -s.shape[2]:] = s
+    scale = 0.1
+    for seq in (1, 20, 1300):
+        rows = min(seq, 100)
+        q = torch.randn(1, seq, kv * group, d, generator=gen, device=cuda).half()
+        n = capacity - 3
+        if seq >= small:  # the first tokens' windows lie in front of what is compared
+            for t, r in zip(cache, (1, 2, 1)):
+                t[:, :, (capacity - 4096) // r:(capacity - small) // r] = 0
+        out = ops.attention_kv4(q, *cache, lengths_tensor([n], cuda), 100, 0, scale, 1)[:, -rows:]
+        want, _, near, _ = oracle.attention(q[:, -rows:].contiguous(), *part, [small - 3], 100, 0, scale)
+        bound = near + want.abs() * half_step(dtype) * (1 + half_step(dtype)) + near * half_step(dtype) + torch.finfo(dtype).smallest_normal * half_step(dtype) * 2
+        assert ((out.double() - want).abs() <= bound).all(), seq
+    # three more, written and read back
+    qkv = torch.randn(3, (kv * group + 2 * kv) * d, generator=gen, device=cuda).half()
+    cos, sin = plain_tables(4, d, cuda)
+    for t, length in ((cache, capacity), (part, small)):
+        ops.append_kv4(qkv, torch.arange(3, device=cuda), cos, sin, lengths_tensor([length], cuda), *t, kv * group, 1)
+    for big, little in zip(ops.dequantize_kv4(*cache, lengths_tensor([capacity], cuda), 20, 1), ops.dequantize_kv4(*part, lengths_tensor([small], cuda), 20, 1)):
+        assert torch.equal(big, little)
+    # and the last ones kept
+    weights = torch.zeros(1, kv, capacity, device=cuda)
+    weights[:, :, -small:] = 1 + torch.rand(1, kv, small, generator=gen, device=cuda)
+    order = weights[0, :, -small:].clone()
+    rows = oracle.unpack_k(part[0])
+    new, kept = ops.evict_kv4(*cache, weights, lengths_tensor([capacity], cuda), 100, 0, 0, 0, 1)
+    for head in range(kv):
+        at = order[head].topk(100).indices.sort().values
+        assert (kept[0, head] == at + capacity - small).all()
+        assert torch.equal(oracle.unpack_k(cache[0][:, :, :128])[0, head, :100], rows[0, head, at])
+    assert new.tolist() == [100] and status() == 0
+
+
+# ---- ways to call ------------------------------------------------------------------------------------------------------
+def test_the_operators_with_and_without_a_dispatch_mode(cuda):
+    """A mode sees every one of them, and what they answer is the same; what they write to is marked as written."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from matgptq_b200 import ops
+
+    class Seen(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.names = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.append(func._schema.name.split("::")[-1])
+            return func(*args, **(kwargs or {}))
+
+    b, seq, heads, kv, d, capacity = 2, 3, 4, 2, 64, 64
+    gen = torch.Generator(device=cuda).manual_seed(5)
+    qkv = torch.randn(b * seq, (heads + 2 * kv) * d, generator=gen, device=cuda).half()
+    cos, sin = plain_tables(seq, d, cuda)
+    n, positions = lengths_tensor([9, 5], cuda), torch.arange(seq, device=cuda)
+
+    def run():
+        start = torch.Generator(device=cuda).manual_seed(6)
+        cache = filled_cache(b, kv, capacity, d, torch.float16, [6, 2], cuda, start)
+        weights = torch.zeros(b, kv, capacity, device=cuda)
+        versions = [t._version for t in (*cache, weights)]
+        q = ops.append_kv4(qkv, positions, cos, sin, n, *cache, heads, 1)
+        out = ops.attention_kv4(q, *cache, n, 4, 1, 0.125, 1, weights)
+        new, kept = ops.evict_kv4(*cache, weights, n, 4, 0, 1, 1, 1)
+        k, v = ops.dequantize_kv4(*cache, new, 4, 1)
+        assert all(t._version > old for t, old in zip((*cache, weights), versions))
+        return q, out, new, kept, k, v, weights
+
+    plain = run()
+    with Seen() as mode:
+        moded = run()
+    assert all(torch.equal(x, y) for x, y in zip(plain, moded))
+    assert all(any(name == want for name in mode.names) for want in ("append_kv4", "attention_kv4", "evict_kv4", "dequantize_kv4"))
+
+
+def test_two_streams_at_once(cuda):
+    """Calls in flight at the same time have workspaces of their own."""
+    from matgptq_b200 import ops
+    gen = torch.Generator(device=cuda).manual_seed(13)
+    n = lengths_tensor([20000], cuda)
+    caches = [filled_cache(1, 1, 20032, 64, torch.float16, [20000], cuda, gen) for _ in range(2)]
+    qs = [torch.randn(1, 1, 8, 64, generator=gen, device=cuda).half() for _ in range(2)]
+    want = [ops.attention_kv4(q, *c, n, 0, 0, 0.1, 1) for q, c in zip(qs, caches)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.attention_kv4(qs[i], *caches[i], n, 0, 0, 0.1, 1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])
+
+
+def test_two_graphs_replayed_in_turn(cuda):
+    """Captured calls with workspaces, in two graphs of one pool, replayed one after the other and again with other lengths."""
+    from matgptq_b200 import ops
+    gen = torch.Generator(device=cuda).manual_seed(14)
+    cache = filled_cache(2, 1, 20032, 64, torch.float16, [20000, 19000], cuda, gen)
+    q1, q2 = (torch.randn(2, s, 8, 64, generator=gen, device=cuda).half() for s in (1, 70))
+    n = lengths_tensor([20000, 17000], cuda)
+    ws = [torch.zeros(2, 1, 20032, device=cuda) for _ in range(2)]
+
+    def eager():
+        w = [torch.zeros_like(x) for x in ws]
+        return [ops.attention_kv4(q, *cache, n, 0, 0, 0.1, 1, x) for q, x in zip((q1, q2), w)] + w
+
+    eager()
+    graphs, outs = [], []
+    for q, w in zip((q1, q2), ws):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=graphs[0].pool() if graphs else None):
+            outs.append(ops.attention_kv4(q, *cache, n, 0, 0, 0.1, 1, w))
+        graphs.append(g)
+    for lengths in ([20000, 17000], [100, 19000], [0, 71]):
+        n.copy_(lengths_tensor(lengths, cuda))
+        for w in ws:
+            w.zero_()
+        want = eager()
+        for g, out, expected in zip(graphs, outs, want):
+            g.replay()
+            assert torch.equal(out, expected)
+        assert all(torch.equal(x, y) for x, y in zip(ws, want[2:]))
+
+
 # ---- eviction --------------------------------------------------------------------------------------------------------
 def check_eviction(cuda, weights, lengths, keep, slack=0, sinks=0, recent=0, d=64, dtype=torch.float16):
     from matgptq_b200 import ops
