@@ -27,7 +27,8 @@ namespace mg {
 
 MG_DEFINE_STATUS_ACCESSOR(kv4_prompt_device_status)
 
-constexpr int kPrRows = 256, kPrTile = 128, kPrStep = 64;  // rows of a CTA, entries of a tile and of a step of softmax
+constexpr int kPrRows = 256, kPrTile = 128, kPrStep = 64;  // rows of a CTA at most, entries of a tile and of a step of softmax
+constexpr int kPrSms = 148;  // of a B200, one CTA each
 constexpr int kPrProducers = 2;
 constexpr int kPrWarps = 12;                  // 8 of softmax, the producers, 1 that issues (1 idle: registers are dealt out to four warps)
 // Shared memory: barriers, Q, two stages of K, V and params.
@@ -303,7 +304,7 @@ __device__ __forceinline__ bool prompt_step(PromptRows &r, uint32_t t_s, uint32_
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4AttentionParams p) {
+__global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4AttentionParams p, const int rows) {
   using Plan = PromptPlan<D>;
   extern __shared__ __align__(1024) unsigned char prompt_smem[];
   const uint32_t base = smem_u32(prompt_smem);
@@ -336,11 +337,12 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
   pdl_prologue();
 
   const int bh = blockIdx.x, b = bh / p.cache.kv_heads, h = bh - b * p.cache.kv_heads;
-  const int total = p.seq * p.group;
-  const int r0 = (gridDim.y - 1 - blockIdx.y) * kPrRows;  // the tiles with the most entries first, of all heads
+  const int all_rows = p.seq * p.group;
+  const int r0 = (gridDim.y - 1 - blockIdx.y) * rows;  // the tiles with the most entries first, of all heads
+  const int total = min(all_rows, r0 + rows), halves = total - r0 > 128 ? 2 : 1;
   const int length = kv4_length(p.lengths, b, p.cache.capacity);
   const size_t first = static_cast<size_t>(bh) * p.cache.capacity;
-  const int pos_lo = length - p.seq + r0 / p.group, pos_hi = length - p.seq + (min(r0 + kPrRows, total) - 1) / p.group;
+  const int pos_lo = length - p.seq + r0 / p.group, pos_hi = length - p.seq + (total - 1) / p.group;
   // the tiles that the rows see: those of first entries, then those of the window
   const Kv4Range range = kv4_range<kPrTile>(pos_lo, pos_hi, p.window, p.sinks, p.cache.capacity);
   const int tiles = range.blocks;
@@ -359,7 +361,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
     // this row's tile for the pass that adds up the weights, where there is one
     uint8_t *tile_out = nullptr;
     if (p.row_tiles != nullptr && r0 + half * 128 < total)
-      tile_out = p.row_tiles + (static_cast<size_t>(bh) * ((total + 127) / 128) + (r0 >> 7) + half) * kv4_row_tile_bytes(D);
+      tile_out = p.row_tiles + (static_cast<size_t>(bh) * ((all_rows + 127) / 128) + (r0 >> 7) + half) * kv4_row_tile_bytes(D);
     float unit, sum;
     const uint32_t q_at = (quad * 32 + lane) * 16, dst = base + Plan::q + half * Plan::q_bytes + q_at;
     kv4_operand_row<T, D>(p.q + out_at, live, p.scale_log2, unit, sum, [&](int c, const uint4 &chunk) {
@@ -392,7 +394,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
     }
     r.unset = true;
     r.v_unit = 0.f;
-    for (int u = 0; u < 2 * tiles; ++u) {  // 64 entries
+    for (int u = 0; u < 2 * tiles && half < halves; ++u) {  // 64 entries
       const int t = u >> 1, stage = t & 1, buf = u & 1;
       if (!mbar_wait_chain(base + kPrBarS + 16 * half + 8 * buf, (u >> 1) & 1) || (buf == 0 && !mbar_wait_chain(base + kPrBarVFull + 8 * stage, (t >> 1) & 1))) {
         failed = true;
@@ -588,10 +590,8 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
         if (!mbar_wait_chain(base + kPrBarQ, 0) || !mbar_wait_chain(base + kPrBarKFull, 0)) failed = true;
         tc_fence_after();
         if (!failed && elect_one()) {
-          scores(0, 0);
-          scores(1, 0);
-          scores(0, 1);
-          scores(1, 1);
+          for (int buf = 0; buf < 2; ++buf)
+            for (int half = 0; half < halves; ++half) scores(half, buf);
         }
         __syncwarp();
       }
@@ -603,7 +603,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
           failed = true;
           break;
         }
-        for (int half = 0; half < 2; ++half) {
+        for (int half = 0; half < halves; ++half) {
           if (!mbar_wait_chain(base + kPrBarP + 16 * half + 8 * buf, (u >> 1) & 1)) {
             failed = true;
             break;
@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
               mma_ts(tmem + 256 + half * D, tmem + half * 128 + buf * kPrStep + k * 8,
                      dv + stage * (2 * Plan::k_bytes >> 4) + (buf * (kPrStep / 16) + k) * (2 * kChunkV >> 4), idesc_o, (u > 0 || k > 0) ? 1u : 0u);
             umma_commit(base + kPrBarO + 8 * half);
-            if (half == 1 && buf == 1) umma_commit(base + kPrBarEmpty + 8 * stage);
+            if (half == halves - 1 && buf == 1) umma_commit(base + kPrBarEmpty + 8 * stage);
             if (more) scores(half, u + 2);
           }
           __syncwarp();
@@ -876,7 +876,11 @@ template <typename T, int D> int launch_prompt(const Kv4AttentionParams &p, bool
   const int st = opt_in.ensure(kv4_prompt_kernel<T, D>, smem);
   if (st != MG_OK) return st;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.cache.batch * p.cache.kv_heads, (p.seq * p.group + kPrRows - 1) / kPrRows);
+  const int heads = p.cache.batch * p.cache.kv_heads, all = p.seq * p.group;
+  // Half as many rows a CTA while these run at once: a half alone takes 0.8 of the time of two.  1024 rows of 8 heads of 8192 entries
+  // (64 CTAs) 140 us, with 256 rows 181; of 48 heads (384 CTAs) 413 and 358.
+  const int rows = static_cast<long long>(heads) * ((all + 127) / 128) <= kPrSms ? 128 : kPrRows;
+  cfg.gridDim = dim3(heads, (all + rows - 1) / rows);
   cfg.blockDim = dim3(kPrWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -885,7 +889,7 @@ template <typename T, int D> int launch_prompt(const Kv4AttentionParams &p, bool
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
-  if (cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, p) != cudaSuccess) return MG_ERR_CUDA;
+  if (cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, p, rows) != cudaSuccess) return MG_ERR_CUDA;
   return p.weights != nullptr ? launch_weights<T, D>(p, stream) : MG_OK;
 }
 

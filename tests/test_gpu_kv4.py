@@ -368,29 +368,33 @@ def test_strides_streams_and_empty_batches(cuda):
 # ---- many rows: enough of them, over all heads, that 256 rows share an entry's operands -----------------------------------
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("b, seq, kv, group", [(20, 33, 5, 1), (5, 130, 3, 4), (3, 257, 4, 3), (10, 70, 2, 8), (1, 1200, 4, 1)])
+@pytest.mark.parametrize("b, seq, kv, group", [(20, 33, 5, 1), (5, 130, 3, 4), (3, 257, 4, 3), (10, 70, 2, 8), (1, 1200, 4, 1),
+                                               (8, 300, 10, 2), (19, 33, 8, 8), (160, 35, 1, 1)])
 def test_attention_of_many_rows(cuda, dtype, d, b, seq, kv, group):
     """Prompts of which some are padded on the left (rows that see nothing), later pieces, sequences of one entry and of none."""
-    lengths = ([seq, seq + 61, max(1, seq // 2), 0, 1, 129, seq + 200] * 3)[:b]
+    lengths = ([seq, seq + 61, max(1, seq // 2), 0, 1, 129, seq + 200] * 23)[:b]
     check_attention(cuda, dtype, d, b, seq, kv, group, lengths, seed=seq)
 
 
 @pytest.mark.parametrize("window, sinks", [(1, 0), (1, 3), (17, 1), (64, 0), (65, 64), (128, 129), (200, 4), (1000, 5), (0, 7)])
-def test_attention_of_many_rows_with_a_window(cuda, window, sinks):
-    check_attention(cuda, torch.float16, 128, 4, 150, 8, 2, [450, 331, 150, 149], window, sinks, capacity=512, seed=window)
-    check_attention(cuda, torch.bfloat16, 64, 4, 150, 8, 2, [450, 331, 20, 0], window, sinks, capacity=512, seed=window + 1)
+@pytest.mark.parametrize("kv", [8, 20])  # few CTAs of 128 rows, more of 256
+def test_attention_of_many_rows_with_a_window(cuda, window, sinks, kv):
+    check_attention(cuda, torch.float16, 128, 4, 150, kv, 2, [450, 331, 150, 149], window, sinks, capacity=512, seed=window)
+    check_attention(cuda, torch.bfloat16, 64, 4, 150, kv, 2, [450, 331, 20, 0], window, sinks, capacity=512, seed=window + 1)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("q_size, v_size", [(30.0, 1.0), (1e-3, 1.0), (1.5, 1e-4), (1.5, 200.0), (0.0, 1.0)])
-def test_attention_of_large_and_small_values_in_many_rows(cuda, dtype, q_size, v_size):
-    check_attention(cuda, dtype, 128, 2, 160, 8, 2, [300, 160], q_size=q_size, v_size=v_size, seed=6)
+@pytest.mark.parametrize("kv", [8, 26])
+def test_attention_of_large_and_small_values_in_many_rows(cuda, dtype, q_size, v_size, kv):
+    check_attention(cuda, dtype, 128, 2, 160, kv, 2, [300, 160], q_size=q_size, v_size=v_size, seed=6)
 
 
-def test_attention_of_many_rows_over_scales_that_vary_widely(cuda):
+@pytest.mark.parametrize("kv", [8, 40])
+def test_attention_of_many_rows_over_scales_that_vary_widely(cuda, kv):
     """As test_attention_of_scales_that_vary_widely; the unit of a tile's weights rises and what was added up follows it."""
     from matgptq_b200 import ops
-    dtype, d, n, kv = torch.bfloat16, 128, 400, 8
+    dtype, d, n = torch.bfloat16, 128, 400
     gen = torch.Generator(device=cuda).manual_seed(8)
     cache = filled_cache(1, kv, 448, d, dtype, [n], cuda, gen)
     power = 2.0 ** torch.randint(-40, 41, (kv, n, 1), generator=gen, device=cuda)
@@ -401,12 +405,13 @@ def test_attention_of_many_rows_over_scales_that_vary_widely(cuda):
     assert ((out.double() - want).abs() <= near * 1.01 + want.abs() * half_step(dtype) * 1.01).all()
 
 
-def test_nan_reaches_the_rows_that_see_it_among_many(cuda):
+@pytest.mark.parametrize("b, group", [(64, 2), (100, 4)])
+def test_nan_reaches_the_rows_that_see_it_among_many(cuda, b, group):
     """As test_nan_reaches_the_rows_that_see_it_and_no_others.  Beside a NaN the other rows keep their bits.  An infinite score makes its
     warp take all its rows' weights against new maxima: by whole powers of two, so with the same error bound, but the exponents
     score - maximum are rounded elsewhere, by half a step of fp32 of the larger of the two: these rows are held to the bound, not the bits."""
     from matgptq_b200 import ops
-    dtype, d, kv, group, capacity, seq, b = torch.float16, 64, 1, 2, 192, 40, 64
+    dtype, d, kv, capacity, seq = torch.float16, 64, 1, 192, 40
     n = [150] * b
     for column in range(4):
         gen = torch.Generator(device=cuda).manual_seed(column)
@@ -427,12 +432,13 @@ def test_nan_reaches_the_rows_that_see_it_among_many(cuda):
                 assert out[i].isnan().all(-1).all(-1).cpu().tolist() == seen.tolist(), (column, i)
 
 
-def test_attention_of_many_rows_has_one_order(cuda):
+@pytest.mark.parametrize("group", [4, 8])
+def test_attention_of_many_rows_has_one_order(cuda, group):
     from matgptq_b200 import ops
     gen = torch.Generator(device=cuda).manual_seed(9)
     n = [2048, 1000, 377]
     cache = filled_cache(3, 4, 2048, 128, torch.float16, n, cuda, gen)
-    q = torch.randn(3, 300, 16, 128, generator=gen, device=cuda).half()
+    q = torch.randn(3, 300, 4 * group, 128, generator=gen, device=cuda).half()
     runs = []
     for _ in range(4):
         w = torch.zeros(3, 4, 2048, device=cuda)
