@@ -13,7 +13,10 @@
 // v_scale.  The codes of V are centred first: their mean would multiply that rounding, and the tensor cores would sum up numbers of
 // one sign, which over 131072 entries cost three bits of the result.  Row maximum and sums are fp32.
 //
-// This file: up to kKv4FewRows rows, as in decoding.  The entries are read once and that is what bounds it.
+// This file: few rows (few_rows below), as in decoding: the entries are read once, or once for each 16 rows.  What bounds it at 8 rows
+// and long caches is half memory, half instructions (19 a warp and entry, 54 % of the issue slots): one sequence of 131001 entries of 8
+// heads of 128 channels 37.9 us, 3.76 TB/s; 32 sequences of 1089 to 4096 entries 27.9 us, 3.25 TB/s; 129 entries 5.5 us, which are one CTA's
+// latencies.  With a row's weights added up in the same launch: 8 sequences of 2048 entries 13.7 us for 11.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -153,9 +156,10 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
 //
 // A segment is a tile of R = 8 or 16 rows of one key/value head of one sequence, its work the blocks of 32 entries that these rows
 // see.  Segments of few blocks get a CTA each, or a cluster of CTAs as long as there are SMs for it, whose results are joined through
-// distributed shared memory.  Otherwise a segment is cut into pieces of equal size, none larger than a share that
-// makes at most `kStepCtas` pieces of all the work, where there are not more segments already; each piece is a CTA, leaves a partial result, and kv4_finish_kernel joins them in
-// their order.  Lengths are known on the device only: every CTA works out by itself which piece is its own, and the grid is as large as
+// distributed shared memory (2048 entries of 8 heads 7.8 us, cut into pieces 12.9).  Otherwise a segment is cut into pieces of equal size,
+// none larger than a share that makes at most `kStepCtas` pieces of all the work, where there are not more segments already; each piece is
+// a CTA, leaves a partial result, and kv4_finish_kernel joins them in their order.  Lengths are known on the device only: every CTA
+// works out by itself which piece is its own, and the grid is as large as
 // the pieces can become.  (A CTA that goes on into the next segment, for shares that are all equal, has the latencies of a second
 // beginning and end one after the other: 16384 entries of 8 heads 19.6 us.)
 constexpr int kStepWarps = 8;
@@ -163,7 +167,6 @@ constexpr int kStepBlock = 32;       // entries of a block
 constexpr int kStepStages = 3;       // blocks in flight per warp
 constexpr int kStepCtas = 296;       // two on each SM of a B200
 constexpr int kStepLeast = kStepWarps;  // blocks of a share at least: one for each warp
-constexpr int kStepWhole = 64;          // blocks of a CTA up to which segments are not cut
 
 struct Kv4StepParams {
   Kv4AttentionParams a;
@@ -844,7 +847,12 @@ StepPlan step_plan(const Kv4Cache &c, int seq, int group, int window, int sinks,
   // CTAs for a segment while they all run at once and each warp of them has a block
   int cluster = 1;
   while (cluster < 8 && s.segments * cluster * 2 <= kStepCtas && cluster * 2 * kStepWarps <= blocks) cluster *= 2;
-  s.cluster = (blocks + cluster - 1) / cluster <= kStepWhole || s.segments >= 4 * kStepCtas ? cluster : 0;
+  // Cutting evens out what unequal lengths and too few segments leave uneven, and costs a launch and its results' way through memory:
+  // blocks a CTA 32, 64 CTAs 10.8 us, cut 12.7 (one sequence of 8192 entries); 128 of 64 22.5 and 18.0; 256 CTAs of 128 blocks, lengths
+  // from 124 to 4096, 26.2 and 32.3, with weights 37.8 and 74; 1200 CTAs of 128 141 and 176.  The upper limit is for one sequence that is
+  // far longer than the others: 256 blocks are 37 us.
+  const int most = std::min(std::max(s.segments * cluster, 32), 256);
+  s.cluster = (blocks + cluster - 1) / cluster <= most || s.segments >= 4 * kStepCtas ? cluster : 0;
   // pieces of all segments: blocks / share and one for what is left over, each; shares are at least all blocks / kStepCtas
   s.slots = s.cluster > 0 ? s.segments : s.segments + kStepCtas;
   s.pieces_bytes = s.cluster > 0 ? 0 : (s.segments * 8 + 15) / 16 * 16;

@@ -466,6 +466,13 @@ def test_attention_over_the_caches_of_many_sequences(cuda, seq, group):
     check_attention(cuda, torch.float16, 64, b, seq, 1, group, lengths[:44] + [17000], capacity=17024, seed=seq + 1, weighted=seq > 1)
 
 
+@pytest.mark.parametrize("b, seq, group, weighted", [(149, 1, 3, True), (149, 1, 16, False), (80, 4, 5, True)])
+def test_attention_over_pieces_of_many_sequences(cuda, b, seq, group, weighted):
+    """Long enough for pieces; more sequences than a warp has lanes, lengths from none to all."""
+    lengths = [(i * 1237) % 5313 for i in range(b)]
+    check_attention(cuda, torch.bfloat16, 64, b, seq, 1, group, lengths, capacity=5312, seed=b + seq, weighted=weighted)
+
+
 def test_entries_past_four_gigabytes(cuda):
     """Offsets that pass 32 bits: the last entries of the second head of a cache of 2**26 entries do what they do in a small one."""
     from matgptq_b200 import ops
