@@ -302,6 +302,7 @@ matgptq_b200_kv4_cache check_kv4(const char *what, const Tensor &k_codes, const 
   TORCH_CHECK(k_codes.scalar_type() == at::kByte && k_codes.dim() == 4, what, ": k_codes must be uint8 of shape (B, KV, capacity, d/2)");
   const int64_t b = k_codes.size(0), kv = k_codes.size(1), capacity = k_codes.size(2), d = 2 * k_codes.size(3);
   TORCH_CHECK(d == 64 || d == 128, what, ": the head dimension must be 64 or 128, got ", d);
+  TORCH_CHECK(kv > 0, what, ": the cache must have at least one key/value head");
   TORCH_CHECK(capacity > 0 && capacity % 64 == 0, what, ": the capacity must be a multiple of 64, got ", capacity);
   TORCH_CHECK(v_codes.scalar_type() == at::kByte && v_codes.sizes() == at::IntArrayRef({b, kv, capacity / 2, d}), what,
               ": v_codes must be uint8 of shape (", b, ", ", kv, ", ", capacity / 2, ", ", d, ")");

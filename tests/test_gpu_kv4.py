@@ -822,6 +822,17 @@ def test_two_captured_graphs_do_not_share_state(cuda):
             assert torch.equal(out, want) and torch.equal(w, want_w)
 
 
+def test_a_cache_without_heads_is_refused(cuda):
+    """By a message: the number of heads is divided by the cache's."""
+    from matgptq_b200 import ops
+    cache = [t[:, :0] for t in empty_cache(2, 1, 64, 64, torch.float16, cuda)]
+    n = lengths_tensor([1, 1], cuda)
+    for call in (lambda: ops.attention_kv4(torch.zeros(2, 1, 4, 64, dtype=torch.float16, device=cuda), *cache, n, 0, 0, 1.0, 1),
+                 lambda: ops.dequantize_kv4(*cache, n, 1, 1), lambda: ops.evict_kv4(*cache, torch.zeros(2, 0, 64, device=cuda), n, 1, 0, 0, 0, 1)):
+        with pytest.raises(RuntimeError, match="at least one key/value head"):
+            call()
+
+
 @pytest.mark.parametrize("name", ["append_kv4", "attention_kv4", "evict_kv4", "dequantize_kv4"])
 def test_schema_and_fake_agree(cuda, name):
     gen = torch.Generator(device=cuda).manual_seed(41)
