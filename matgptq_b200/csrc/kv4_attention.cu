@@ -136,12 +136,6 @@ __device__ __forceinline__ void kv4_scores(float (&s)[4], const uint32_t (&k0)[D
   }
 }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
-  return v;
-}
-
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -157,7 +151,7 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
 // A segment is a tile of R = 8 or 16 rows of one key/value head of one sequence, its work the blocks of 32 entries that these rows
 // see.  Segments of few blocks get a CTA each, or a cluster of CTAs as long as there are SMs for it, whose results are joined through
 // distributed shared memory (2048 entries of 8 heads 7.8 us, cut into pieces 12.9).  Otherwise a segment is cut into pieces of equal size,
-// none larger than a share that makes at most `kStepCtas` pieces of all the work, where there are not more segments already; each piece is
+// none larger than a share that makes at most `step_ctas` pieces of all the work, where there are not more segments already; each piece is
 // a CTA, leaves a partial result, and kv4_finish_kernel joins them in their order.  Lengths are known on the device only: every CTA
 // works out by itself which piece is its own, and the grid is as large as
 // the pieces can become.  (A CTA that goes on into the next segment, for shares that are all equal, has the latencies of a second
@@ -165,7 +159,8 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
 constexpr int kStepWarps = 8;
 constexpr int kStepBlock = 32;       // entries of a block
 constexpr int kStepStages = 3;       // blocks in flight per warp
-constexpr int kStepCtas = 296;       // two on each SM of a B200
+// CTAs that run at once on a B200: two on each SM, one with tiles of 16 rows
+__host__ __device__ constexpr int step_ctas(int rows) { return rows == 8 ? 296 : 148; }
 constexpr int kStepLeast = kStepWarps;  // blocks of a share at least: one for each warp
 
 struct Kv4StepParams {
@@ -218,18 +213,19 @@ template <int R> __device__ __forceinline__ bool step_find(StepPiece &s, const K
     return step_range<R>(p.a, length, i - b * p.tiles).blocks;
   };
   const auto sum = [&](auto of) {
-    uint32_t x = 0;  // (296 tiles of 2^28 entries pass 31 bits)
+    uint32_t x = 0;  // (148 tiles of 2^28 entries pass 30 bits)
     int length;
     for (int i = lane; i < tiles; i += 32) x += of(blocks_of(i, length));
     return warp_sum(x) * kv;
   };
   const uint32_t all = sum([](int blocks) { return blocks; });
   const int segments = tiles * kv;
-  const int room = segments < kStepCtas ? kStepCtas - segments / 2 : kStepCtas;
+  constexpr int kCtas = step_ctas(R);
+  const int room = segments < kCtas ? kCtas - segments / 2 : kCtas;
   int share = max(static_cast<int>((all + room - 1) / room), kStepLeast);
   const auto cut = [&](int blocks) { return (blocks + share - 1) / share; };
-  if (segments < kStepCtas)
-    for (int i = 0; i < 16 && sum(cut) > kStepCtas; ++i) share += max(share >> 4, 1);
+  if (segments < kCtas)
+    for (int i = 0; i < 16 && sum(cut) > kCtas; ++i) share += max(share >> 4, 1);
   int before = 0;
   for (int i0 = 0; i0 < tiles; i0 += 32) {
     int length = 0, pieces = 0;
@@ -830,12 +826,11 @@ int step_blocks(const Kv4Cache &c, int seq, int window, int sinks) {
 }
 
 // Whether the kernels of this file take the rows.  A head's rows are 16 in a tile here, each of which goes over the entries anew, and
-// 256 in kv4_prompt.cu, one CTA with all their entries: with few tiles the one keeps more SMs busy, with many the other does less work.
-// 8 heads of 4096 entries, here and there: 128 rows 27 and 92 us, 512 rows 64 and 97, 1024 rows 123 and 97; 16 sequences of these 8
-// heads, 36 rows each, 96 and 93.  Up to 32 rows, whatever the number of heads, this side was ahead: 768 heads of 2048 entries, 32
-// rows 182 and 292.
+// 128 or 256 in kv4_prompt.cu: while the tiles all run at once they are ahead here.  8 heads of 2048 entries, here and there: 64 rows
+// 11.7 and 15.3 us, 256 rows (128 tiles) 17.9 and 20.3, 512 rows 33.6 and 22.3; of 8192 entries 19.4 and 27.7, 52 and 45, 92 and 47.
+// Up to 32 rows, whatever the number of heads, this side was ahead from 1000 entries on: 768 heads of 2048 entries, 32 rows 182 and 292.
 bool few_rows(const Kv4Cache &c, int64_t rows) {
-  return rows <= kKv4FewRows || static_cast<int64_t>(c.batch) * c.kv_heads * ((rows + 15) / 16) <= kStepCtas;
+  return rows <= kKv4FewRows || static_cast<int64_t>(c.batch) * c.kv_heads * ((rows + 15) / 16) <= step_ctas(16);
 }
 
 StepPlan step_plan(const Kv4Cache &c, int seq, int group, int window, int sinks, bool weights) {
@@ -846,15 +841,16 @@ StepPlan step_plan(const Kv4Cache &c, int seq, int group, int window, int sinks,
   const int blocks = step_blocks(c, seq, window, sinks);
   // CTAs for a segment while they all run at once and each warp of them has a block
   int cluster = 1;
-  while (cluster < 8 && s.segments * cluster * 2 <= kStepCtas && cluster * 2 * kStepWarps <= blocks) cluster *= 2;
+  const int ctas = step_ctas(s.rows);
+  while (cluster < 8 && s.segments * cluster * 2 <= cluster_ctas(ctas, cluster * 2) && cluster * 2 * kStepWarps <= blocks) cluster *= 2;
   // Cutting evens out what unequal lengths and too few segments leave uneven, and costs a launch and its results' way through memory:
   // blocks a CTA 32, 64 CTAs 10.8 us, cut 12.7 (one sequence of 8192 entries); 128 of 64 22.5 and 18.0; 256 CTAs of 128 blocks, lengths
   // from 124 to 4096, 26.2 and 32.3, with weights 37.8 and 74; 1200 CTAs of 128 141 and 176.  The upper limit is for one sequence that is
   // far longer than the others: 256 blocks are 37 us.
   const int most = std::min(std::max(s.segments * cluster, 32), 256);
-  s.cluster = (blocks + cluster - 1) / cluster <= most || s.segments >= 4 * kStepCtas ? cluster : 0;
-  // pieces of all segments: blocks / share and one for what is left over, each; shares are at least all blocks / kStepCtas
-  s.slots = s.cluster > 0 ? s.segments : s.segments + kStepCtas;
+  s.cluster = (blocks + cluster - 1) / cluster <= most || s.segments >= 4 * ctas ? cluster : 0;
+  // pieces of all segments: blocks / share and one for what is left over, each; shares are at least all blocks / ctas
+  s.slots = s.cluster > 0 ? s.segments : s.segments + ctas;
   s.pieces_bytes = s.cluster > 0 ? 0 : (s.segments * 8 + 15) / 16 * 16;
   s.weighs = s.cluster > 0 && s.tiles == 1;  // the CTAs of a segment see all rows and all entries
   s.ml_bytes = s.cluster > 0 && (!weights || s.weighs) ? 0 : s.slots * 2 * s.rows * 4;

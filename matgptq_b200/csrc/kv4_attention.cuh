@@ -71,6 +71,12 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+
 // Codes of two neighbours less 8, exact: 1024 + c and 1024 + 16 c are fp16 numbers with the code in their last bits.  The constants are
 // made once, as registers: an instruction takes one literal.
 struct Centring {
@@ -144,6 +150,10 @@ __device__ __forceinline__ void kv4_row_numbers(uint8_t *all, int of, float unit
   numbers[2] = sum * unit;
   numbers[4] = l == 0.f ? -INFINITY : -(m + log2f(l));
 }
+
+// How many CTAs run at once in clusters of 2, 4 or 8, of `ctas` that do alone: a cluster's lie in one GPC, and some have fewer SMs than
+// others.  (16 clusters of 8, one CTA an SM, took two rounds, 27.9 us for 16.6 without clusters.)
+constexpr int cluster_ctas(int ctas, int cluster) { return ctas > 148 || cluster == 2 ? ctas : cluster == 4 ? 128 : 96; }
 
 // kv4_prompt.cu
 int kv4_prompt_weights_launch(const Kv4AttentionParams &p, bool bf16, cudaStream_t stream);  // from row_tiles

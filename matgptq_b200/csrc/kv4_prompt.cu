@@ -1,5 +1,6 @@
 // Attention over the 4-bit cache for many rows (the mathematics: kv4_attention.cu), on the tensor cores: a CTA takes 256 rows of one
-// key/value head (128 where there are few CTAs) and goes over tiles of 128 entries, in steps of 64.
+// key/value head (128 where there are few CTAs, in clusters that share the entries where there are fewer still) and goes over tiles of 128
+// entries, in steps of 64.
 //
 //   * two producer warps turn a tile's codes into operands in shared memory, once for both halves of the rows: K as fp16 subnormals
 //     (one mask per two codes; the codes that sit 4 bits up meet a q that was divided by 16), V centred; and its scales and minima as fp32;
@@ -35,7 +36,7 @@ namespace mg {
 MG_DEFINE_STATUS_ACCESSOR(kv4_prompt_device_status)
 
 constexpr int kPrRows = 256, kPrTile = 128, kPrStep = 64;  // rows of a CTA at most, entries of a tile and of a step of softmax
-constexpr int kPrSms = 148;  // of a B200, one CTA each
+constexpr int kPrSms = 148, kPrSplits = 4;  // of a B200, one CTA each; CTAs of a cluster at most
 constexpr int kPrProducers = 2;
 constexpr int kPrWarps = 12;                  // 8 of softmax, the producers, 1 that issues (1 idle: registers are dealt out to four warps)
 // Shared memory: barriers, Q, two stages of K, V and params.
@@ -310,8 +311,10 @@ __device__ __forceinline__ bool prompt_step(PromptRows &r, uint32_t t_s, uint32_
   return true;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4AttentionParams p, const int rows) {
+// SPLIT: a cluster of `in_cluster` CTAs has the same rows
+template <typename T, int D, bool SPLIT>
+__global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4AttentionParams p, const int rows, const int in_cluster) {
+  const int splits = SPLIT ? in_cluster : 1;
   using Plan = PromptPlan<D>;
   extern __shared__ __align__(1024) unsigned char prompt_smem[];
   const uint32_t base = smem_u32(prompt_smem);
@@ -343,7 +346,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(prompt_smem + kPrTmemSlot);
   pdl_prologue();
 
-  const int bh = blockIdx.x, b = bh / p.cache.kv_heads, h = bh - b * p.cache.kv_heads;
+  const int bh = blockIdx.x / splits, rank = blockIdx.x - bh * splits, b = bh / p.cache.kv_heads, h = bh - b * p.cache.kv_heads;
   const int all_rows = p.seq * p.group;
   const int r0 = (gridDim.y - 1 - blockIdx.y) * rows;  // the tiles with the most entries first, of all heads
   const int total = min(all_rows, r0 + rows), halves = total - r0 > 128 ? 2 : 1;
@@ -352,9 +355,11 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
   const int pos_lo = length - p.seq + r0 / p.group, pos_hi = length - p.seq + (total - 1) / p.group;
   // the tiles that the rows see: those of first entries, then those of the window
   const Kv4Range range = kv4_range<kPrTile>(pos_lo, pos_hi, p.window, p.sinks, p.cache.capacity);
-  const int tiles = range.blocks;
+  // of these, this CTA's share, where a cluster of `splits` has the same rows
+  const int tile0 = range.blocks * rank / splits, tiles = range.blocks * (rank + 1) / splits - tile0;
   constexpr uint32_t kChunkQ = 128 * 16, kChunkV = D * 16;
   bool failed = false;
+  float row_unit = 0.f, row_sum = 0.f;  // of this thread's row
 
   if (warp < kProducer) {
     // ------------------------------------------------------------------ softmax: a thread per row
@@ -367,7 +372,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
     const size_t out_at = ((static_cast<size_t>(b) * p.seq + query) * p.heads + static_cast<size_t>(h) * p.group + (live ? row - query * p.group : 0)) * D;
     // this row's tile for the pass that adds up the weights, where there is one
     uint8_t *tile_out = nullptr;
-    if (p.row_tiles != nullptr && r0 + half * 128 < total)
+    if (p.row_tiles != nullptr && rank == 0 && r0 + half * 128 < total)
       tile_out = p.row_tiles + (static_cast<size_t>(bh) * ((all_rows + 127) / 128) + (r0 >> 7) + half) * kv4_row_tile_bytes(D);
     float unit, sum;
     const uint32_t q_at = (quad * 32 + lane) * 16, dst = base + Plan::q + half * Plan::q_bytes + q_at;
@@ -375,6 +380,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
       sts_v4(dst + c * kChunkQ, chunk.x, chunk.y, chunk.z, chunk.w);
       if (tile_out != nullptr) *reinterpret_cast<uint4 *>(tile_out + c * kChunkQ + q_at) = chunk;
     });
+    row_unit = unit, row_sum = sum;
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     if (lane == 0) mbar_arrive(base + kPrBarQ);
@@ -410,7 +416,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
       tc_fence_after();
       const uint32_t par = base + Plan::params + stage * Plan::param_bytes + buf * (kPrStep * 16);
       const float unit_now = lds_f32(base + kPrUnit + 4 * stage);
-      const int j0 = range.block(t) * kPrTile + buf * kPrStep;
+      const int j0 = range.block(tile0 + t) * kPrTile + buf * kPrStep;
       const bool whole = j0 + kPrStep - 1 <= wg_lo && (p.window == 0 || j0 > wg_hi - p.window || j0 + kPrStep <= p.sinks);
       int hi[4];
 #pragma unroll
@@ -462,7 +468,15 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
 #pragma unroll
           for (int i = 0; i < 4; ++i) tmem_ld16(t_o + i * U + u0, o[i]);
         }
-        if (live) {
+        if (SPLIT) {  // for the join: four channels of all rows side by side
+#pragma unroll
+          for (int u = 0; u < 16; ++u) {
+            uint32_t x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = __float_as_uint(fmaf(__uint_as_float(o[i][u]), r.v_unit, fix));
+            if (half == 0) sts_v4(base + Plan::stages + ((u0 + u) * 128 + threadIdx.x) * 16, x[0], x[1], x[2], x[3]);
+          }
+        } else if (live) {
 #pragma unroll
           for (int u = 0; u < 16; u += 2) {
             uint32_t w[4];
@@ -478,7 +492,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
           }
         }
       }
-      if (tile_out != nullptr) kv4_row_numbers(tile_out + 128 * D * 2, quad * 32 + lane, unit, sum, live ? l : 0.f, lds_f32(my_row + 8));
+      if (tile_out != nullptr && !SPLIT) kv4_row_numbers(tile_out + 128 * D * 2, quad * 32 + lane, unit, sum, live ? l : 0.f, lds_f32(my_row + 8));
     }
   } else if (warp < kMma) {
     // ------------------------------------------------------------------ producers
@@ -492,7 +506,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
     uint2 par[E];
     const int unit_lane = lane & (U - 1), group0 = G * pw + (G == 2 ? lane >> 4 : 0);
     auto load = [&](int t) {
-      const int j0 = range.block(t) * kPrTile;
+      const int j0 = range.block(tile0 + t) * kPrTile;
 #pragma unroll
       for (int n = 0; n < E; ++n) {
         const int j = j0 + tid + n * kThreads;
@@ -634,6 +648,56 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
       if (!mbar_wait_chain(base + kPrBarEnd, 0)) failed = true;
       if (failed) report_status(kStatusMmaTimeout);
     }
+  }
+  if constexpr (SPLIT) {
+    // The cluster's sums of the same 128 rows, joined through distributed shared memory in the order of their tiles, each CTA a part of
+    // the channels.
+    __syncwarp();
+    cluster_sync_all();
+    if (warp < 8) {
+      const int of = threadIdx.x & 127, row = r0 + of, share = D / 4 / splits;
+      const uint32_t numbers = base + Plan::rows + of * 12;
+      float l[kPrSplits], f[kPrSplits], top = -INFINITY, norm = 0.f;
+#pragma unroll
+      for (int c = 0; c < kPrSplits; ++c) {
+        l[c] = 0.f, f[c] = -INFINITY;
+        if (c < splits) l[c] = ld_cluster_f32(map_to_cta(numbers, c)), f[c] = ld_cluster_f32(map_to_cta(numbers + 8, c));
+        if (l[c] != 0.f) top = fmaxf(top, f[c]);
+      }
+#pragma unroll
+      for (int c = 0; c < kPrSplits; ++c) {
+        if (l[c] == 0.f) continue;  // nothing seen
+        f[c] = exp2_approx(f[c] - top);
+        norm = fmaf(l[c], f[c], norm);
+      }
+      const float inv = norm == 0.f ? 0.f : 1.f / norm;  // a row that sees nothing: zeros
+      if (row < total) {
+        const int query = row / p.group;
+        uint16_t *out = p.out + ((static_cast<size_t>(b) * p.seq + query) * p.heads + static_cast<size_t>(h) * p.group + (row - query * p.group)) * D;
+        for (int ch = rank * share + (threadIdx.x >> 7); ch < (rank + 1) * share; ch += 2) {
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int c = 0; c < kPrSplits; ++c) {
+            if (l[c] == 0.f) continue;
+            const float4 x = ld_cluster_f32x4(map_to_cta(base + Plan::stages + (ch * 128 + of) * 16, c));
+            sum.x = fmaf(x.x, f[c], sum.x);
+            sum.y = fmaf(x.y, f[c], sum.y);
+            sum.z = fmaf(x.z, f[c], sum.z);
+            sum.w = fmaf(x.w, f[c], sum.w);
+          }
+          uint2 w;
+          w.x = kv4_bits<T>(sum.x * inv) | static_cast<uint32_t>(kv4_bits<T>(sum.y * inv)) << 16;
+          w.y = kv4_bits<T>(sum.z * inv) | static_cast<uint32_t>(kv4_bits<T>(sum.w * inv)) << 16;
+          *reinterpret_cast<uint2 *>(out + 4 * ch) = w;
+        }
+      }
+      if (p.row_tiles != nullptr && rank == 0 && threadIdx.x < 128) {
+        uint8_t *tile_out = p.row_tiles + (static_cast<size_t>(bh) * ((all_rows + 127) / 128) + (r0 >> 7)) * kv4_row_tile_bytes(D);
+        kv4_row_numbers(tile_out + 128 * D * 2, of, row_unit, row_sum, row < total ? norm : 0.f, top);
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();  // no CTA leaves while another reads its shared memory
   }
   tc_fence_before();
   __syncthreads();
@@ -881,24 +945,39 @@ template <typename T, int D> int launch_weights(const Kv4AttentionParams &p, cud
 
 template <typename T, int D> int launch_prompt(const Kv4AttentionParams &p, bool pdl, cudaStream_t stream) {
   constexpr int smem = PromptPlan<D>::end;
-  static SharedMemoryOptIn opt_in;
-  const int st = opt_in.ensure(kv4_prompt_kernel<T, D>, smem);
-  if (st != MG_OK) return st;
   cudaLaunchConfig_t cfg = {};
   const int heads = p.cache.batch * p.cache.kv_heads, all = p.seq * p.group;
   // Half as many rows a CTA while these run at once: a half alone takes 0.8 of the time of two.  1024 rows of 8 heads of 8192 entries
   // (64 CTAs) 140 us, with 256 rows 181; of 48 heads (384 CTAs) 413 and 358.
-  const int rows = static_cast<long long>(heads) * ((all + 127) / 128) <= kPrSms ? 128 : kPrRows;
-  cfg.gridDim = dim3(heads, (all + rows - 1) / rows);
+  const long long tiles = static_cast<long long>(heads) * ((all + 127) / 128);
+  const int rows = tiles <= kPrSms ? 128 : kPrRows;
+  // A cluster for the same rows where CTAs are fewer still, each with its share of the entries: 8192 entries of 8 heads, 1024 rows in
+  // clusters of 2 78.5 us, alone 140; 512 rows in clusters of 4 46.7, alone 140; 512 entries, 1024 rows 17.8 and 17.0.
+  int splits = 1;
+  while (splits < kPrSplits && tiles * splits * 2 <= cluster_ctas(kPrSms, splits * 2)) splits *= 2;
+  cfg.gridDim = dim3(heads * splits, (all + rows - 1) / rows);
   cfg.blockDim = dim3(kPrWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (splits > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = splits;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
-  if (cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, D>, p, rows) != cudaSuccess) return MG_ERR_CUDA;
+  cfg.numAttrs = n;
+  static SharedMemoryOptIn opt_in, opt_in_split;
+  const int st = splits > 1 ? opt_in_split.ensure(kv4_prompt_kernel<T, D, true>, smem) : opt_in.ensure(kv4_prompt_kernel<T, D, false>, smem);
+  if (st != MG_OK) return st;
+  const auto kernel = splits > 1 ? kv4_prompt_kernel<T, D, true> : kv4_prompt_kernel<T, D, false>;
+  if (cudaLaunchKernelEx(&cfg, kernel, p, rows, splits) != cudaSuccess) return MG_ERR_CUDA;
   return p.weights != nullptr ? launch_weights<T, D>(p, stream) : MG_OK;
 }
 

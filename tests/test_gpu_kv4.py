@@ -369,7 +369,8 @@ def test_strides_streams_and_empty_batches(cuda):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("b, seq, kv, group", [(20, 33, 5, 1), (5, 130, 3, 4), (3, 257, 4, 3), (10, 70, 2, 8), (1, 1200, 4, 1),
-                                               (8, 300, 10, 2), (19, 33, 8, 8), (160, 35, 1, 1)])
+                                               (8, 300, 10, 2), (19, 33, 8, 8), (160, 35, 1, 1),
+                                               (1, 700, 4, 1), (3, 100, 2, 5), (4, 130, 2, 4)])
 def test_attention_of_many_rows(cuda, dtype, d, b, seq, kv, group):
     """Prompts of which some are padded on the left (rows that see nothing), later pieces, sequences of one entry and of none."""
     lengths = ([seq, seq + 61, max(1, seq // 2), 0, 1, 129, seq + 200] * 23)[:b]
@@ -377,7 +378,7 @@ def test_attention_of_many_rows(cuda, dtype, d, b, seq, kv, group):
 
 
 @pytest.mark.parametrize("window, sinks", [(1, 0), (1, 3), (17, 1), (64, 0), (65, 64), (128, 129), (200, 4), (1000, 5), (0, 7)])
-@pytest.mark.parametrize("kv", [8, 20])  # few CTAs of 128 rows, more of 256
+@pytest.mark.parametrize("kv", [2, 5, 8, 20])  # clusters of four and of two that share the entries, CTAs of 128 rows, more of 256
 def test_attention_of_many_rows_with_a_window(cuda, window, sinks, kv):
     check_attention(cuda, torch.float16, 128, 4, 150, kv, 2, [450, 331, 150, 149], window, sinks, capacity=512, seed=window)
     check_attention(cuda, torch.bfloat16, 64, 4, 150, kv, 2, [450, 331, 20, 0], window, sinks, capacity=512, seed=window + 1)
@@ -385,12 +386,12 @@ def test_attention_of_many_rows_with_a_window(cuda, window, sinks, kv):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("q_size, v_size", [(30.0, 1.0), (1e-3, 1.0), (1.5, 1e-4), (1.5, 200.0), (0.0, 1.0)])
-@pytest.mark.parametrize("kv", [8, 26])
+@pytest.mark.parametrize("kv", [2, 4, 8, 26])
 def test_attention_of_large_and_small_values_in_many_rows(cuda, dtype, q_size, v_size, kv):
     check_attention(cuda, dtype, 128, 2, 160, kv, 2, [300, 160], q_size=q_size, v_size=v_size, seed=6)
 
 
-@pytest.mark.parametrize("kv", [8, 40])
+@pytest.mark.parametrize("kv", [4, 8, 40])
 def test_attention_of_many_rows_over_scales_that_vary_widely(cuda, kv):
     """As test_attention_of_scales_that_vary_widely; the unit of a tile's weights rises and what was added up follows it."""
     from matgptq_b200 import ops
@@ -405,7 +406,7 @@ def test_attention_of_many_rows_over_scales_that_vary_widely(cuda, kv):
     assert ((out.double() - want).abs() <= near * 1.01 + want.abs() * half_step(dtype) * 1.01).all()
 
 
-@pytest.mark.parametrize("b, group", [(64, 2), (100, 4)])
+@pytest.mark.parametrize("b, group", [(30, 3), (64, 2), (100, 4)])
 def test_nan_reaches_the_rows_that_see_it_among_many(cuda, b, group):
     """As test_nan_reaches_the_rows_that_see_it_and_no_others.  Beside a NaN the other rows keep their bits.  An infinite score makes its
     warp take all its rows' weights against new maxima: by whole powers of two, so with the same error bound, but the exponents
@@ -432,7 +433,7 @@ def test_nan_reaches_the_rows_that_see_it_among_many(cuda, b, group):
                 assert out[i].isnan().all(-1).all(-1).cpu().tolist() == seen.tolist(), (column, i)
 
 
-@pytest.mark.parametrize("group", [4, 8])
+@pytest.mark.parametrize("group", [1, 4, 8])
 def test_attention_of_many_rows_has_one_order(cuda, group):
     from matgptq_b200 import ops
     gen = torch.Generator(device=cuda).manual_seed(9)
