@@ -33,23 +33,12 @@ MG_DEFINE_STATUS_ACCESSOR(kv4_device_status)
 static __device__ __noinline__ float turned_exactly(float x, float a, float y, float b) {
   return static_cast<float>(static_cast<double>(x) * a + static_cast<double>(y) * b);
 }
-template <typename T> __device__ __forceinline__ uint32_t two_bits(float a, float b) {
-  return kv4_bits<T>(a) | static_cast<uint32_t>(kv4_bits<T>(b)) << 16;
-}
-template <> __device__ __forceinline__ uint32_t two_bits<__half>(float a, float b) {
-  const __half2 r = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t *>(&r);
-}
-template <> __device__ __forceinline__ uint32_t two_bits<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t *>(&r);
-}
 // the pair (x, y) turned by the angle of cosine c and sine s; `doubt` where 64 bits have to decide
 template <typename T> __device__ __forceinline__ uint32_t turned(float x, float y, float c, float s, bool &doubt) {
   const float p0 = __fmul_rn(y, -s), r0 = __fmaf_rn(x, c, p0), p1 = __fmul_rn(x, s), r1 = __fmaf_rn(y, c, p1);
   const float off0 = __fmaf_rn(0x1p-23f, fabsf(r0) + fabsf(p0), FLT_MIN), off1 = __fmaf_rn(0x1p-23f, fabsf(r1) + fabsf(p1), FLT_MIN);
-  const uint32_t low = two_bits<T>(r0 - off0, r1 - off1);
-  doubt |= low != two_bits<T>(r0 + off0, r1 + off1);
+  const uint32_t low = kv4_two_bits<T>(r0 - off0, r1 - off1);
+  doubt |= low != kv4_two_bits<T>(r0 + off0, r1 + off1);
   return low;
 }
 
@@ -161,8 +150,8 @@ __global__ void __launch_bounds__(256, 4) append_kv4_kernel(const T *__restrict_
         uint32_t pair[4] = {in[0], in[1], in[2], in[3]};
         if (row < heads) {
 #pragma unroll
-          for (int p = 0; p < 4; ++p) pair[p] = two_bits<T>(rotated_even(x(p), y(p), cv[p], sv[p]), rotated_odd(x(p), y(p), cv[p], sv[p]));
-          if (!placed && !padding) pair[0] = pair[1] = pair[2] = pair[3] = two_bits<T>(NAN, NAN);
+          for (int p = 0; p < 4; ++p) pair[p] = kv4_two_bits<T>(rotated_even(x(p), y(p), cv[p], sv[p]), rotated_odd(x(p), y(p), cv[p], sv[p]));
+          if (!placed && !padding) pair[0] = pair[1] = pair[2] = pair[3] = kv4_two_bits<T>(NAN, NAN);
           *reinterpret_cast<uint4 *>(dst + row * cache.dim) = make_uint4(pair[0], pair[1], pair[2], pair[3]);
         }
         if (__all_sync(0xffffffffu, row < heads || row >= all)) continue;  // nothing to quantise in this warp
@@ -174,9 +163,9 @@ __global__ void __launch_bounds__(256, 4) append_kv4_kernel(const T *__restrict_
           for (int p = 0; p < 4; ++p) pair[p] = turned<T>(x(p), y(p), cv[p], sv[p], doubt);
           if (doubt) {
 #pragma unroll
-            for (int p = 0; p < 4; ++p) pair[p] = two_bits<T>(turned_exactly(x(p), cv[p], y(p), -sv[p]), turned_exactly(y(p), cv[p], x(p), sv[p]));
+            for (int p = 0; p < 4; ++p) pair[p] = kv4_two_bits<T>(turned_exactly(x(p), cv[p], y(p), -sv[p]), turned_exactly(y(p), cv[p], x(p), sv[p]));
           }
-          if (!placed) pair[0] = pair[1] = pair[2] = pair[3] = two_bits<T>(NAN, NAN);
+          if (!placed) pair[0] = pair[1] = pair[2] = pair[3] = kv4_two_bits<T>(NAN, NAN);
         }
         const size_t entry = (static_cast<size_t>(b) * cache.kv_heads + (is_v ? kv - cache.kv_heads : max(kv, 0))) * cache.capacity + max(slot, 0);
         quantise_row<T>(pair, kv >= 0 && row < all && !padding && slot < cache.capacity, lanes, cache, entry, c0, is_v);

@@ -48,5 +48,15 @@ template <> __device__ __forceinline__ float kv4_to_f<__nv_bfloat16>(uint16_t v)
 template <typename T> __device__ __forceinline__ uint16_t kv4_bits(float v);
 template <> __device__ __forceinline__ uint16_t kv4_bits<__half>(float v) { return __half_as_ushort(__float2half_rn(v)); }
 template <> __device__ __forceinline__ uint16_t kv4_bits<__nv_bfloat16>(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+// two of them, the first in the low half, in one instruction
+template <typename T> __device__ __forceinline__ uint32_t kv4_two_bits(float a, float b);
+template <> __device__ __forceinline__ uint32_t kv4_two_bits<__half>(float a, float b) {
+  const __half2 r = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+template <> __device__ __forceinline__ uint32_t kv4_two_bits<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
 
 }  // namespace mg

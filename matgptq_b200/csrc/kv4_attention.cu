@@ -506,8 +506,8 @@ __global__ void __launch_bounds__(kStepWarps * 32, NT == 1 ? 2 : 1) kv4_step_ker
       const int q = row / p.group;
       const size_t at = ((static_cast<size_t>(b) * p.seq + q) * p.heads + static_cast<size_t>(h) * p.group + (row - q * p.group)) * D + (i % (D / 4)) * 4;
       uint2 w;
-      w.x = kv4_bits<T>(sum.x * inv) | static_cast<uint32_t>(kv4_bits<T>(sum.y * inv)) << 16;
-      w.y = kv4_bits<T>(sum.z * inv) | static_cast<uint32_t>(kv4_bits<T>(sum.w * inv)) << 16;
+      w.x = kv4_two_bits<T>(sum.x * inv, sum.y * inv);
+      w.y = kv4_two_bits<T>(sum.z * inv, sum.w * inv);
       *reinterpret_cast<uint2 *>(p.out + at) = w;
     }
   };
@@ -714,8 +714,8 @@ template <typename T, int D, int NT, int LANES> __global__ void __launch_bounds_
         const int q = row / p.group;
         const size_t at = ((static_cast<size_t>(b) * p.seq + q) * p.heads + static_cast<size_t>(h) * p.group + (row - q * p.group)) * D + (i % (D / 4)) * 4;
         uint2 w;
-        w.x = kv4_bits<T>(sum.x * inv) | static_cast<uint32_t>(kv4_bits<T>(sum.y * inv)) << 16;
-        w.y = kv4_bits<T>(sum.z * inv) | static_cast<uint32_t>(kv4_bits<T>(sum.w * inv)) << 16;
+        w.x = kv4_two_bits<T>(sum.x * inv, sum.y * inv);
+        w.y = kv4_two_bits<T>(sum.z * inv, sum.w * inv);
         *reinterpret_cast<uint2 *>(p.out + at) = w;
       }
     }

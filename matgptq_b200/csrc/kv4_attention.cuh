@@ -109,7 +109,7 @@ __host__ __device__ constexpr int kv4_row_tile_bytes(int dim) { return 128 * dim
 template <typename T, int D, typename Store>
 __device__ __forceinline__ void kv4_operand_row(const uint16_t *q, bool live, float scale_log2, float &unit, float &sum, Store store) {
   uint4 raw[D / 8];
-  float top = 0.f;
+  uint32_t top2 = 0;  // the largest magnitudes of the even and the odd channels, as bits
 #pragma unroll
   for (int c = 0; c < D / 8; ++c) {
     raw[c] = make_uint4(0, 0, 0, 0);
@@ -119,27 +119,31 @@ __device__ __forceinline__ void kv4_operand_row(const uint16_t *q, bool live, fl
   for (int c = 0; c < D / 8; ++c) {
     const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      top = fmaxf(top, fmaxf(fabsf(kv4_to_f<T>(static_cast<uint16_t>(u[i]))), fabsf(kv4_to_f<T>(static_cast<uint16_t>(u[i] >> 16)))));
+    for (int i = 0; i < 4; ++i) top2 = __vmaxu2(top2, u[i] & 0x7fff7fffu);
   }
+  const float top = kv4_to_f<T>(static_cast<uint16_t>(max(top2 & 0xffffu, top2 >> 16)));
   const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 16), 253);
   const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * (scale_log2 < 0.f ? -256.f : 256.f);
   // 2^24 / 2^8; never 0
   unit = fmaxf(__uint_as_float(static_cast<uint32_t>(e) << 23) * (fabsf(scale_log2) * 65536.f), FLT_MIN);
-  sum = 0.f;
+  float sums[2] = {0.f, 0.f};
+  const __half2 sixteenth = __floats2half2_rn(1.f, 0.0625f);
 #pragma unroll
   for (int c = 0; c < D / 8; ++c) {
     const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
-    uint32_t x[8];
+    uint32_t x[4];  // channels 2 i and 2 i + 1
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float v = kv4_to_f<T>(static_cast<uint16_t>(u[i >> 1] >> (16 * (i & 1)))) * down;
-      const __half q16 = __float2half_rn(v);
-      sum += __half2float(q16);
-      x[i] = __half_as_ushort(i & 1 ? __float2half_rn(__half2float(q16) * 0.0625f) : q16);
+    for (int i = 0; i < 4; ++i) {
+      const __half2 q16 = __floats2half2_rn(kv4_to_f<T>(static_cast<uint16_t>(u[i])) * down, kv4_to_f<T>(static_cast<uint16_t>(u[i] >> 16)) * down);
+      const float2 back = __half22float2(q16);
+      sums[0] += back.x;
+      sums[1] += back.y;
+      const __half2 scaled = __hmul2(q16, sixteenth);
+      x[i] = *reinterpret_cast<const uint32_t *>(&scaled);
     }
-    store(c, make_uint4(x[0] | x[4] << 16, x[1] | x[5] << 16, x[2] | x[6] << 16, x[3] | x[7] << 16));
+    store(c, make_uint4(__byte_perm(x[0], x[2], 0x5410), __byte_perm(x[0], x[2], 0x7632), __byte_perm(x[1], x[3], 0x5410), __byte_perm(x[1], x[3], 0x7632)));
   }
+  sum = sums[0] + sums[1];
   sum *= 0x1p-24f;
 }
 

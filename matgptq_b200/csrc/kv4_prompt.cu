@@ -50,16 +50,12 @@ template <int D> struct PromptPlan {
   static constexpr int end = rows + kPrRows * 12;
 };
 
-// 32 columns of this warp's 32 lanes of tensor memory, and back; the caller waits
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *v) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
-      "%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
-        "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
-        "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]),
-        "=r"(v[31])
-      : "r"(taddr));
+// 16 columns of this warp's 32 lanes of tensor memory; the caller waits
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+                 "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+               : "r"(taddr));
 }
 // 32 columns of 16 lanes: a lane (g, t) has of row g the columns 8 i + 2 t and + 1 in v[4 i] and v[4 i + 1], of row g + 8 in v[4 i + 2]
 // and v[4 i + 3]; the caller waits
@@ -466,7 +462,8 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
         uint32_t o[4][16];
         if (tiles > 0) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) tmem_ld16(t_o + i * U + u0, o[i]);
+          for (int i = 0; i < 4; ++i) tmem_ld_32x16(t_o + i * U + u0, o[i]);
+          tmem_wait_ld();
         }
         if (SPLIT) {  // for the join: four channels of all rows side by side
 #pragma unroll
@@ -482,11 +479,11 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
             uint32_t w[4];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              uint16_t c[4];
+              float c[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) c[i] = kv4_bits<T>(l == 0.f ? 0.f : fmaf(__uint_as_float(o[i][u + k]), r.v_unit, fix) * inv);
-              w[2 * k] = c[0] | static_cast<uint32_t>(c[1]) << 16;
-              w[2 * k + 1] = c[2] | static_cast<uint32_t>(c[3]) << 16;
+              for (int i = 0; i < 4; ++i) c[i] = l == 0.f ? 0.f : fmaf(__uint_as_float(o[i][u + k]), r.v_unit, fix) * inv;
+              w[2 * k] = kv4_two_bits<T>(c[0], c[1]);
+              w[2 * k + 1] = kv4_two_bits<T>(c[2], c[3]);
             }
             *reinterpret_cast<uint4 *>(p.out + out_at + 4 * (u0 + u)) = make_uint4(w[0], w[1], w[2], w[3]);
           }
@@ -686,8 +683,8 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
             sum.w = fmaf(x.w, f[c], sum.w);
           }
           uint2 w;
-          w.x = kv4_bits<T>(sum.x * inv) | static_cast<uint32_t>(kv4_bits<T>(sum.y * inv)) << 16;
-          w.y = kv4_bits<T>(sum.z * inv) | static_cast<uint32_t>(kv4_bits<T>(sum.w * inv)) << 16;
+          w.x = kv4_two_bits<T>(sum.x * inv, sum.y * inv);
+          w.y = kv4_two_bits<T>(sum.z * inv, sum.w * inv);
           *reinterpret_cast<uint2 *>(out + 4 * ch) = w;
         }
       }
