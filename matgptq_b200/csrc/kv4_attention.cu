@@ -781,14 +781,21 @@ template <typename T, int D> __global__ void __launch_bounds__(128) kv4_row_tile
   pdl_prologue();
   const Kv4AttentionParams &p = sp.a;
   const int kv = p.cache.kv_heads, total = p.seq * p.group, b = blockIdx.y / kv, h = blockIdx.y - b * kv;
-  const int row = blockIdx.x * 128 + threadIdx.x, query = row / p.group;
+  const int row = blockIdx.x * 128 + threadIdx.x, row0 = blockIdx.x * 128 + (threadIdx.x & ~31);
   const bool live = row < total;
   uint8_t *tile = p.row_tiles + (static_cast<size_t>(blockIdx.y) * gridDim.x + blockIdx.x) * kv4_row_tile_bytes(D);
-  float unit, sum, l = 0.f, m = -INFINITY;
-  const size_t at = ((static_cast<size_t>(b) * p.seq + query) * p.heads + static_cast<size_t>(h) * p.group + (row - query * p.group)) * D;
-  kv4_operand_row<T, D>(p.q + at, live, p.scale_log2, unit, sum, [&](int c, const uint4 &chunk) {
-    *reinterpret_cast<uint4 *>(tile + c * (128 * 16) + threadIdx.x * 16) = chunk;
-  });
+  __shared__ float2 unit_sum[128];
+  float l = 0.f, m = -INFINITY;
+  const auto at = [&](int of) -> const uint16_t * {
+    const int r = row0 + of, query = r / p.group;
+    if (r >= total) return nullptr;
+    return p.q + ((static_cast<size_t>(b) * p.seq + query) * p.heads + static_cast<size_t>(h) * p.group + (r - query * p.group)) * D;
+  };
+  kv4_operand_rows<T, D>(
+      p.scale_log2, at,
+      [&](int of, int c, const uint4 &chunk) { *reinterpret_cast<uint4 *>(tile + c * (128 * 16) + ((threadIdx.x & ~31) + of) * 16) = chunk; },
+      [&](int of, float unit, float sum) { unit_sum[(threadIdx.x & ~31) + of] = make_float2(unit, sum); });
+  __syncwarp();
   if (live) {
     const int segment = (b * sp.tiles + row / R) * kv + h, r = row % R;
     int2 of = make_int2(segment, 1);
@@ -802,7 +809,7 @@ template <typename T, int D> __global__ void __launch_bounds__(128) kv4_row_tile
       m = top;
     }
   }
-  kv4_row_numbers(tile + 128 * D * 2, threadIdx.x, unit, sum, l, m);
+  kv4_row_numbers(tile + 128 * D * 2, threadIdx.x, unit_sum[threadIdx.x].x, unit_sum[threadIdx.x].y, l, m);
 }
 
 namespace {

@@ -13,10 +13,11 @@
 // (fp16 holds P until then and well beyond), which after the first tiles is rare.  Fp32 work goes two numbers an instruction.
 //
 // What bounds it: a step of 64 entries takes 2400 cycles, 1024 of them exponentials (16 a cycle and SM), 1300 MMAs; the softmax warps
-// never wait for S, two of them on a scheduler do not cover each other's latencies, and a half alone still takes 1900.  2048 tokens of 32
-// heads, 8 key/value heads, 128 channels, causal: 64.5 us, 533 TFLOP/s.  Measured and taken back: 16 softmax warps of 16 rows (scales
-// and minima pass through shared memory twice as often: 68.3), tiles that come by bulk copies instead of loads (65.3, with 16 warps
-// 71.7), masks without the guard against NaN where a tile has none (64.7; with a window 91.6 for 93), steps of 128 with one buffer (69).
+// never wait for S, two of them on a scheduler do not cover each other's latencies, and a half alone still takes 1900.  Around the steps a
+// CTA takes 18000 cycles, 8000 for q and 6000 for the results.  2048 tokens of 32 heads, 8 key/value heads, 128 channels, causal: 61.5 us,
+// 559 TFLOP/s.  Measured and taken back, at 64.5: 16 softmax warps of 16 rows (scales and minima pass through shared memory twice as
+// often: 68.3), tiles that come by bulk copies instead of loads (65.3, with 16 warps 71.7), masks without the guard against NaN where a
+// tile has none (64.7; with a window 91.6 for 93), steps of 128 with one buffer (69).
 // Every mbarrier wait is bounded; a warp that gives up hands nothing on, so that the others give up in turn; the issuing warp stays until
 // its MMAs have ended and tensor memory is freed on every path.
 #include <cuda_runtime.h>
@@ -50,12 +51,9 @@ template <int D> struct PromptPlan {
   static constexpr int end = rows + kPrRows * 12;
 };
 
-// 16 columns of this warp's 32 lanes of tensor memory; the caller waits
-__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&v)[16]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-                 "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-               : "r"(taddr));
+// 4 columns of this warp's 32 lanes of tensor memory; the caller waits
+__device__ __forceinline__ void tmem_ld_32x4(uint32_t taddr, uint32_t (&v)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(taddr));
 }
 // 32 columns of 16 lanes: a lane (g, t) has of row g the columns 8 i + 2 t and + 1 in v[4 i] and v[4 i + 1], of row g + 8 in v[4 i + 2]
 // and v[4 i + 3]; the caller waits
@@ -106,6 +104,9 @@ __device__ __forceinline__ float lds_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
+}
+__device__ __forceinline__ void lds_v4(uint32_t (&v)[4], uint32_t addr) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void lds_2x64(uint32_t addr, uint64_t &a, uint64_t &b) {
   asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(addr) : "memory");
@@ -358,35 +359,41 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
   float row_unit = 0.f, row_sum = 0.f;  // of this thread's row
 
   if (warp < kProducer) {
-    // ------------------------------------------------------------------ softmax: a thread per row
+    // ------------------------------------------------------------------ softmax
     const int half = warp >> 2, quad = warp & 3;
-    const int row = r0 + threadIdx.x;  // of the key/value head
-    const bool live = row < total;
-    const int query = live ? row / p.group : 0;
+    const bool live = r0 + static_cast<int>(threadIdx.x) < total;
     const int wg_lo = length - p.seq + (r0 + half * 128) / p.group;                                  // of this half's rows
     const int wg_hi = length - p.seq + (min(r0 + half * 128 + 128, total) - 1) / p.group;
-    const size_t out_at = ((static_cast<size_t>(b) * p.seq + query) * p.heads + static_cast<size_t>(h) * p.group + (live ? row - query * p.group : 0)) * D;
     // this row's tile for the pass that adds up the weights, where there is one
     uint8_t *tile_out = nullptr;
     if (p.row_tiles != nullptr && rank == 0 && r0 + half * 128 < total)
       tile_out = p.row_tiles + (static_cast<size_t>(bh) * ((all_rows + 127) / 128) + (r0 >> 7) + half) * kv4_row_tile_bytes(D);
-    float unit, sum;
-    const uint32_t q_at = (quad * 32 + lane) * 16, dst = base + Plan::q + half * Plan::q_bytes + q_at;
-    kv4_operand_row<T, D>(p.q + out_at, live, p.scale_log2, unit, sum, [&](int c, const uint4 &chunk) {
-      sts_v4(dst + c * kChunkQ, chunk.x, chunk.y, chunk.z, chunk.w);
-      if (tile_out != nullptr) *reinterpret_cast<uint4 *>(tile_out + c * kChunkQ + q_at) = chunk;
-    });
-    row_unit = unit, row_sum = sum;
+    const uint32_t warp_rows = base + Plan::rows + warp * 32 * 12, my_row = warp_rows + lane * 12, q_at = base + Plan::q + half * Plan::q_bytes;
+    const auto at = [&](int of) -> const uint16_t * {
+      const int i = r0 + warp * 32 + of, query = i / p.group;
+      if (i >= total) return nullptr;
+      return p.q + ((static_cast<size_t>(b) * p.seq + query) * p.heads + static_cast<size_t>(h) * p.group + (i - query * p.group)) * D;
+    };
+    kv4_operand_rows<T, D>(
+        p.scale_log2, at,
+        [&](int of, int c, const uint4 &chunk) {
+          const uint32_t to = c * kChunkQ + (quad * 32 + of) * 16;
+          sts_v4(q_at + to, chunk.x, chunk.y, chunk.z, chunk.w);
+          if (tile_out != nullptr) *reinterpret_cast<uint4 *>(tile_out + to) = chunk;
+        },
+        [&](int of, float unit, float sum) {
+          sts_f32(warp_rows + of * 12, unit);
+          sts_f32(warp_rows + of * 12 + 4, sum);
+        });
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     if (lane == 0) mbar_arrive(base + kPrBarQ);
 
     const uint32_t t_s0 = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * 128;
     const uint32_t t_o = tmem + (static_cast<uint32_t>(quad * 32) << 16) + 256 + half * D;
-    // from here on a lane has four rows: their numbers go through shared memory
-    const uint32_t warp_rows = base + Plan::rows + warp * 32 * 12, my_row = warp_rows + lane * 12;
-    sts_f32(my_row, unit);
-    sts_f32(my_row + 4, sum);
+    // from here on a lane has four rows
+    const float unit = lds_f32(my_row), sum = lds_f32(my_row + 4);
+    row_unit = unit, row_sum = sum;
     __syncwarp();
     PromptRows r;
     int row_pos[4];
@@ -457,25 +464,25 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
       const float l = lds_f32(my_row), fix = lds_f32(my_row + 4), inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
       // column i D/4 + u of the accumulator is channel 4 u + i
       constexpr int U = D / 4;
-#pragma unroll
-      for (int u0 = 0; u0 < U; u0 += 16) {
-        uint32_t o[4][16];
+#pragma unroll 1
+      for (int u0 = 0; u0 < U; u0 += 4) {  // (unrolled, a CTA waits for its instructions)
+        uint32_t o[4][4];
         if (tiles > 0) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) tmem_ld_32x16(t_o + i * U + u0, o[i]);
+          for (int i = 0; i < 4; ++i) tmem_ld_32x4(t_o + i * U + u0, o[i]);
           tmem_wait_ld();
         }
         if (SPLIT) {  // for the join: four channels of all rows side by side
 #pragma unroll
-          for (int u = 0; u < 16; ++u) {
+          for (int u = 0; u < 4; ++u) {
             uint32_t x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = __float_as_uint(fmaf(__uint_as_float(o[i][u]), r.v_unit, fix));
             if (half == 0) sts_v4(base + Plan::stages + ((u0 + u) * 128 + threadIdx.x) * 16, x[0], x[1], x[2], x[3]);
           }
-        } else if (live) {
+        } else {  // 16 bytes of all rows side by side, in the stages, which are done with
 #pragma unroll
-          for (int u = 0; u < 16; u += 2) {
+          for (int u = 0; u < 4; u += 2) {
             uint32_t w[4];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -485,7 +492,22 @@ __global__ void __launch_bounds__(kPrWarps * 32, 1) kv4_prompt_kernel(const Kv4A
               w[2 * k] = kv4_two_bits<T>(c[0], c[1]);
               w[2 * k + 1] = kv4_two_bits<T>(c[2], c[3]);
             }
-            *reinterpret_cast<uint4 *>(p.out + out_at + 4 * (u0 + u)) = make_uint4(w[0], w[1], w[2], w[3]);
+            sts_v4(base + Plan::stages + (((u0 + u) >> 1) * kPrRows + threadIdx.x) * 16, w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      if (!SPLIT) {  // out with them as q came in
+        __syncwarp();
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k) {
+          const int i = r0 + warp * 32 + (lane & 7) + 8 * k, query = i / p.group;
+          if (i >= total) continue;
+          uint16_t *out = p.out + ((static_cast<size_t>(b) * p.seq + query) * p.heads + static_cast<size_t>(h) * p.group + (i - query * p.group)) * D;
+#pragma unroll
+          for (int c = lane >> 3; c < D / 8; c += 4) {
+            uint32_t w[4];
+            lds_v4(w, base + Plan::stages + (c * kPrRows + (i - r0)) * 16);
+            *reinterpret_cast<uint4 *>(out + 8 * c) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
       }
