@@ -107,8 +107,7 @@ __host__ __device__ constexpr int kv4_row_tile_bytes(int dim) { return 128 * dim
 // that the largest value lies in [2^8, 2^9), which leaves the odd channels their bits when they are divided by 16.  numbers(row, unit,
 // sum), by one lane: log2 of a weight per score, and the sum of the scaled values in units of a code.  at(row): the row's values, or
 // null.  A lane has a quarter of the channels of rows lane & 7, + 8, + 16 and + 24, so that eight lanes write 128 bytes side by side and
-// four read 64.  (A row each, unrolled: 8500
-// cycles for 256 rows of 128 channels; as here 8000, and a prompt of 2048 tokens 0.5 us less.)
+// four read 64.  (A row each, unrolled: 8500 cycles for 256 rows of 128 channels; as here 8000, and a prompt of 2048 tokens 0.5 us less.)
 template <typename T, int D, typename At, typename Store, typename Numbers>
 __device__ __forceinline__ void kv4_operand_rows(float scale_log2, At at, Store store, Numbers numbers) {
   constexpr int C = D / 32;  // 16 bytes of each row
